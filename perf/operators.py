@@ -1,5 +1,6 @@
 """Cases of the sequence-layer operators: a short causal convolution and a selective state-space scan, for whole prompts
-(forward, and training with its gradients) and for single tokens, and the global gradient norm with clipping.
+(forward, and training with its gradients) and for single tokens, the projections around them (a matrix product with bias,
+activation and residual in one pass), and the global gradient norm with clipping.
 
 ``own = False`` computes every case in plain torch operations; ``own = True`` makes the calls a user of the framework
 makes (``audiofakedetect.ops``).  Tensors are [batch, time, channels]; parameters of the layers are fp32, activations
@@ -36,10 +37,6 @@ def listed():
         # a training batch of long recordings
         dict(name="conv_train_long_bf16", op="conv", train=True, dtype="bf16", B=4, L=4096, D=2048, W=4, bias=True,
              act="silu", lengths=False, state=False),
-        # one live stream, one frame: latency is all that counts
-        dict(name="conv_step_one_fp32", op="conv_step", dtype="fp32", B=1, D=1024, W=4, bias=True, act="silu"),
-        # many live streams at once
-        dict(name="conv_step_many_bf16", op="conv_step", dtype="bf16", B=512, D=2048, W=4, bias=True, act="silu"),
         # the training batch of the detector: 128 one-second clips of 101 frames, fp32, twice the LCNN's 512 features
         dict(name="scan_train_frames_fp32", op="scan", train=True, dtype="fp32", B=128, L=101, D=1024, N=16, gate=True,
              lengths=False, state=False),
@@ -52,10 +49,17 @@ def listed():
         # one very long recording: too few rows to fill the card, the time axis has to be split
         dict(name="scan_prompt_long_bf16", op="scan", train=False, dtype="bf16", B=1, L=16384, D=1024, N=16, gate=True,
              lengths=False, state=False),
-        # one live stream, one frame
-        dict(name="scan_step_one_fp32", op="scan_step", dtype="fp32", B=1, D=1024, N=16, gate=True),
         # many live streams at once: the states are what is read and written
         dict(name="scan_step_many_bf16", op="scan_step", dtype="bf16", B=512, D=2048, N=16, gate=True),
+        # the projection into such a layer, trained on 128 clips of 101 frames: 512 features in, 1024 out
+        dict(name="linear_train_frames_fp32", op="linear", train=True, dtype="fp32", M=12928, K=512, N=1024, bias=True,
+             act="silu", residual=False),
+        # a projection onto a residual stream, trained on long recordings
+        dict(name="linear_train_long_bf16", op="linear", train=True, dtype="bf16", M=16384, K=2048, N=2048, bias=True,
+             act="gelu", residual=True),
+        # one frame of a few live streams: the weights are what is read
+        dict(name="linear_step_bf16", op="linear", train=False, dtype="bf16", M=5, K=2048, N=4096, bias=True, act="silu",
+             residual=False),
         # gradients of a small detector: few elements in many tensors, launches count
         dict(name="clip_small_fp32", op="clip", dtype="fp32", tensors=48, total=1000003),
         # gradients of a large model
@@ -68,7 +72,7 @@ def _log(rng, lo, hi):
 
 
 def draw(rng):
-    op = rng.choice(["conv", "conv_step", "scan", "scan", "scan_step", "clip", "norm"])
+    op = rng.choice(["conv", "conv_step", "scan", "scan", "scan_step", "linear", "linear", "clip", "norm"])
     dtype = rng.choice(["fp32", "bf16", "fp16"])
     if op == "conv":
         while True:
@@ -86,6 +90,15 @@ def draw(rng):
                      D=_log(rng, 64, 2500), N=rng.choice([4, 8, 16, 16, 16, 13, 32, 64]), gate=rng.random() < 0.7,
                      lengths=rng.random() < 0.4, state=rng.random() < 0.4)
             if 50000 <= c["B"] * c["L"] * c["D"] and c["B"] * c["L"] * c["D"] * c["N"] <= 4 * 4096 * 2048 * 16:
+                return c
+    if op == "linear":
+        while True:
+            c = dict(op=op, train=rng.random() < 0.5, dtype=dtype, M=_log(rng, 1, 16384), K=_log(rng, 16, 4096),
+                     N=_log(rng, 16, 4096), bias=rng.random() < 0.7, act=rng.choice(["none", "relu", "silu", "gelu"]),
+                     residual=rng.random() < 0.4)
+            if rng.random() < 0.7:  # widths are mostly multiples of 8, but not all
+                c["K"], c["N"] = (c["K"] + 7) // 8 * 8, (c["N"] + 7) // 8 * 8
+            if 100000 <= c["M"] * c["K"] * c["N"] <= 16384 * 2048 * 2048:
                 return c
     if op == "scan_step":
         return dict(op=op, dtype=dtype, B=_log(rng, 1, 512), D=_log(rng, 64, 2048), N=rng.choice([4, 8, 13, 16, 16]),
@@ -149,6 +162,17 @@ def prepare(case, seed):
             s["dy"] = torch.randn(rows + (case["D"],), generator=g, device=_DEVICE).to(t)
             names = ["x", "w", "b"] if case["op"] == "conv" else ["x", "dt", "a", "b", "c", "d", "gate", "dt_bias"]
             s["leaves"] = [k for k in names + ["state"] if s[k] is not None]
+            for k in s["leaves"]:
+                s[k].requires_grad_(True)
+    elif op == "linear":
+        M, K, N = case["M"], case["K"], case["N"]
+        s["x"] = torch.randn((M, K), generator=g, device=_DEVICE).to(t)
+        s["w"] = (torch.randn((N, K), generator=g, device=_DEVICE) / math.sqrt(K)).to(t)
+        s["b"] = 0.1 * torch.randn((N,), generator=g, device=_DEVICE) if case["bias"] else None
+        s["residual"] = torch.randn((M, N), generator=g, device=_DEVICE).to(t) if case["residual"] else None
+        if case["train"]:
+            s["dy"] = torch.randn((M, N), generator=g, device=_DEVICE).to(t)
+            s["leaves"] = [k for k in ("x", "w", "b", "residual") if s[k] is not None]
             for k in s["leaves"]:
                 s[k].requires_grad_(True)
     elif case["op"] == "conv_step":
@@ -238,6 +262,14 @@ def _plain(s):
     elif op == "scan":
         y, st = _plain_scan(s["x"], s["dt"], s["a"], s["b"], s["c"], s["d"], s["gate"], s["dt_bias"], s["state"],
                             s["lengths"])
+    elif op == "linear":
+        z = s["x"].float() @ s["w"].float().t()
+        z = z + s["b"].float() if s["b"] is not None else z
+        act = case["act"]
+        y = (_silu(z) if act == "silu" else torch.clamp(z, min=0) if act == "relu"
+             else 0.5 * z * (1 + torch.erf(z * math.sqrt(0.5))) if act == "gelu" else z)
+        y = (y + s["residual"].float() if s["residual"] is not None else y).to(s["x"].dtype)
+        st = None
     elif op == "conv_step":
         full = torch.cat([s["state"].float(), s["x"].float()[:, None]], dim=1)
         z = (full * s["w"].float().t()).sum(1)
@@ -263,7 +295,7 @@ def _plain(s):
         return norm.float(), s["flat"]
     if case["train"]:
         return (y.detach(), *torch.autograd.grad(y, [s[k] for k in s["leaves"]], s["dy"]))
-    return y, st
+    return (y, st) if st is not None else y
 
 
 def _framework(s):
@@ -276,6 +308,8 @@ def _framework(s):
     elif op == "scan":
         y = ops.state_scan(s["x"], s["dt"], s["a"], s["b"], s["c"], d=s["d"], gate=s["gate"], dt_bias=s["dt_bias"],
                            softplus=True, state=s["state"], lengths=s["lengths"], return_state=not case["train"])
+    elif op == "linear":
+        y = ops.linear(s["x"], s["w"], s["b"], case["act"], residual=s["residual"])
     elif op == "conv_step":
         return ops.causal_conv_step(s["x"], s["state"], s["w"], s["b"], case["act"],
                                     state_out=s["state_out"]), s["state_out"]
@@ -300,6 +334,11 @@ def work(case):
     op, e = case["op"], _SIZE[case["dtype"]]
     if op in ("clip", "norm"):
         return {"bytes": float((2 if op == "clip" else 1) * e * case["total"]), "flops": 3.0 * case["total"]}
+    if op == "linear":
+        M, K, N = case["M"], case["K"], case["N"]
+        if case["train"]:  # x, w, residual, dy in; y, dx, dw and the residual's gradient out
+            return {"bytes": float(e * (2 * M * K + 2 * N * K + (2 + 2 * case["residual"]) * M * N)), "flops": 6.0 * M * N * K}
+        return {"bytes": float(e * (M * K + N * K + (1 + case["residual"]) * M * N)), "flops": 2.0 * M * N * K}
     rows = case["B"] * case.get("L", 1)
     D = case["D"]
     if op in ("conv", "conv_step"):
@@ -358,6 +397,24 @@ def _exact_conv(s):
         dfull[:, j:j + L] += dz * w[:, j]
         dw[:, j] = (dz * full[:, j:j + L]).sum((0, 1))
     got = {"x": dfull[:, W - 1:] * live, "w": dw, "b": dz.sum((0, 1)), "state": dfull[:, :W - 1]}
+    return (y, *[got[k] for k in s["leaves"]])
+
+
+def _exact_linear(s):
+    case = s["case"]
+    x, w = s["x"].detach().double(), s["w"].detach().double()
+    z = torch.nn.functional.linear(x, w, s["b"].detach().double() if s["b"] is not None else None)
+    sg, cdf = _sig(z), 0.5 * torch.erfc(-z * math.sqrt(0.5))
+    y, slope = {"none": (z, torch.ones_like(z)), "relu": (torch.relu(z), (z > 0).double()),
+                "silu": (z * sg, sg + z * sg * (1 - sg)),
+                "gelu": (z * cdf, cdf + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi))}[case["act"]]
+    if s["residual"] is not None:
+        y = y + s["residual"].detach().double()
+    if not case["train"]:
+        return y
+    dy = s["dy"].double()
+    dz = dy * slope
+    got = {"x": dz @ w, "w": dz.t() @ x, "b": dz.sum(0), "residual": dy}
     return (y, *[got[k] for k in s["leaves"]])
 
 
@@ -436,6 +493,8 @@ def exact(case, seed):
             return _exact_conv(s)
         if op == "scan":
             return _exact_scan(s)
+        if op == "linear":
+            return _exact_linear(s)
         if op == "conv_step":
             taps = torch.cat([s["state"].double(), s["x"].double()[:, None]], 1)
             z = torch.einsum("bwd,dw->bd", taps, s["w"].double())
