@@ -135,6 +135,22 @@ _SIGNATURES = {
     "afd_lstm_cell_backward": (c_i, [c_p, c_p, c_p, c_p, c_i, c_p, c_p, c_i, c_i, c_p]),
     "afd_cross_entropy": (c_i, [c_p, c_p, c_p, c_p, c_p, c_i, c_i, c_p]),
     "afd_adam_step": (c_i, [c_p, c_p, c_p, c_p, c_sz, c_f, c_f, c_f, c_f, c_f, c_i, c_f, c_p]),
+    "afd_adam_step_clipped": (c_i, [c_p, c_p, c_p, c_p, c_sz, c_f, c_f, c_f, c_f, c_f, c_i, c_p, c_p]),
+    "afd_global_norm_workspace_bytes": (c_sz, [ctypes.POINTER(c_l), c_i]),
+    "afd_global_norm": (c_i, [ctypes.POINTER(c_p), ctypes.POINTER(c_l), ctypes.POINTER(c_i), c_i, c_i, c_f, c_f, c_p, c_p,
+                              c_sz, c_p]),
+    "afd_multi_scale": (c_i, [ctypes.POINTER(c_p), ctypes.POINTER(c_p), ctypes.POINTER(c_l), ctypes.POINTER(c_i), c_i, c_p,
+                              c_p]),
+    "afd_causal_conv_forward": (c_i, [c_p, c_l, c_l, c_p, c_p, c_i, c_p, c_p, c_p, c_p] + [c_i] * 6 + [c_p]),
+    "afd_causal_conv_backward_workspace_bytes": (c_sz, [c_i] * 4),
+    "afd_causal_conv_backward": (c_i, [c_p, c_l, c_l, c_p, c_p, c_i, c_p, c_p, c_p, c_l, c_l] + [c_p] * 5 + [c_i] * 6
+                                 + [c_p, c_sz, c_p]),
+    "afd_causal_conv_step": (c_i, [c_p, c_l, c_p, c_p, c_i, c_p, c_p, c_p] + [c_i] * 5 + [c_p]),
+    "afd_state_scan_workspace_bytes": (c_sz, [c_i] * 5),
+    "afd_state_scan_checkpoint_floats": (c_sz, [c_i] * 4),
+    "afd_state_scan_forward": (c_i, [c_p] * 5 + [ctypes.POINTER(c_l)] + [c_p] * 8 + [c_i] * 6 + [c_p, c_sz, c_p]),
+    "afd_state_scan_backward": (c_i, [c_p] * 6 + [ctypes.POINTER(c_l)] + [c_p] * 15 + [c_i] * 6 + [c_p, c_sz, c_p]),
+    "afd_state_scan_step": (c_i, [c_p] * 5 + [ctypes.POINTER(c_l)] + [c_p] * 6 + [c_i] * 5 + [c_p]),
 }
 
 
@@ -189,7 +205,7 @@ def float_array(vals):
 
 KERNEL_CLASSES = {"wpt": 0, "conv_igemm": 1, "conv_wgrad": 2, "stft": 3, "conv_direct": 4,
                   "conv_winograd": 5, "conv_wgrad_1x1": 6, "lcnn_bf16": 7, "conv_first": 8, "batchnorm": 9,
-                  "elementwise": 10, "conv1x1": 11}
+                  "elementwise": 10, "conv1x1": 11, "sequence": 12}
 
 
 def timing_enable(on: bool) -> None:

@@ -1482,6 +1482,446 @@ class CrossEntropyLoss(torch.nn.Module):
 
 
 # --------------------------------------------------------------------------------------
+# Sequence layers: a short causal convolution and a selective state-space scan over [batch, time, channels] tensors, the
+# causal counterpart of the bidirectional LSTM layers (lcnn.py).  Whole sequences are differentiable; the `_step` forms take
+# one time step and continue the state that `return_state` left.
+_SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTIVATIONS = {"none": 0, "silu": 1}
+
+
+def _need(ok: bool, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+def _seq_input(what: str, x, ndim: int) -> None:
+    """The tensor that fixes type, device and sizes of a call."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{what}: x is a {type(x).__name__}, not a tensor")
+    _need(x.dim() == ndim, f"{what}: x has {x.dim()} dimensions, {ndim} expected")
+    if x.dtype not in _SEQ_DTYPES:
+        raise TypeError(f"{what}: x is {x.dtype}; float32, bfloat16 or float16 expected")
+
+
+def _seq_check(what: str, name: str, t, shape, dtype, device) -> None:
+    if t is None:
+        return
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: {name} is a {type(t).__name__}, not a tensor")
+    _need(tuple(t.shape) == tuple(shape), f"{what}: {name} has shape {tuple(t.shape)}, {tuple(shape)} expected")
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: {name} is {t.dtype}, {dtype} expected")
+    _need(t.device == device, f"{what}: {name} is on {t.device}, x on {device}")
+
+
+def _seq_gpu(what: str, x) -> None:
+    if not x.is_cuda:
+        raise RuntimeError(f"{what}: tensors on {x.device}; there is no CPU path")
+
+
+class _OnDevice:
+    """Launches go to the device of the tensors, whatever the current one is."""
+
+    def __init__(self, t: torch.Tensor) -> None:
+        i = t.device.index
+        self.guard = torch.cuda.device(i) if i != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """`t` with a contiguous last axis (batch and row strides are free)."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _seq_lengths(what: str, lengths, x) -> Optional[torch.Tensor]:
+    if lengths is None:
+        return None
+    if not isinstance(lengths, torch.Tensor) or lengths.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: lengths has to be an int32 or int64 tensor")
+    _need(tuple(lengths.shape) == (x.shape[0],), f"{what}: lengths has shape {tuple(lengths.shape)}, ({x.shape[0]},) expected")
+    _need(lengths.device == x.device, f"{what}: lengths is on {lengths.device}, x on {x.device}")
+    if lengths.dtype == torch.int64:
+        lengths = lengths.clamp(0, x.shape[1]).to(torch.int32)
+    return _dense(lengths)
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _step_state(what: str, state, state_out, tensors) -> torch.Tensor:
+    """The tensor a step writes its state to: `state` itself, or `state_out`, which may not overlap it otherwise."""
+    if _wants_grad(*tensors):
+        raise RuntimeError(f"{what}: single steps have no backward pass: call it under torch.no_grad() (the whole-sequence "
+                           "form is differentiable)")
+    _need(state.is_contiguous(), f"{what}: state has to be contiguous (it is updated in place)")
+    if state_out is None:
+        return state
+    _seq_check(what, "state_out", state_out, state.shape, state.dtype, state.device)
+    _need(state_out.is_contiguous(), f"{what}: state_out has to be contiguous")
+    p, q, n = state.data_ptr(), state_out.data_ptr(), state.numel() * state.element_size()
+    _need(p == q or p + n <= q or q + n <= p, f"{what}: state_out overlaps state without being it")
+    return state_out
+
+
+def _conv_check(what: str, x, w, b, activation, ndim: int):
+    _seq_input(what, x, ndim)
+    if not isinstance(w, torch.Tensor):
+        raise TypeError(f"{what}: w is a {type(w).__name__}, not a tensor")
+    _need(w.dim() == 2 and w.shape[0] == x.shape[-1], f"{what}: w has shape {tuple(w.shape)}, ({x.shape[-1]}, taps) expected")
+    _need(2 <= w.shape[1] <= 8, f"{what}: {w.shape[1]} taps; 2 to 8 are supported")
+    if w.dtype not in (torch.float32, x.dtype):
+        raise TypeError(f"{what}: w is {w.dtype}; float32 or the type of x ({x.dtype}) expected")
+    _need(w.device == x.device, f"{what}: w is on {w.device}, x on {x.device}")
+    _seq_check(what, "b", b, (x.shape[-1],), w.dtype, x.device)
+    _need(activation in _ACTIVATIONS, f"{what}: activation {activation!r}; one of {sorted(_ACTIVATIONS)} expected")
+    return _ACTIVATIONS[activation]
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, state, lengths, act, return_state):
+        ctx.set_materialize_grads(False)
+        bsz, steps, d = x.shape
+        taps = w.shape[1]
+        x, w, b, state = _rows(x), _dense(w), _dense(b), _dense(state)
+        y = torch.empty((bsz, steps, d), dtype=x.dtype, device=x.device)
+        state_out = torch.empty((bsz, taps - 1, d), dtype=x.dtype, device=x.device) if return_state else None
+        if y.numel() > 0:
+            with _OnDevice(x):
+                _native.check(_lib().afd_causal_conv_forward(
+                    x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _native.ptr(b), int(w.dtype == torch.float32),
+                    _native.ptr(state), _native.ptr(lengths), y.data_ptr(), _native.ptr(state_out), bsz, steps, d, taps, act,
+                    _SEQ_DTYPES[x.dtype], _native.stream_ptr()), "afd_causal_conv_forward")
+        elif state_out is not None:
+            state_out.copy_(state) if state is not None else state_out.zero_()
+        ctx.save_for_backward(x, w, b, state, lengths)
+        ctx.act = act
+        return y, state_out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dstate_out):
+        x, w, b, state, lengths = ctx.saved_tensors
+        bsz, steps, d = x.shape
+        taps = w.shape[1]
+        need = ctx.needs_input_grad
+        if x.numel() == 0:
+            dstate = None
+            if need[3]:
+                dstate = dstate_out.clone() if dstate_out is not None else torch.zeros_like(state)
+            return (torch.zeros_like(x), torch.zeros_like(w), torch.zeros_like(b) if need[2] else None, dstate,
+                    None, None, None)
+        dy = _rows(dy) if dy is not None else torch.zeros_like(x)
+        dstate_out = _dense(dstate_out)
+        dx = torch.empty((bsz, steps, d), dtype=x.dtype, device=x.device)
+        dw = torch.empty_like(w)
+        db = torch.empty_like(b) if b is not None else None
+        dstate = torch.empty_like(state) if need[3] else None
+        with _OnDevice(x):
+            lib = _lib()
+            ws = torch.empty(lib.afd_causal_conv_backward_workspace_bytes(bsz, steps, d, taps), dtype=torch.uint8,
+                             device=x.device)
+            _native.check(lib.afd_causal_conv_backward(
+                x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _native.ptr(b), int(w.dtype == torch.float32),
+                _native.ptr(state), _native.ptr(lengths), dy.data_ptr(), dy.stride(0), dy.stride(1),
+                _native.ptr(dstate_out), dx.data_ptr(), dw.data_ptr(), _native.ptr(db), _native.ptr(dstate), bsz, steps, d,
+                taps, ctx.act, _SEQ_DTYPES[x.dtype], ws.data_ptr(), ws.numel(), _native.stream_ptr()),
+                "afd_causal_conv_backward")
+        return dx, dw, db, dstate, None, None, None
+
+
+def causal_conv(x, w, b=None, activation: str = "none", state=None, lengths=None, return_state: bool = False):
+    """Causal depthwise convolution along time: y[:, t, c] = act(b[c] + sum_j w[c, j] x[:, t - (W - 1) + j, c]).
+
+    x [B, L, D] float32 / bfloat16 / float16 (batch and row strides are free); w [D, W], 2 <= W <= 8, and b [D] float32 or
+    the type of x; `activation` "none" or "silu".  `state` [B, W - 1, D] (type of x): the rows in front of the first, oldest
+    first; zeros if absent.  `lengths` [B] (int32 / int64, on the device): rows from lengths[i] on are padding -- they are
+    never read, their outputs and gradients are zero.  With `return_state` the result is (y, state behind the last token),
+    which `causal_conv` or `causal_conv_step` takes for what follows.  Differentiable in x, w, b and state; sums in
+    float32, results rounded once to the type of their tensor."""
+    act = _conv_check("causal_conv", x, w, b, activation, 3)
+    _seq_check("causal_conv", "state", state, (x.shape[0], w.shape[1] - 1, x.shape[2]), x.dtype, x.device)
+    lengths = _seq_lengths("causal_conv", lengths, x)
+    _seq_gpu("causal_conv", x)
+    y, state_out = _CausalConv.apply(x, w, b, state, lengths, act, bool(return_state))
+    return (y, state_out) if return_state else y
+
+
+def causal_conv_step(x, state, w, b=None, activation: str = "none", state_out=None):
+    """One time step of `causal_conv`: x [B, D] -> y [B, D].  `state` [B, W - 1, D] is moved on by one row in place, or into
+    `state_out` (same shape) if given.  No backward pass."""
+    act = _conv_check("causal_conv_step", x, w, b, activation, 2)
+    if state is None:
+        raise TypeError("causal_conv_step: state has to be a tensor")
+    _seq_check("causal_conv_step", "state", state, (x.shape[0], w.shape[1] - 1, x.shape[1]), x.dtype, x.device)
+    into = _step_state("causal_conv_step", state, state_out, (x, w, b, state))
+    _seq_gpu("causal_conv_step", x)
+    x, w, b = _rows(x), _dense(w), _dense(b)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if y.numel() > 0:
+        with _OnDevice(x):
+            _native.check(_lib().afd_causal_conv_step(
+                x.data_ptr(), x.stride(0), w.data_ptr(), _native.ptr(b), int(w.dtype == torch.float32), state.data_ptr(),
+                y.data_ptr(), into.data_ptr(), x.shape[0], x.shape[1], w.shape[1], act, _SEQ_DTYPES[x.dtype],
+                _native.stream_ptr()), "afd_causal_conv_step")
+    return y
+
+
+def _scan_check(what: str, x, dt, a, b, c, d, gate, dt_bias, state, ndim: int) -> None:
+    _seq_input(what, x, ndim)
+    chans, lead = x.shape[-1], tuple(x.shape[:-1])
+    if not isinstance(a, torch.Tensor):
+        raise TypeError(f"{what}: a is a {type(a).__name__}, not a tensor")
+    _need(a.dim() == 2 and a.shape[0] == chans, f"{what}: a has shape {tuple(a.shape)}, ({chans}, states) expected")
+    n = a.shape[1]
+    _need(1 <= n <= 64, f"{what}: {n} states per channel; 1 to 64 are supported")
+    for name, t in (("dt", dt), ("b", b), ("c", c)):
+        if t is None:
+            raise TypeError(f"{what}: {name} has to be a tensor")
+    for name, t, shape in (("dt", dt, lead + (chans,)), ("b", b, lead + (n,)), ("c", c, lead + (n,)),
+                           ("gate", gate, lead + (chans,))):
+        _seq_check(what, name, t, shape, x.dtype, x.device)
+    for name, t, shape in (("a", a, (chans, n)), ("d", d, (chans,)), ("dt_bias", dt_bias, (chans,)),
+                           ("state", state, (x.shape[0], chans, n))):
+        _seq_check(what, name, t, shape, torch.float32, x.device)
+
+
+def _scan_strides(tensors, axes):
+    out = []
+    for t in tensors:
+        out += [t.stride(i) if t is not None else 0 for i in axes]
+    return (_native.c_l * len(out))(*out)
+
+
+class _StateScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, a, b, c, d, gate, dt_bias, state, lengths, softplus, return_state, keep):
+        ctx.set_materialize_grads(False)
+        bsz, steps, chans = x.shape
+        n = a.shape[1]
+        x, dt, b, c, gate = _rows(x), _rows(dt), _rows(b), _rows(c), _rows(gate)
+        a, d, dt_bias, state = _dense(a), _dense(d), _dense(dt_bias), _dense(state)
+        y = torch.empty((bsz, steps, chans), dtype=x.dtype, device=x.device)
+        state_out = torch.empty((bsz, chans, n), dtype=torch.float32, device=x.device) if return_state else None
+        ckpt = None
+        if y.numel() > 0:
+            with _OnDevice(x):
+                lib = _lib()
+                if keep:
+                    ckpt = torch.empty(lib.afd_state_scan_checkpoint_floats(bsz, steps, chans, n), dtype=torch.float32,
+                                       device=x.device)
+                nbytes = lib.afd_state_scan_workspace_bytes(bsz, steps, chans, n, 0)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+                _native.check(lib.afd_state_scan_forward(
+                    x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _native.ptr(gate),
+                    _scan_strides((x, dt, b, c, gate), (0, 1)), a.data_ptr(), _native.ptr(d), _native.ptr(dt_bias),
+                    _native.ptr(state), _native.ptr(lengths), y.data_ptr(), _native.ptr(state_out), _native.ptr(ckpt), bsz,
+                    steps, chans, n, softplus, _SEQ_DTYPES[x.dtype], _native.ptr(ws), nbytes, _native.stream_ptr()),
+                    "afd_state_scan_forward")
+        elif state_out is not None:
+            state_out.copy_(state) if state is not None else state_out.zero_()
+        ctx.save_for_backward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, ckpt)
+        ctx.softplus = softplus
+        return y, state_out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dstate_out):
+        x, dt, a, b, c, d, gate, dt_bias, state, lengths, ckpt = ctx.saved_tensors
+        bsz, steps, chans = x.shape
+        n = a.shape[1]
+        need = ctx.needs_input_grad
+
+        def like(t, want=True):
+            return torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and want else None
+
+        grads = [like(t) for t in (x, dt, a, b, c, d, gate, dt_bias)] + [like(state, need[8])]
+        if x.numel() == 0:
+            for g in grads:
+                if g is not None:
+                    g.zero_()
+            if grads[8] is not None and dstate_out is not None:
+                grads[8].copy_(dstate_out)
+            return (*grads, None, None, None, None)
+        dx, ddt, da, db, dc, dd, dgate, dbias, dstate = grads
+        dy = _rows(dy) if dy is not None else torch.zeros_like(x)
+        dstate_out = _dense(dstate_out)
+        with _OnDevice(x):
+            lib = _lib()
+            ws = torch.empty(lib.afd_state_scan_workspace_bytes(bsz, steps, chans, n, 1), dtype=torch.uint8, device=x.device)
+            _native.check(lib.afd_state_scan_backward(
+                x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _native.ptr(gate), dy.data_ptr(),
+                _scan_strides((x, dt, b, c, gate, dy), (0, 1)), a.data_ptr(), _native.ptr(d), _native.ptr(dt_bias),
+                _native.ptr(lengths), ckpt.data_ptr(), _native.ptr(dstate_out), dx.data_ptr(), ddt.data_ptr(),
+                db.data_ptr(), dc.data_ptr(), _native.ptr(dgate), da.data_ptr(), _native.ptr(dd), _native.ptr(dbias),
+                _native.ptr(dstate), bsz, steps, chans, n, ctx.softplus, _SEQ_DTYPES[x.dtype], ws.data_ptr(), ws.numel(),
+                _native.stream_ptr()), "afd_state_scan_backward")
+        return (*grads, None, None, None, None)
+
+
+def state_scan(x, dt, a, b, c, d=None, gate=None, dt_bias=None, softplus: bool = False, state=None, lengths=None,
+               return_state: bool = False):
+    """Selective state-space scan along time, N states per channel:
+
+        delta = softplus(dt + dt_bias)  (or dt + dt_bias)
+        h[t] = exp(delta[t] a) h[t-1] + delta[t] b[t] x[t],   y[t] = (c[t] . h[t] + d x[t]) * silu(gate[t])
+
+    x, dt, gate [B, L, D] and b, c [B, L, N] of one type (float32 / bfloat16 / float16; batch and row strides are free);
+    a [D, N], 1 <= N <= 64, d [D], dt_bias [D] and `state` [B, D, N] float32.  gate, d, dt_bias and state may be absent.
+    `lengths` and `return_state` as `causal_conv`'s; the state is float32.  Differentiable in every tensor but lengths; the
+    recurrence and all sums in float32, results rounded once to the type of their tensor.  Gradients do not depend on the
+    order of execution.  Training keeps the state in front of every 16 tokens (float32)."""
+    _scan_check("state_scan", x, dt, a, b, c, d, gate, dt_bias, state, 3)
+    lengths = _seq_lengths("state_scan", lengths, x)
+    _seq_gpu("state_scan", x)
+    keep = _wants_grad(x, dt, a, b, c, d, gate, dt_bias, state)
+    y, state_out = _StateScan.apply(x, dt, a, b, c, d, gate, dt_bias, state, lengths, int(bool(softplus)),
+                                    bool(return_state), keep)
+    return (y, state_out) if return_state else y
+
+
+def state_scan_step(x, state, dt, a, b, c, d=None, gate=None, dt_bias=None, softplus: bool = False, state_out=None):
+    """One time step of `state_scan`: x, dt, gate [B, D] and b, c [B, N] -> y [B, D].  `state` [B, D, N] (float32) is moved on
+    in place, or into `state_out` (same shape) if given.  No backward pass."""
+    if state is None:
+        raise TypeError("state_scan_step: state has to be a tensor")
+    _scan_check("state_scan_step", x, dt, a, b, c, d, gate, dt_bias, state, 2)
+    into = _step_state("state_scan_step", state, state_out, (x, state, dt, a, b, c, d, gate, dt_bias))
+    _seq_gpu("state_scan_step", x)
+    x, dt, b, c, gate = _rows(x), _rows(dt), _rows(b), _rows(c), _rows(gate)
+    a, d, dt_bias = _dense(a), _dense(d), _dense(dt_bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if y.numel() > 0:
+        with _OnDevice(x):
+            _native.check(_lib().afd_state_scan_step(
+                x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _native.ptr(gate),
+                _scan_strides((x, dt, b, c, gate), (0,)), a.data_ptr(), _native.ptr(d), _native.ptr(dt_bias),
+                state.data_ptr(), y.data_ptr(), into.data_ptr(), x.shape[0], x.shape[1], a.shape[1], int(bool(softplus)),
+                _SEQ_DTYPES[x.dtype], _native.stream_ptr()), "afd_state_scan_step")
+    return y
+
+
+# --------------------------------------------------------------------------------------
+def _norm_tables(what: str, tensors, norm_type):
+    """(tensors in dense memory, pointers, counts, types) of a list for `afd_global_norm`."""
+    _need(norm_type in (2, 2.0, float("inf")), f"{what}: norm_type {norm_type}; 2 or inf expected")
+    dense, device = [], None
+    for i, t in enumerate(tensors):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: entry {i} is a {type(t).__name__}, not a tensor")
+        if t.layout != torch.strided or t.dtype not in _SEQ_DTYPES:
+            raise TypeError(f"{what}: entry {i} is {t.layout} {t.dtype}; dense float32, bfloat16 or float16 expected")
+        device = t.device if device is None else device
+        _need(t.device == device, f"{what}: entry {i} is on {t.device}, entry 0 on {device}")
+        t = t.detach()
+        # (the order of the elements is of no interest: a permuted but gapless tensor is taken as it lies in memory)
+        by_stride = t.permute(sorted(range(t.dim()), key=lambda k: -t.stride(k)))
+        dense.append(t if t.is_contiguous() or by_stride.is_contiguous() else t.contiguous())
+    return dense, device
+
+
+def _norm_arrays(dense):
+    n = len(dense)
+    return ((_native.c_p * n)(*[t.data_ptr() for t in dense]), (_native.c_l * n)(*[t.numel() for t in dense]),
+            (_native.c_i * n)(*[_SEQ_DTYPES[t.dtype] for t in dense]))
+
+
+def _launch_norm(dense, arrays, norm_type, max_norm: float, scale: float) -> torch.Tensor:
+    """[norm, factor] of `afd_global_norm` on the device of the tensors (which is the current one)."""
+    lib = _lib()
+    ptrs, counts, types = arrays
+    n = len(dense)
+    stats = torch.empty(2, dtype=torch.float32, device=dense[0].device)
+    ws = torch.empty(lib.afd_global_norm_workspace_bytes(counts, n), dtype=torch.uint8, device=stats.device)
+    _native.check(lib.afd_global_norm(ptrs, counts, types, n, int(norm_type == float("inf")), max_norm, scale,
+                                      stats.data_ptr(), ws.data_ptr(), ws.numel(), _native.stream_ptr()), "afd_global_norm")
+    return stats
+
+
+def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
+    """Norm of all elements of all `tensors` (float32 / bfloat16 / float16, mixed as they come) as one float32 scalar on their
+    device, without a host synchronisation: the root of the sum of squares, taken in float64, or the largest magnitude
+    (norm_type inf).  NaN if an element is; zero for an empty list."""
+    dense, device = _norm_tables("global_norm", list(tensors), norm_type)
+    if not dense:
+        return torch.zeros(())
+    _seq_gpu("global_norm", dense[0])
+    with _OnDevice(dense[0]):
+        return _launch_norm(dense, _norm_arrays(dense), norm_type, 1.0, 1.0)[0]
+
+
+def _check_disjoint(src, dst) -> None:
+    """No element may be scaled twice, nor be read after it was written for another tensor."""
+    spans = []
+    for s, o in zip(src, dst):
+        n = s.numel() * s.element_size()
+        if n == 0:
+            continue
+        spans.append((o.data_ptr(), o.data_ptr() + n, True))
+        if s.data_ptr() != o.data_ptr():
+            spans.append((s.data_ptr(), s.data_ptr() + n, False))
+    spans.sort()
+    end_any = end_written = 0
+    for lo, hi, written in spans:
+        _need(lo >= (end_any if written else end_written), "clip_gradients: tensors to be scaled overlap in memory")
+        end_any = max(end_any, hi)
+        end_written = max(end_written, hi) if written else end_written
+
+
+def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
+    """Scales `grads` by min(1, max_norm / (norm + 1e-6)), norm being their `global_norm`, in place or into the tensors of
+    `out` (same shapes and types; in place where an entry is the gradient itself).  Returns the norm in front of the
+    scaling, a float32 scalar on the device; nothing waits for it on the host.  A norm of inf gives zeros, NaN gives NaN."""
+    what = "clip_gradients"
+    max_norm = float(max_norm)
+    _need(max_norm >= 0.0, f"{what}: max_norm {max_norm} has to be a number from 0 on")
+    grads = list(grads)
+    dense, _ = _norm_tables(what, grads, norm_type)
+    back = []  # (gradient, dense copy) where the gradient's memory has gaps
+    if out is None:
+        for g, t in zip(grads, dense):
+            if t.data_ptr() != g.data_ptr():
+                _need(all(s != 0 or k <= 1 for s, k in zip(g.stride(), g.shape)),
+                      f"{what}: a gradient with elements that share memory cannot be scaled in place")
+                back.append((g, t))
+        into = dense
+    else:
+        into = list(out)
+        _need(len(into) == len(grads), f"{what}: {len(into)} tensors in out for {len(grads)} gradients")
+        for i, (g, o) in enumerate(zip(grads, into)):
+            _seq_check(what, f"out[{i}]", o, g.shape, g.dtype, g.device)
+            if o.stride() != dense[i].stride():
+                dense[i] = g.detach().contiguous()
+            _need(o.stride() == dense[i].stride(), f"{what}: out[{i}] has to be contiguous, or strided as its gradient")
+            into[i] = o.detach()
+    if not dense:
+        return torch.zeros(())
+    _seq_gpu(what, dense[0])
+    _check_disjoint(dense, into)
+    with _OnDevice(dense[0]):
+        arrays = _norm_arrays(dense)
+        stats = _launch_norm(dense, arrays, norm_type, max_norm, 1.0)
+        dst = (_native.c_p * len(into))(*[t.data_ptr() for t in into])
+        _native.check(_lib().afd_multi_scale(arrays[0], dst, arrays[1], arrays[2], len(dense), stats.data_ptr(),
+                                             _native.stream_ptr()), "afd_multi_scale")
+        for g, t in back:
+            g.detach().copy_(t)
+    return stats[0]
+
+
+# --------------------------------------------------------------------------------------
 class FusedAdam(torch.optim.Optimizer):
     """Adam with coupled L2 over ONE flat fp32 arena (params, grads, m, v contiguous).
 
@@ -1518,6 +1958,7 @@ class FusedAdam(torch.optim.Optimizer):
                 off += n
         self._relink()
         self.step_count = 0
+        self.last_grad_norm: Optional[torch.Tensor] = None
 
     @property
     def flat_grad(self) -> torch.Tensor:
@@ -1565,10 +2006,25 @@ class FusedAdam(torch.optim.Optimizer):
         self._relink()  # (the sources die here; the allocator is stream-ordered)
 
     @torch.no_grad()
-    def step(self, closure=None, grad_scale: float = 1.0):
+    def step(self, closure=None, grad_scale: float = 1.0, max_grad_norm: Optional[float] = None):
+        """One update; gradients are multiplied by `grad_scale` first.  With `max_grad_norm` they are also scaled to that
+        global norm (of the scaled gradients, as `clip_gradients`) inside the update's launch: the norm stays on the
+        device, in `last_grad_norm`."""
         g = self.param_groups[0]
+        if max_grad_norm is not None:
+            _need(float(max_grad_norm) >= 0.0, f"max_grad_norm {max_grad_norm} has to be a number from 0 on")
+            _seq_gpu("FusedAdam.step", self.flat)
         self.step_count += 1
         self.gather_grads()
+        if max_grad_norm is not None:
+            arena = [self._flat_grad]
+            stats = _launch_norm(arena, _norm_arrays(arena), 2.0, float(max_grad_norm), float(grad_scale))
+            _native.check(_lib().afd_adam_step_clipped(
+                _native.ptr(self.flat), _native.ptr(self._flat_grad), _native.ptr(self.m), _native.ptr(self.v),
+                self.flat.numel(), g["lr"], g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"], self.step_count,
+                _native.ptr(stats), _native.stream_ptr()), "afd_adam_step_clipped")
+            self.last_grad_norm = stats[0]
+            return None
         _native.check(_lib().afd_adam_step(
             _native.ptr(self.flat), _native.ptr(self._flat_grad), _native.ptr(self.m),
             _native.ptr(self.v), self.flat.numel(), g["lr"], g["betas"][0], g["betas"][1], g["eps"],

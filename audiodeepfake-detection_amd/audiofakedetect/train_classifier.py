@@ -257,9 +257,13 @@ class Trainer:
         start_gradient_allreduce(self.optimizer)
         loss.backward()
         scale = sync_gradients(self.model, self.optimizer)
+        clip = self.args.clip_grad_norm
         if isinstance(self.optimizer, ops.FusedAdam):
-            self.optimizer.step(grad_scale=scale)
+            # the norm is taken of the averaged gradients, the same on every rank
+            self.optimizer.step(grad_scale=scale, max_grad_norm=clip)
         else:
+            if clip is not None:
+                ops.clip_gradients([p.grad for p in self.model.parameters() if p.grad is not None], clip)
             self.optimizer.step()
         self.step_total += 1
         if self.step_total == 2:

@@ -96,6 +96,8 @@ def add_default_parser_args(parser: ArgumentParser) -> ArgumentParser:
     # batches straight from the library's threaded WAV reader + GPU PCM conversion / resampling instead of
     # DataLoader workers (16-bit PCM WAV datasets; same values)
     f("--native-loader", action="store_true")
+    # scale the gradients of a step to this global norm where it is larger (default: no clipping)
+    f("--clip-grad-norm", type=float, default=None)
     return parser
 
 

@@ -747,7 +747,8 @@ __global__ void ce_kernel(const float* __restrict__ logits, const long long* __r
 // ------------------------------- Adam (coupled L2) -------------------------------------
 __global__ void adam_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m,
                             float* __restrict__ v, size_t n, float lr, float b1, float b2, float eps,
-                            float wd, float bc1, float bc2_sqrt, float gscale) {
+                            float wd, float bc1, float bc2_sqrt, float gscale, const float* __restrict__ stats) {
+    if (stats) gscale = stats[1];  // (afd_global_norm's factor)
     for (size_t i = (size_t)blockIdx.x * kT + threadIdx.x; i < n; i += (size_t)gridDim.x * kT) {
         const float pi = p[i];
         const float gi = fmaf(wd, pi, g[i] * gscale);
@@ -1322,14 +1323,26 @@ extern "C" int afd_multi_gather(const float* const* srcs, const long* offsets, c
     return afd::check_launch("multi_gather_kernel");
 }
 
-extern "C" int afd_adam_step(float* params, const float* grads, float* m, float* v, size_t n, float lr,
-                             float beta1, float beta2, float eps, float weight_decay, int step,
-                             float grad_scale, afd_stream_t stream) {
+static int adam_step(float* params, const float* grads, float* m, float* v, size_t n, float lr, float beta1, float beta2,
+                     float eps, float weight_decay, int step, float grad_scale, const float* stats, afd_stream_t stream) {
     if (!params || !grads || !m || !v || step < 1) return afd::fail(AFD_ERR_ARG, "adam: bad argument");
     afd::ScopedBytes timing(AFD_K_ELEMENTWISE, 28.0 * (double)n, AFD_STREAM);
     const float bc1 = (float)(1.0 - pow((double)beta1, (double)step));
     const float bc2 = (float)sqrt(1.0 - pow((double)beta2, (double)step));
     hipLaunchKernelGGL(adam_kernel, dim3(grid1d(n)), dim3(kT), 0, AFD_STREAM, params, grads, m, v, n,
-                       lr, beta1, beta2, eps, weight_decay, bc1, bc2, grad_scale);
+                       lr, beta1, beta2, eps, weight_decay, bc1, bc2, grad_scale, stats);
     return afd::check_launch("adam_kernel");
+}
+
+extern "C" int afd_adam_step(float* params, const float* grads, float* m, float* v, size_t n, float lr,
+                             float beta1, float beta2, float eps, float weight_decay, int step,
+                             float grad_scale, afd_stream_t stream) {
+    return adam_step(params, grads, m, v, n, lr, beta1, beta2, eps, weight_decay, step, grad_scale, nullptr, stream);
+}
+
+extern "C" int afd_adam_step_clipped(float* params, const float* grads, float* m, float* v, size_t n, float lr, float beta1,
+                                     float beta2, float eps, float weight_decay, int step, const float* stats,
+                                     afd_stream_t stream) {
+    if (!stats) return afd::fail(AFD_ERR_ARG, "adam: no clipping factor");
+    return adam_step(params, grads, m, v, n, lr, beta1, beta2, eps, weight_decay, step, 1.f, stats, stream);
 }

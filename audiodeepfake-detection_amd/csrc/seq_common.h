@@ -1,0 +1,61 @@
+// Shared by the sequence-layer kernels (causal_conv.hip, state_scan*.hip, grad_clip.hip): element types, the
+// non-linearities of the state-space layer and the column sums that end their parameter gradients.
+#pragma once
+
+#include "afd_common.h"
+#include "../../include/afd_hip.h"
+
+namespace afd {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
+template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }  // round to nearest even
+
+inline size_t dtype_bytes(int dtype) { return dtype == AFD_T_F32 ? 4 : 2; }
+inline bool dtype_ok(int dtype) { return dtype == AFD_T_F32 || dtype == AFD_T_BF16 || dtype == AFD_T_F16; }
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// 1 / (1 + exp(-x)): the hardware's base-2 exponential and reciprocal, 1 ulp each.  exp overflows to inf for x < -88 and
+// the reciprocal of that is 0, which is the limit.
+__device__ __forceinline__ float sigmoid_f32(float x) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * x));
+}
+
+// log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1].  The step widths of a state-space layer start at
+// 1e-3 .. 1e-1, where log(1 + e) taken at face value has lost ten bits: log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3,
+// as its odd series up to s^15 (the next term is 2 s^17 / 17 < 1e-9 of the sum).
+__device__ __forceinline__ float softplus_f32(float x) {
+    const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(x));
+    const float s = e * __builtin_amdgcn_rcpf(2.f + e);
+    const float q = s * s;
+    float p = 1.f / 15.f;
+    p = fmaf(p, q, 1.f / 13.f);
+    p = fmaf(p, q, 1.f / 11.f);
+    p = fmaf(p, q, 1.f / 9.f);
+    p = fmaf(p, q, 1.f / 7.f);
+    p = fmaf(p, q, 1.f / 5.f);
+    p = fmaf(p, q, 1.f / 3.f);
+    p = fmaf(p, q, 1.f);
+    // (x = NaN: fmaxf would drop it)
+    return (x > 0.f ? x : 0.f * x) + 2.f * s * p;
+}
+
+// Sums of the columns of part[rows][cols]: each workgroup takes 64 columns, its 16 waves take every 16th row and meet in LDS.
+// Column c goes to the output that owns it (fixed order: no atomics, the same bits every time).  The partial rows are
+// written just before by the same stream: L2-resident in most cases, a tenth or less of the main kernel's bytes.
+struct ColumnOut {
+    void* out;       // NULL: dropped
+    int begin, end;  // the columns [begin, end) of a row belong to this output
+    int width, keep; // inside it, column i = (i / width, i % width) is kept where i % width < keep, at i / width * keep + i % width
+    int dtype;
+};
+struct ColumnOuts {
+    ColumnOut o[4];
+    int n;
+};
+int launch_column_sums(const float* part, long rows, int cols, const ColumnOuts& outs, hipStream_t s);
+
+}  // namespace afd

@@ -1,0 +1,221 @@
+// Selective state-space scan: argument block and device helpers shared by state_scan_fwd.hip and state_scan_bwd.hip.
+//
+//   delta = softplus(dt + dt_bias)  (or dt + dt_bias)
+//   h[t][c][n] = exp(delta[t][c] a[c][n]) h[t-1][c][n] + delta[t][c] b[t][n] x[t][c]
+//   y0[t][c]   = sum_n c[t][n] h[t][c][n] + d[c] x[t][c],      y = y0  or  y0 silu(gate)
+//
+// Lane layout (both directions): a lane owns NS (<= 4) states of one channel, Q neighbouring lanes own the channel, so a wave
+// holds 64 / Q channels and the states live in registers for the whole walk over time.  The Q lanes of a channel also
+// share its per-token work: time advances in blocks of 16 tokens, lane q of a channel loads tokens q, q + Q, ... and
+// computes their softplus / gate ONCE, and the value a token needs is broadcast to the channel's lanes by a DPP move.  Against
+// one lane per channel this quarters the transcendental work that is not exp(delta a), and it gives 4 x the waves from
+// the same rows, which is what a scan lacks: its only parallel axes are batch and channel.
+// The b and c rows are the same for every channel: a workgroup (4 waves) stages a block's rows in LDS as fp32, double
+// buffered, and each lane reads its own NS of them as one vector.
+#pragma once
+
+#include "seq_common.h"
+
+namespace afd {
+
+constexpr int kTok = 16;       // tokens per block
+constexpr int kScanT = 256;    // threads per workgroup: 4 waves
+
+struct ScanArgs {
+    const void *x, *dt, *b, *c, *gate, *dy;
+    long xb, xl, tb, tl, bb, bl, cb, cl, gb, gl, yb, yl;  // batch / row strides in elements; the last axis is contiguous
+    const float *a, *d, *dt_bias, *state;
+    const int* lengths;
+    void* y;
+    float* state_out;
+    float* ckpt;  // [B][ceil(L / 16)][D][NP]: the state in front of every block of 16 tokens (written for training)
+    float* seg_h;  // [B][S][D][NP]: what a time segment leaves on its own (forward: state, backward: gradient)
+    float* seg_d;  // [B][S][D]: the segment's sum of delta
+    int B, L, D, N, softplus;
+    int S, seg_blocks;  // time segments and blocks per segment
+    int nb;             // workgroups per row of channels
+    // backward only
+    const float* dstate_out;
+    void *dx, *ddt, *dgate;
+    float* dstate;
+    float* part_bc;  // [nb][B][L][2 NP]
+    float* part_p;   // [B S][D NP + 2 D]: da, dd, ddt_bias
+};
+
+// Everything below is device code.
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+
+// the value that lane j of the channel's Q lanes holds, to all of them (j is a constant once the callers are unrolled)
+template <int Q> __device__ __forceinline__ float from_lane(float v, int j) {
+    if constexpr (Q == 4) {
+        switch (j) {  // quad_perm [j, j, j, j]
+            case 0: return dpp<0x00>(v);
+            case 1: return dpp<0x55>(v);
+            case 2: return dpp<0xaa>(v);
+            default: return dpp<0xff>(v);
+        }
+    } else if constexpr (Q == 16) {
+        switch (j) {  // row_newbcast:j
+            case 0: return dpp<0x150>(v);
+            case 1: return dpp<0x151>(v);
+            case 2: return dpp<0x152>(v);
+            case 3: return dpp<0x153>(v);
+            case 4: return dpp<0x154>(v);
+            case 5: return dpp<0x155>(v);
+            case 6: return dpp<0x156>(v);
+            case 7: return dpp<0x157>(v);
+            case 8: return dpp<0x158>(v);
+            case 9: return dpp<0x159>(v);
+            case 10: return dpp<0x15a>(v);
+            case 11: return dpp<0x15b>(v);
+            case 12: return dpp<0x15c>(v);
+            case 13: return dpp<0x15d>(v);
+            case 14: return dpp<0x15e>(v);
+            default: return dpp<0x15f>(v);
+        }
+    } else {
+        static_assert(Q == 8, "lanes per channel");
+        float lo, hi;  // the two channels of a row of 16 lanes
+        switch (j) {
+            case 0: lo = dpp<0x150>(v); hi = dpp<0x158>(v); break;
+            case 1: lo = dpp<0x151>(v); hi = dpp<0x159>(v); break;
+            case 2: lo = dpp<0x152>(v); hi = dpp<0x15a>(v); break;
+            case 3: lo = dpp<0x153>(v); hi = dpp<0x15b>(v); break;
+            case 4: lo = dpp<0x154>(v); hi = dpp<0x15c>(v); break;
+            case 5: lo = dpp<0x155>(v); hi = dpp<0x15d>(v); break;
+            case 6: lo = dpp<0x156>(v); hi = dpp<0x15e>(v); break;
+            default: lo = dpp<0x157>(v); hi = dpp<0x15f>(v); break;
+        }
+        return (threadIdx.x & 8) ? hi : lo;
+    }
+}
+
+// sum over the Q lanes of a channel, in all of them
+template <int Q> __device__ __forceinline__ float sum_lanes(float v) {
+    v += dpp<0xb1>(v);  // quad_perm [1, 0, 3, 2]
+    v += dpp<0x4e>(v);  // quad_perm [2, 3, 0, 1]
+    if constexpr (Q >= 8) v += dpp<0x141>(v);   // row_half_mirror: the quads are uniform by now
+    if constexpr (Q >= 16) v += dpp<0x140>(v);  // row_mirror
+    return v;
+}
+
+template <int NS> struct Vec;
+template <> struct Vec<1> { typedef float type; };
+template <> struct Vec<2> { typedef float type __attribute__((ext_vector_type(2))); };
+template <> struct Vec<4> { typedef float type __attribute__((ext_vector_type(4))); };
+
+template <int NS> __device__ __forceinline__ void load_vec(const float* p, float (&r)[NS]) {
+    const typename Vec<NS>::type v = *reinterpret_cast<const typename Vec<NS>::type*>(p);
+    if constexpr (NS == 1) r[0] = v;
+    else {
+#pragma unroll
+        for (int k = 0; k < NS; ++k) r[k] = v[k];
+    }
+}
+template <int NS> __device__ __forceinline__ void store_vec(float* p, const float (&r)[NS]) {
+    typename Vec<NS>::type v;
+    if constexpr (NS == 1) v = r[0];
+    else {
+#pragma unroll
+        for (int k = 0; k < NS; ++k) v[k] = r[k];
+    }
+    *reinterpret_cast<typename Vec<NS>::type*>(p) = v;
+}
+
+// rows of N floats that need not be aligned or padded (the caller's state, a): n0 = this lane's first state
+template <int NS> __device__ __forceinline__ void load_states(const float* p, int n0, int N, bool live, float (&r)[NS]) {
+#pragma unroll
+    for (int k = 0; k < NS; ++k) r[k] = (live && p && n0 + k < N) ? p[n0 + k] : 0.f;
+}
+template <int NS> __device__ __forceinline__ void store_states(float* p, int n0, int N, bool live, const float (&r)[NS]) {
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+        if (live && n0 + k < N) p[n0 + k] = r[k];
+}
+
+__device__ __forceinline__ int scan_rows(const int* lengths, int b, int L) {
+    if (!lengths) return L;
+    const int n = lengths[b];
+    return n < 0 ? 0 : (n > L ? L : n);
+}
+
+// The b and c rows of one block on their way into LDS: E values per thread, fetched early and written late.
+template <typename T, int NP> struct BcStage {
+    static constexpr int kAll = kTok * 2 * NP;
+    static constexpr int E = (kAll + kScanT - 1) / kScanT;
+    T v[E];
+    __device__ __forceinline__ void fetch(const ScanArgs& p, const T* brow, const T* crow, int t0, int n) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = e * kScanT + (int)threadIdx.x;
+            const int tok = i / (2 * NP), col = i % (2 * NP);
+            const int s = col % NP;
+            v[e] = (T)0.f;
+            if (i < kAll && s < p.N && t0 + tok < n) {
+                v[e] = col < NP ? brow[(size_t)(t0 + tok) * p.bl + s] : crow[(size_t)(t0 + tok) * p.cl + s];
+            }
+        }
+    }
+    __device__ __forceinline__ void put(float* lds) const {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = e * kScanT + (int)threadIdx.x;
+            if (i < kAll) lds[i] = to_f32(v[e]);
+        }
+    }
+};
+
+// Tokens q, q + Q, ... of a block for this lane's channel (zero behind row n, so what lies there is never used).
+template <typename T, int Q> struct TokLoad {
+    static constexpr int R = kTok / Q;
+    T v[R];
+    __device__ __forceinline__ void fetch(const T* col, long row, int t0, int q, int n, bool live) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int t = t0 + i * Q + q;
+            v[i] = (T)0.f;
+            if (live && t < n) v[i] = col[(size_t)t * row];
+        }
+    }
+};
+
+struct ScanPlace {
+    int b, s, cb, ch, q, n0, n;
+    bool live;
+};
+// workgroup id -> (row of the batch, time segment, block of channels), channel blocks fastest
+template <int Q, int NS> __device__ __forceinline__ ScanPlace scan_place(const ScanArgs& p) {
+    ScanPlace w;
+    const int id = blockIdx.x;
+    w.cb = id % p.nb;
+    const int r = id / p.nb;
+    w.s = r % p.S;
+    w.b = r / p.S;
+    w.q = threadIdx.x & (Q - 1);
+    w.ch = w.cb * (kScanT / Q) + (int)threadIdx.x / Q;
+    w.live = w.ch < p.D;
+    w.n0 = w.q * NS;
+    w.n = scan_rows(p.lengths, w.b, p.L);
+    return w;
+}
+
+struct ScanShape {
+    int Q, NS, NP;  // lanes per channel, states per lane, Q NS
+};
+// The smallest padded state count that holds N; 4 lanes per channel up to 16 states, then 4 states per lane.
+inline ScanShape scan_shape(int N) {
+    if (N <= 4) return {4, 1, 4};
+    if (N <= 8) return {4, 2, 8};
+    if (N <= 16) return {4, 4, 16};
+    if (N <= 32) return {8, 4, 32};
+    return {16, 4, 64};
+}
+
+int scan_forward_launch(const ScanArgs& p, int dtype, hipStream_t s);
+int scan_backward_launch(const ScanArgs& p, int dtype, hipStream_t s);
+// db and dc [B][L][N] from the workgroups' partial sums
+int scan_bc_gradients(const ScanArgs& p, void* db, void* dc, int dtype, hipStream_t s);
+
+}  // namespace afd

@@ -57,7 +57,13 @@ int afd_version(void);
 #define AFD_K_ELEMENTWISE 10 /* pool, dropout, permute, Linear + mean, cross entropy, gather, Adam, normalise */
 #define AFD_K_CONV1X1 11    /* 1x1 convolutions forward / backward-data: GEMMs at 16 flop per byte, HBM-leaning;
                                work = direct-form flops, issued = the same with tile padding, bytes = tensors once */
-#define AFD_K_COUNT 12
+#define AFD_K_SEQUENCE 12   /* causal convolution, state-space scan, global norm / gradient scaling: work = bytes */
+#define AFD_K_COUNT 13
+
+/* Element types of the entry points that take more than fp32 */
+#define AFD_T_F32 0
+#define AFD_T_BF16 1
+#define AFD_T_F16 2
 int afd_timing_enable(int on);
 int afd_timing_collect(int id, double* total_ms, long long* count, double* total_work,
                        double* total_issued_flops, double* total_algorithmic_bytes);
@@ -590,6 +596,67 @@ int afd_multi_gather(const float* const* srcs, const long* offsets, const long* 
 int afd_adam_step(float* params, const float* grads, float* m, float* v, size_t n, float lr,
                   float beta1, float beta2, float eps, float weight_decay, int step,
                   float grad_scale, afd_stream_t stream);
+
+/* ... with the gradients also multiplied by stats[1] (afd_global_norm's factor, which already holds its `scale`; device
+ * memory): clipping without a pass of its own and without the host waiting for the norm. */
+int afd_adam_step_clipped(float* params, const float* grads, float* m, float* v, size_t n, float lr, float beta1,
+                          float beta2, float eps, float weight_decay, int step, const float* stats,
+                          afd_stream_t stream);
+
+/* Global norm of n tensors and the factor that brings it to max_norm.  src / counts / dtypes (AFD_T_*) are HOST arrays of n
+ * device pointers, element counts and types; stats [2] (device): stats[0] = |scale| * norm, the norm being the root of the
+ * sum of squares or, with maximum != 0, the largest magnitude; stats[1] = scale * min(1, max_norm / (stats[0] + 1e-6)).
+ * A NaN among the elements makes both NaN.
+ * afd_multi_scale: dst[k] = src[k] * stats[1] for n tensors (dst[k] may be src[k]; the same types). */
+size_t afd_global_norm_workspace_bytes(const long* counts, int n);
+int afd_global_norm(const void* const* src, const long* counts, const int* dtypes, int n, int maximum, float max_norm,
+                    float scale, float* stats, void* ws, size_t ws_bytes, afd_stream_t stream);
+int afd_multi_scale(const void* const* src, void* const* dst, const long* counts, const int* dtypes, int n,
+                    const float* stats, afd_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Sequence layers: a short causal convolution and a selective state-space scan over [batch, time, channels] tensors.
+ * Activations (x, dt, b, c, gate, y and their gradients) are of type `dtype` (AFD_T_*); their last axis is contiguous, batch
+ * and row strides are given in elements (outputs are dense).  lengths [B] (device, may be NULL: L): rows from lengths[b] on
+ * are not read, their outputs and gradients are 0 and the state behind a row is the one after its last token; values
+ * outside 0 .. L count as the nearer end.
+ *
+ * Causal convolution, W = 2 .. 8 taps w [D][W], bias [D] (may be NULL), both fp32 when w_f32 != 0, else of type dtype:
+ *   z[t][c] = bias[c] + sum_j w[c][j] x[t - (W - 1) + j][c],  y = z (act 0) or z sigmoid(z) (act 1)
+ * state / state_out [B][W - 1][D]: the rows in front of the first / up to the last token, oldest first (NULL: zero / not
+ * wanted).  The step form takes one row x [B][D] and may write the state in place. */
+int afd_causal_conv_forward(const void* x, long long xb, long long xl, const void* w, const void* bias, int w_f32,
+                            const void* state, const int* lengths, void* y, void* state_out, int B, int L, int D, int W,
+                            int act, int dtype, afd_stream_t stream);
+size_t afd_causal_conv_backward_workspace_bytes(int B, int L, int D, int W);
+int afd_causal_conv_backward(const void* x, long long xb, long long xl, const void* w, const void* bias, int w_f32,
+                             const void* state, const int* lengths, const void* dy, long long dyb, long long dyl,
+                             const void* dstate_out, void* dx, void* dw, void* dbias, void* dstate, int B, int L, int D,
+                             int W, int act, int dtype, void* ws, size_t ws_bytes, afd_stream_t stream);
+int afd_causal_conv_step(const void* x, long long xb, const void* w, const void* bias, int w_f32, const void* state,
+                         void* y, void* state_out, int B, int D, int W, int act, int dtype, afd_stream_t stream);
+
+/* Selective state-space scan with N = 1 .. 64 states per channel; a [D][N], d [D], dt_bias [D], state [B][D][N] fp32:
+ *   delta = softplus(dt + dt_bias) (softplus != 0) or dt + dt_bias
+ *   h[t] = exp(delta a) h[t-1] + delta b[t] x[t],   y = (sum_n c[t][n] h[t][n] + d x[t]) * silu(gate)
+ * gate, d, dt_bias, state, state_out may be NULL.  strides (HOST): batch, row of x, dt, b, c, gate (10 values), then
+ * of dy (backward: 12); the step form takes the batch strides alone (5).  checkpoints: NULL, or
+ * afd_state_scan_checkpoint_floats floats that the backward reads (the state in front of every 16 tokens).
+ * b, c [B][L][N]; db, dc likewise, dense.  dgate, dd, ddt_bias, dstate may be NULL where the input is. */
+size_t afd_state_scan_workspace_bytes(int B, int L, int D, int N, int backward);
+size_t afd_state_scan_checkpoint_floats(int B, int L, int D, int N);
+int afd_state_scan_forward(const void* x, const void* dt, const void* b, const void* c, const void* gate,
+                           const long long* strides, const float* a, const float* d, const float* dt_bias,
+                           const float* state, const int* lengths, void* y, float* state_out, float* checkpoints, int B,
+                           int L, int D, int N, int softplus, int dtype, void* ws, size_t ws_bytes, afd_stream_t stream);
+int afd_state_scan_backward(const void* x, const void* dt, const void* b, const void* c, const void* gate, const void* dy,
+                            const long long* strides, const float* a, const float* d, const float* dt_bias,
+                            const int* lengths, const float* checkpoints, const float* dstate_out, void* dx, void* ddt,
+                            void* db, void* dc, void* dgate, float* da, float* dd, float* ddt_bias, float* dstate, int B,
+                            int L, int D, int N, int softplus, int dtype, void* ws, size_t ws_bytes, afd_stream_t stream);
+int afd_state_scan_step(const void* x, const void* dt, const void* b, const void* c, const void* gate,
+                        const long long* strides, const float* a, const float* d, const float* dt_bias, const float* state,
+                        void* y, float* state_out, int B, int D, int N, int softplus, int dtype, afd_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
  * The in-step collectives of data-parallel training straight on RCCL, on the caller's stream (opt-in).

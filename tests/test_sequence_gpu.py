@@ -1,0 +1,683 @@
+"""GPU parity of the sequence-layer operators (csrc/causal_conv.hip, state_scan_*.hip, grad_clip.hip) against the float64
+restatements of sequence_ref.py.
+
+Tolerances (sequence_ref.close): half a step of the result's type, plus a count of float32 roundings times 2^-24 of the sums
+of magnitudes behind the result.  The counts, worst case, errors adding up linearly:
+  convolution          W products and sums, sigmoid and product (10)                       -> 2 W + 32
+    dw, db             plus 64 rows in a thread's sum and the partial rows behind it       -> + 64 + B ceil(L / 64)
+  scan                 per step 5 (decay: exponent and exponential 3, product and sum 2); the error of delta (softplus: 20)
+                       reaches a decay exp(-s) as 22 s <= 22 / e of it; c . h and gate 40   -> 64 + 5 L
+    gradients          the same again backwards, sums over channels or rows                 -> 160 + 12 L + B + D / 16
+"""
+
+import pytest
+import torch
+
+import sequence_ref as ref
+from audiofakedetect import ops
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def _rnd(g, *shape, scale=1.0, dtype=torch.float32):
+    return (scale * torch.randn(*shape, generator=g)).to(dtype).cuda()
+
+
+def _conv_inputs(seed, dtype, b, l, d, w, bias=True, state=False, wtype=None):
+    g = torch.Generator().manual_seed(seed)
+    t = TYPES[dtype]
+    wt = t if wtype == "same" else torch.float32
+    return dict(x=_rnd(g, b, l, d, dtype=t), w=_rnd(g, d, w, scale=0.5, dtype=wt), b=_rnd(g, d, dtype=wt) if bias else None,
+                state=_rnd(g, b, w - 1, d, dtype=t) if state else None)
+
+
+def _lengths(kind, b, l):
+    if kind is None:
+        return None
+    some = [l, 0, 1, max(1, l // 2), max(0, l - 1), l + 5, -3, 17]
+    return torch.tensor([some[i % len(some)] for i in range(b)], dtype=kind, device="cuda")
+
+
+CONV = [
+    # dtype, B, L, D, W, act, bias, state, lengths, taps of x's type
+    ("fp32", 1, 1, 1, 2, "none", False, False, None, None),
+    ("fp32", 2, 3, 4, 4, "silu", True, True, None, None),
+    ("bf16", 3, 17, 8, 4, "silu", True, True, torch.int32, None),
+    ("bf16", 8, 33, 24, 3, "none", True, False, torch.int64, "same"),
+    ("fp16", 2, 70, 37, 5, "silu", False, True, None, "same"),
+    ("fp16", 8, 131, 40, 4, "silu", True, True, torch.int32, None),
+    ("fp32", 2, 129, 67, 8, "silu", True, True, torch.int32, None),
+    ("fp32", 1, 200, 128, 6, "none", True, False, None, None),
+    ("bf16", 2, 65, 264, 7, "silu", True, True, None, None),
+    ("bf16", 1, 5, 16, 8, "silu", True, True, None, None),  # fewer rows than taps
+    ("bf16", 2, 64, 513, 4, "silu", True, False, None, None),
+]
+
+
+@pytest.mark.parametrize("dtype, b, l, d, w, act, bias, state, lens, wtype", CONV)
+def test_conv_forward_and_gradients(dtype, b, l, d, w, act, bias, state, lens, wtype):
+    t = _conv_inputs(l * 7 + d, dtype, b, l, d, w, bias, state, wtype)
+    lengths = _lengths(lens, b, l)
+    for v in t.values():
+        if v is not None:
+            v.requires_grad_(True)
+    y, so = ops.causal_conv(t["x"], t["w"], t["b"], act, state=t["state"], lengths=lengths, return_state=True)
+    g = torch.Generator().manual_seed(5)
+    dy, ds = _rnd(g, b, l, d, dtype=y.dtype), _rnd(g, b, w - 1, d, dtype=y.dtype)
+    names = [k for k, v in t.items() if v is not None]
+    grads = dict(zip(names, torch.autograd.grad((y, so), [t[k] for k in names], (dy, ds))))
+    kw = dict(act=act, lengths=lengths, dy=dy, dstate_out=ds)
+    want, bound = ref.conv(**t, **kw), ref.conv(**t, **kw, absolute=True)
+    k = 2 * w + 32
+    ref.close(y, want["y"], bound["y"], k, "y")
+    assert torch.equal(so.cpu().double(), want["state"]), "state: a copy of rows"
+    rows = 64 + b * ((l + 63) // 64)
+    for name in names:
+        ref.close(grads[name], want["d" + name], bound["d" + name], k + (rows if name in ("w", "b") else 0), "d" + name)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("d", [1, 37, 64])
+@pytest.mark.parametrize("w", [2, 4, 8])
+def test_conv_steps_continue_a_prompt(dtype, d, w):
+    t = _conv_inputs(3, dtype, 3, 12, d, w, True, True)
+    with torch.no_grad():
+        y, so = ops.causal_conv(t["x"], t["w"], t["b"], "silu", state=t["state"], return_state=True)
+        head, st = ops.causal_conv(t["x"][:, :5], t["w"], t["b"], "silu", state=t["state"], return_state=True)
+        assert torch.equal(head, y[:, :5])
+        spare = torch.empty_like(st)
+        for i in range(5, 12):
+            if i % 2:
+                yi = ops.causal_conv_step(t["x"][:, i], st, t["w"], t["b"], "silu")
+            else:
+                yi = ops.causal_conv_step(t["x"][:, i], st, t["w"], t["b"], "silu", state_out=spare)
+                st, spare = spare, st
+            assert torch.equal(yi, y[:, i]), i  # the same products in the same order
+        assert torch.equal(st, so)
+
+
+def test_conv_padding_is_never_read():
+    t = _conv_inputs(9, "bf16", 4, 40, 48, 4, True, False)
+    lengths = torch.tensor([40, 0, 3, 21], device="cuda", dtype=torch.int32)
+    dirty = t["x"].clone()
+    for i, n in enumerate(lengths.tolist()):
+        dirty[i, n:] = float("nan") if i % 2 else float("inf")
+    outs = []
+    for x in (t["x"], dirty):
+        x = x.detach().requires_grad_(True)
+        y, so = ops.causal_conv(x, t["w"].requires_grad_(True), t["b"], "silu", lengths=lengths, return_state=True)
+        dy = torch.ones_like(y)
+        for i, n in enumerate(lengths.tolist()):
+            dy[i, n:] = float("nan")
+        outs.append((y, so, *torch.autograd.grad(y, [x, t["w"]], dy)))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b) and bool(torch.isfinite(a.float()).all())
+    assert not outs[0][0][1].any() and not outs[0][2][2, 3:].any()
+
+
+def test_conv_strided_and_unaligned_views():
+    g = torch.Generator().manual_seed(4)
+    both = _rnd(g, 3, 21, 2 * 48 + 1, dtype=torch.bfloat16)
+    w, b = _rnd(g, 48, 4), _rnd(g, 48)
+    for x in (both[:, :, :48], both[:, :, 49:], both[:, ::2, 1:49], both[:, :, :96:2], both.transpose(0, 1)[:, :, 1:49]):
+        y = ops.causal_conv(x, w, b, "silu")
+        assert torch.equal(y, ops.causal_conv(x.contiguous(), w, b, "silu"))
+        assert y.is_contiguous()
+    one = _rnd(g, 1, 1, 48, dtype=torch.bfloat16).expand(3, 20, 48)
+    assert torch.equal(ops.causal_conv(one, w, b), ops.causal_conv(one.contiguous(), w, b))
+    x = both[:, :, :48].detach().requires_grad_(True)
+    (dx,) = torch.autograd.grad(ops.causal_conv(x, w, b).float().sum(), [x])  # an expanded gradient arrives
+    (want,) = torch.autograd.grad(ops.causal_conv(x, w, b), [x], torch.ones(3, 21, 48, device="cuda", dtype=torch.bfloat16))
+    assert torch.equal(dx, want)
+
+
+def _scan_inputs(seed, dtype, b, l, d, n, gate=True, skip=True, bias=True, state=True):
+    g = torch.Generator().manual_seed(seed)
+    t = TYPES[dtype]
+    return dict(x=_rnd(g, b, l, d, dtype=t), dt=_rnd(g, b, l, d, scale=0.5, dtype=t),
+                a=-(torch.arange(1, n + 1).float() * torch.exp(0.1 * torch.randn(d, n, generator=g))).cuda(),
+                b=_rnd(g, b, l, n, dtype=t), c=_rnd(g, b, l, n, dtype=t), d=_rnd(g, d) if skip else None,
+                gate=_rnd(g, b, l, d, dtype=t) if gate else None,
+                dt_bias=(torch.rand(d, generator=g) * 5 - 6).cuda() if bias else None,
+                state=_rnd(g, b, d, n, scale=0.3) if state else None)
+
+
+SCAN = [
+    # dtype, B, L, D, N, lengths, absent inputs
+    ("fp32", 1, 1, 1, 1, None, ("gate", "d", "state")),
+    ("fp32", 2, 2, 3, 2, None, ()),
+    ("fp32", 2, 15, 64, 16, None, ()),
+    ("bf16", 3, 16, 65, 16, None, ("state",)),
+    ("fp16", 8, 17, 40, 16, torch.int32, ()),
+    ("fp32", 8, 37, 67, 13, torch.int64, ("gate",)),
+    ("bf16", 2, 33, 130, 4, None, ()),
+    ("fp32", 2, 50, 20, 3, torch.int32, ("d", "dt_bias")),
+    ("fp16", 2, 33, 66, 8, None, ("state",)),
+    ("fp32", 3, 34, 33, 5, torch.int32, ()),
+    ("bf16", 2, 35, 40, 32, None, ()),
+    ("fp32", 8, 40, 35, 17, torch.int32, ()),
+    ("fp32", 2, 33, 20, 64, None, ()),
+    ("fp16", 3, 20, 17, 33, torch.int32, ("gate",)),
+    # few rows and many blocks of tokens: the time axis is split
+    ("fp32", 1, 300, 20, 16, None, ()),
+    ("bf16", 2, 517, 70, 16, torch.int32, ()),
+    ("fp32", 8, 400, 9, 7, torch.int32, ()),
+    ("fp32", 3, 390, 5, 40, torch.int32, ()),
+]
+
+
+@pytest.mark.parametrize("dtype, b, l, d, n, lens, absent", SCAN)
+def test_scan_forward_and_gradients(dtype, b, l, d, n, lens, absent):
+    t = _scan_inputs(l * 3 + n, dtype, b, l, d, n, **{{"gate": "gate", "d": "skip", "dt_bias": "bias", "state": "state"}[k]: False
+                                                  for k in absent})
+    softplus = "dt_bias" not in absent
+    if not softplus:
+        t["dt"] = t["dt"].abs()
+    lengths = _lengths(lens, b, l)
+    for v in t.values():
+        if v is not None:
+            v.requires_grad_(True)
+    y, so = ops.state_scan(**t, softplus=softplus, lengths=lengths, return_state=True)
+    with torch.no_grad():
+        assert torch.equal(ops.state_scan(**t, softplus=softplus, lengths=lengths), y), "with and without what training keeps"
+    g = torch.Generator().manual_seed(6)
+    dy, ds = _rnd(g, b, l, d, dtype=y.dtype), _rnd(g, b, d, n, scale=0.3)
+    names = [k for k, v in t.items() if v is not None]
+    grads = dict(zip(names, torch.autograd.grad((y, so), [t[k] for k in names], (dy, ds))))
+    kw = dict(softplus=softplus, lengths=lengths, dy=dy, dstate_out=ds)
+    want, bound = ref.scan(**t, **kw), ref.scan(**t, **kw, absolute=True)
+    ref.close(y, want["y"], bound["y"], 64 + 5 * l, "y")
+    ref.close(so, want["state"], bound["state"], 64 + 5 * l, "state")
+    for name in names:
+        ref.close(grads[name], want["d" + name], bound["d" + name], 160 + 12 * l + b + d / 16, "d" + name)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("n", [1, 4, 7, 8, 16, 24, 64])
+def test_scan_steps_continue_a_prompt(dtype, n):
+    t = _scan_inputs(n, dtype, 3, 9, 70, n)
+    par = {k: t[k] for k in ("a", "d", "dt_bias")}
+    seq = ("x", "dt", "b", "c", "gate")
+    with torch.no_grad():
+        y, so = ops.state_scan(**t, softplus=True, return_state=True)
+        _, st = ops.state_scan(**{k: t[k][:, :4] for k in seq}, **par, softplus=True, state=t["state"], return_state=True)
+        spare = torch.empty_like(st)
+        for i in range(4, 9):
+            one = {k: t[k][:, i] for k in seq}
+            if i % 2:
+                yi = ops.state_scan_step(state=st, **one, **par, softplus=True)
+            else:
+                yi = ops.state_scan_step(state=st, **one, **par, softplus=True, state_out=spare)
+                st, spare = spare, st
+            kw = dict(softplus=True)
+            want = ref.scan(**{k: t[k][:, :i + 1] for k in seq}, **par, state=t["state"], **kw)
+            bound = ref.scan(**{k: t[k][:, :i + 1] for k in seq}, **par, state=t["state"], **kw, absolute=True)
+            ref.close(yi, want["y"][:, i], bound["y"][:, i], 64 + 5 * i, f"y at {i}")
+        want, bound = ref.scan(**t, softplus=True), ref.scan(**t, softplus=True, absolute=True)
+        ref.close(st, want["state"], bound["state"], 64 + 45, "state by steps")
+        ref.close(so, want["state"], bound["state"], 64 + 45, "state of the prompt")
+
+
+def test_scan_step_takes_unaligned_states_and_strided_rows():
+    t = _scan_inputs(2, "bf16", 3, 4, 20, 16)
+    flat = torch.empty(3 * 20 * 16 + 3, device="cuda")
+    par = {k: t[k] for k in ("a", "d", "dt_bias")}
+    one = {k: t[k][:, 2] for k in ("x", "dt", "b", "c", "gate")}  # rows of a longer sequence: batch strides
+    for off in (0, 1, 2):
+        st = flat[off:off + 960].view(3, 20, 16)
+        st.copy_(t["state"])
+        y = ops.state_scan_step(state=st, **one, **par, softplus=True)
+        other = t["state"].clone()
+        want = ops.state_scan_step(state=other, **{k: v.contiguous() for k, v in one.items()}, **par, softplus=True)
+        assert torch.equal(y, want) and torch.equal(st, other)
+
+
+@pytest.mark.parametrize("l, d", [(40, 48), (400, 10)])
+def test_scan_padding_is_never_read(l, d):
+    t = _scan_inputs(11, "bf16", 4, l, d, 16)
+    lens = [l, 0, 1, l // 2 + 3]
+    lengths = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    dirty = dict(t)
+    for k in ("x", "dt", "b", "c", "gate"):
+        dirty[k] = t[k].clone()
+        for i, n in enumerate(lens):
+            dirty[k][i, n:] = float("nan") if i % 2 else float("inf")
+    outs = []
+    for v in (t, dirty):
+        v = {k: x.detach().requires_grad_(True) for k, x in v.items()}
+        y, so = ops.state_scan(**v, softplus=True, lengths=lengths, return_state=True)
+        dy = torch.ones_like(y)
+        for i, n in enumerate(lens):
+            dy[i, n:] = float("nan")
+        outs.append((y, so, *torch.autograd.grad((y, so), list(v.values()), (dy, torch.ones_like(so)))))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b) and bool(torch.isfinite(a.float()).all())
+    assert torch.equal(outs[0][1][1], t["state"][1]), "an empty sequence leaves its state"
+
+
+def test_scan_decays_to_zero_and_stays_finite():
+    """Steps so wide that every decay underflows, and none at all: exp(-inf) = 0 and exp(0) = 1, no NaN either way."""
+    t = _scan_inputs(12, "fp32", 2, 40, 33, 16)
+    for dt in (1e4, 0.0):
+        v = dict(t, dt=torch.full_like(t["dt"], dt), dt_bias=None)
+        v = {k: x if x is None else x.detach().requires_grad_(True) for k, x in v.items()}
+        y, so = ops.state_scan(**v, return_state=True)
+        grads = torch.autograd.grad(y.sum() + so.sum(), [x for x in v.values() if x is not None])
+        assert all(bool(torch.isfinite(g).all()) for g in (y, so, *grads))
+        want = ref.scan(**v)
+        bound = ref.scan(**v, absolute=True)
+        ref.close(y, want["y"], bound["y"], 64 + 200, f"dt {dt}")
+        if dt == 0.0:
+            assert torch.equal(so, t["state"])
+
+
+def test_scan_strided_views_and_expanded_rows():
+    g = torch.Generator().manual_seed(8)
+    d, n, r = 40, 16, 3
+    proj = _rnd(g, 2, 35, 2 * d, dtype=torch.bfloat16)            # x | gate, as one projection leaves them
+    bcd = _rnd(g, 2, 35, r + 2 * n, dtype=torch.bfloat16)         # low-rank dt | b | c
+    t = _scan_inputs(8, "bf16", 2, 35, d, n)
+    v = dict(t, x=proj[..., :d], gate=proj[..., d:], b=bcd[..., r:r + n], c=bcd[..., r + n:], dt=t["dt"][:1, :1].expand(2, 35, d))
+    y, so = ops.state_scan(**v, softplus=True, return_state=True)
+    w = {k: x.contiguous() for k, x in v.items()}
+    y2, so2 = ops.state_scan(**w, softplus=True, return_state=True)
+    assert torch.equal(y, y2) and torch.equal(so, so2)
+    swapped = proj[..., :d].transpose(0, 1).contiguous().transpose(0, 1)  # time-major memory
+    assert torch.equal(ops.state_scan(**dict(v, x=swapped), softplus=True), y)
+    v["x"] = v["x"].transpose(1, 2).contiguous().transpose(1, 2)  # channels not contiguous: copied
+    assert torch.equal(ops.state_scan(**v, softplus=True), y)
+    x = proj.detach().requires_grad_(True)
+    (dp,) = torch.autograd.grad(ops.state_scan(**dict(v, x=x[..., :d], gate=x[..., d:]), softplus=True).float().sum(), [x])
+    parts = {k: w[k].detach().requires_grad_(True) for k in ("x", "gate")}
+    dx, dg = torch.autograd.grad(ops.state_scan(**dict(w, **parts), softplus=True).float().sum(), list(parts.values()))
+    assert torch.equal(dp, torch.cat([dx, dg], -1))
+
+
+def test_gradients_flow_through_the_state_between_parts():
+    """Two parts joined by their state have the gradients of the whole, for both operators."""
+    t = _scan_inputs(13, "fp32", 2, 50, 21, 6)
+    c = _conv_inputs(13, "fp32", 2, 50, 21, 4, True, True)
+    v = {k: x.requires_grad_(True) for k, x in t.items()}
+    seq = ("x", "dt", "b", "c", "gate")
+    dy = torch.randn(2, 50, 21, generator=torch.Generator().manual_seed(1)).cuda()
+    par = {k: v[k] for k in ("a", "d", "dt_bias")}
+    y1, st = ops.state_scan(**{k: v[k][:, :23] for k in seq}, **par, softplus=True, state=v["state"], return_state=True)
+    y2 = ops.state_scan(**{k: v[k][:, 23:] for k in seq}, **par, softplus=True, state=st)
+    got = dict(zip(v, torch.autograd.grad(torch.cat([y1, y2], 1), list(v.values()), dy)))
+    want, bound = ref.scan(**v, softplus=True, dy=dy), ref.scan(**v, softplus=True, dy=dy, absolute=True)
+    for k in v:
+        ref.close(got[k], want["d" + k], bound["d" + k], 160 + 12 * 50 + 4, "d" + k)
+    u = {k: x.requires_grad_(True) for k, x in c.items()}
+    y1, st = ops.causal_conv(u["x"][:, :2], u["w"], u["b"], "silu", state=u["state"], return_state=True)
+    y2 = ops.causal_conv(u["x"][:, 2:], u["w"], u["b"], "silu", state=st)
+    got = dict(zip(u, torch.autograd.grad(torch.cat([y1, y2], 1), list(u.values()), dy)))
+    want, bound = ref.conv(**u, act="silu", dy=dy), ref.conv(**u, act="silu", dy=dy, absolute=True)
+    for k in u:
+        ref.close(got[k], want["d" + k], bound["d" + k], 40 + 64 + 4, "d" + k)
+
+
+def test_same_bits_every_time():
+    t = _scan_inputs(14, "bf16", 2, 600, 80, 16)
+    v = {k: x.requires_grad_(True) for k, x in t.items()}
+    c = _conv_inputs(14, "bf16", 2, 600, 80, 4)
+    u = {k: c[k].requires_grad_(True) for k in ("x", "w", "b")}
+    runs = []
+    for _ in range(3):
+        y = ops.state_scan(**v, softplus=True)
+        z = ops.causal_conv(**u, activation="silu")
+        runs.append([y, *torch.autograd.grad(y, list(v.values()), torch.ones_like(y)),
+                     z, *torch.autograd.grad(z, list(u.values()), torch.ones_like(z))])
+    for r in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], r))
+
+
+@pytest.mark.parametrize("b, l, d", [(0, 5, 6), (2, 0, 6), (2, 5, 0)])
+def test_empty_batches_sequences_and_channels(b, l, d):
+    t = {k: x.requires_grad_(True) for k, x in _scan_inputs(1, "fp32", b, l, d, 4).items()}
+    y, so = ops.state_scan(**t, softplus=True, return_state=True)
+    assert y.shape == (b, l, d) and torch.equal(so, t["state"]) if l == 0 else so.shape == (b, d, 4)
+    grads = torch.autograd.grad((y, so), list(t.values()), (torch.zeros_like(y), torch.ones_like(so)))
+    assert all(g.shape == x.shape for g, x in zip(grads, t.values()))
+    if l == 0:
+        assert bool((grads[list(t).index("state")] == 1).all())
+    c = {k: x.requires_grad_(True) for k, x in _conv_inputs(1, "fp32", b, l, d, 4, True, True).items()}
+    y, so = ops.causal_conv(c["x"], c["w"], c["b"], state=c["state"], return_state=True)
+    assert y.shape == (b, l, d) and so.shape == (b, 3, d)
+    grads = torch.autograd.grad((y, so), list(c.values()), (torch.zeros_like(y), torch.ones_like(so)))
+    assert all(g.shape == x.shape for g, x in zip(grads, c.values()))
+    if l != 0:
+        with torch.no_grad():
+            assert ops.causal_conv_step(c["x"][:, 0], c["state"], c["w"], c["b"]).shape == (b, d)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the rows at the far end equal a short call that starts from the state in front of them."""
+    l, d, tail = 70000, 32768, 40
+    x = torch.empty(1, l, d, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(0))
+    g = torch.Generator().manual_seed(3)
+    w, bias = _rnd(g, d, 3), _rnd(g, d)
+    with torch.no_grad():
+        y = ops.causal_conv(x, w, bias, "silu")
+        short = ops.causal_conv(x[:, -tail:], w, bias, "silu", state=x[:, -tail - 2:-tail].contiguous())
+        assert torch.equal(y[:, -tail:], short)
+        del y
+        a = -torch.ones(d, 1, device="cuda")
+        b, c = _rnd(g, 1, l, 1, dtype=torch.bfloat16), _rnd(g, 1, l, 1, dtype=torch.bfloat16)
+        y, so = ops.state_scan(x, x, a, b, c, softplus=True, return_state=True)
+        # decays of at least exp(-softplus(x)): 400 tokens in front decide the state to far below a rounding
+        cut = 440
+        s2, _ = ops.state_scan(x[:, -cut:], x[:, -cut:], a, b[:, -cut:], c[:, -cut:], softplus=True, return_state=True)
+        diff = (y[:, -tail:].float() - s2[:, -tail:].float()).abs().max()
+        assert float(diff) <= 2.0 ** -7 * float(s2.float().abs().max())
+        assert bool((so != 0).any())
+
+
+# ---- norm and clipping -------------------------------------------------------------------------------------------------
+def _grads(seed, dtypes=("fp32", "bf16", "fp16"), count=40):
+    g = torch.Generator().manual_seed(seed)
+    sizes = [1, 2, 3, 7, 8, 15, 63, 1000, 16383, 16384, 16385, 40000, 100003]
+    return [_rnd(g, sizes[i % len(sizes)], scale=10.0 ** (-(i % 4)), dtype=TYPES[dtypes[i % len(dtypes)]]) for i in range(count)]
+
+
+def _norm64(ts, kind=2.0):
+    flat = torch.cat([t.detach().cpu().double().reshape(-1) for t in ts])
+    return float(torch.linalg.vector_norm(flat, kind))
+
+
+@pytest.mark.parametrize("count", [1, 13, 40, 128, 129, 300])
+@pytest.mark.parametrize("kind", [2.0, float("inf")])
+def test_global_norm(count, kind):
+    ts = _grads(count, count=count)
+    got, want = float(ops.global_norm(ts, kind)), _norm64(ts, kind)
+    assert abs(got - want) <= 2.0 ** -23 * want  # summed in float64, rounded once (plus the reference's own)
+
+
+def test_global_norm_far_values_views_and_order():
+    big = torch.full((1000,), 1e30, device="cuda")      # squares beyond float32
+    small = torch.full((1000,), 1e-30, device="cuda")   # squares below it
+    for t in (big, small):
+        assert abs(float(ops.global_norm([t])) - _norm64([t])) <= 2.0 ** -23 * _norm64([t])
+    base = torch.randn(5003, generator=torch.Generator().manual_seed(0)).cuda()
+    views = [base[1:], base[:5000].view(50, 100).t(), base[:5000].view(50, 100)[:, 3:50], base[::3], base[:1].expand(77),
+             base.bfloat16()[3:], base.half()[1:2]]
+    for v in views:
+        assert abs(float(ops.global_norm([v])) - _norm64([v])) <= 2.0 ** -23 * _norm64([v])
+    assert float(ops.global_norm([torch.zeros(0, device="cuda")])) == 0.0
+    assert float(ops.global_norm([torch.zeros(0, device="cuda"), torch.tensor(-3.0, device="cuda")])) == 3.0
+    for bad in (float("nan"), float("inf")):
+        for at in (0, 700, 5002):
+            t = base.clone()
+            t[at] = bad
+            for kind in (2.0, float("inf")):
+                got = float(ops.global_norm([base, t, base], kind))
+                assert got != got if bad != bad else got == bad
+
+
+@pytest.mark.parametrize("count", [1, 40, 97, 300])
+@pytest.mark.parametrize("share", [0.25, 1.5])
+@pytest.mark.parametrize("where", ["in place", "out"])
+def test_clip_gradients(count, share, where):
+    ts = _grads(count + 1, count=count)
+    before = [t.clone() for t in ts]
+    norm = _norm64(ts)
+    if where == "out":
+        out = [torch.full_like(t, 7.0) for t in ts]
+        got = ops.clip_gradients(ts, share * norm, out=out)
+        assert all(torch.equal(a, b) for a, b in zip(ts, before)), "inputs are left alone"
+    else:
+        out = ts
+        got = ops.clip_gradients(ts, share * norm)
+    assert abs(float(got) - norm) <= 2.0 ** -23 * norm
+    f = min(1.0, share * norm / (norm + 1e-6))
+    for o, b in zip(out, before):
+        if share > 1:
+            assert torch.equal(o, b)
+        else:
+            want = b.cpu().double() * f
+            ref.close(o, want, want, 2, "scaled")  # the factor (rounded to float32) and the product
+
+
+def test_clip_gradients_of_views_and_odd_places():
+    base = torch.randn(20000, generator=torch.Generator().manual_seed(2)).cuda()
+    for make in (lambda t: [t[1:9000], t[9000:]], lambda t: [t.view(100, 200).t()], lambda t: [t.view(100, 200)[:, 3:77]],
+                 lambda t: [t[::2]], lambda t: [t[:1], t[1:2], t[2:2]]):
+        t = base.clone()
+        views = make(t)
+        want = [v.clone().double() * (0.5 * _norm64(views) / (_norm64(views) + 1e-6)) for v in views]
+        rest = base.clone()
+        ops.clip_gradients(views, 0.5 * _norm64(views))
+        for v, w in zip(views, want):
+            ref.close(v, w.cpu(), w.cpu(), 2, "view")
+            v.copy_(make(rest)[[i for i, u in enumerate(views) if u is v][0]])
+        assert torch.equal(t, base), "nothing outside the views was touched"
+    src, dst = base[1:10001], torch.zeros(10004, device="cuda")  # source and destination differ in alignment
+    for off in (0, 1, 2, 3):
+        ops.clip_gradients([src], 0.5, out=[dst[off:off + 10000]])
+        want = src.cpu().double() * (0.5 / (_norm64([src]) + 1e-6))
+        ref.close(dst[off:off + 10000], want, want, 2, f"offset {off}")
+    with pytest.raises(ValueError):
+        ops.clip_gradients([base[:100], base[50:150]], 1.0)
+    t = base.clone()
+    t[5] = float("nan")
+    ops.clip_gradients([t], 1.0)
+    assert bool(torch.isnan(t).all())
+    t = base.clone()
+    t[5] = float("inf")
+    ops.clip_gradients([t], 1.0)
+    assert not t[:5].any() and not t[6:].any()
+
+
+def test_norm_and_clip_past_32_bits():
+    n = (1 << 31) + 12345
+    t = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    t[-1], t[1 << 31], t[0] = 3.0, 4.0, 12.0
+    assert float(ops.global_norm([t])) == 13.0
+    assert float(ops.clip_gradients([t], 6.5)) == 13.0
+    assert [float(t[i]) for i in (-1, 1 << 31, 0)] == [1.5, 2.0, 6.0]
+
+
+def test_fused_adam_clips_as_clip_then_step():
+    shapes = [(64, 1, 3, 3), (64,), (1,), (96, 64, 3, 3), (2, 320), (2,)]
+    g = torch.Generator().manual_seed(9)
+    p0 = [torch.randn(s, generator=g) for s in shapes]
+    mine = [torch.nn.Parameter(p.clone().cuda()) for p in p0]
+    theirs = [torch.nn.Parameter(p.clone().double()) for p in p0]
+    opt = ops.FusedAdam(mine, lr=1e-2, weight_decay=1e-3)
+    other = torch.optim.Adam(theirs, lr=1e-2, weight_decay=1e-3)
+    for step in range(4):
+        opt.zero_grad()
+        scale = 0.5
+        for p, q in zip(mine, theirs):
+            grad = torch.randn(p.shape, generator=g) * 10.0 ** (step - 2)
+            p.grad, q.grad = grad.cuda(), grad.double() * scale
+        norm = torch.nn.utils.clip_grad_norm_(theirs, 3.0)
+        other.step()
+        opt.step(grad_scale=scale, max_grad_norm=3.0)
+        assert abs(float(opt.last_grad_norm) - float(norm)) <= 2.0 ** -22 * float(norm)
+        for p, q in zip(mine, theirs):
+            # an update is at most lr; its relative error: two dozen float32 roundings
+            assert float((p.detach().cpu().double() - q.detach()).abs().max()) <= (step + 1) * 1e-2 * 2e-5 + 2.0 ** -22 * float(q.detach().abs().max())
+
+
+# ---- streams and graphs ------------------------------------------------------------------------------------------------
+def test_on_another_stream():
+    t = _scan_inputs(20, "bf16", 2, 500, 64, 16)
+    want = ops.state_scan(**t, softplus=True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.state_scan(**t, softplus=True)
+        n = ops.global_norm([got])
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want) and float(n) == float(ops.global_norm([want]))
+
+
+def test_two_streams_at_once_keep_apart():
+    ts = [_scan_inputs(30 + i, "bf16", 1, 800, 40, 16) for i in range(2)]
+    vs = [{k: x.requires_grad_(True) for k, x in t.items()} for t in ts]
+
+    def both(v):
+        y = ops.state_scan(**v, softplus=True)
+        return [y, *torch.autograd.grad(y, list(v.values()), torch.ones_like(y))]
+
+    want = [both(v) for v in vs]
+    streams = [torch.cuda.Stream() for _ in vs]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = both(vs[i])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def _capture(fn):
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        fn()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fn()
+    return graph, out
+
+
+def test_steps_in_a_graph_replay_with_new_inputs():
+    t = _scan_inputs(21, "bf16", 4, 6, 70, 16)
+    c = _conv_inputs(21, "bf16", 4, 6, 70, 4, True, True)
+    par = {k: t[k] for k in ("a", "d", "dt_bias")}
+    seq = ("dt", "b", "c", "gate")
+    live = {k: t[k][:, 0].clone() for k in seq + ("x",)}
+    cst, sst = c["state"].clone(), t["state"].clone()
+
+    def step():
+        x = ops.causal_conv_step(live["x"], cst, c["w"], c["b"], "silu")
+        return ops.state_scan_step(x, sst, live["dt"], par["a"], live["b"], live["c"], d=par["d"], gate=live["gate"],
+                                   dt_bias=par["dt_bias"], softplus=True)
+
+    graph, y = _capture(step)
+    cst.copy_(c["state"])
+    sst.copy_(t["state"])
+    ec, es = c["state"].clone(), t["state"].clone()
+    for i in range(6):
+        for k in live:
+            live[k].copy_(t[k][:, i])
+        graph.replay()
+        torch.cuda.synchronize()
+        x = ops.causal_conv_step(t["x"][:, i], ec, c["w"], c["b"], "silu")
+        want = ops.state_scan_step(x, es, t["dt"][:, i], par["a"], t["b"][:, i], t["c"][:, i], d=par["d"],
+                                   gate=t["gate"][:, i], dt_bias=par["dt_bias"], softplus=True)
+        assert torch.equal(y, want) and torch.equal(cst, ec) and torch.equal(sst, es), i
+
+
+def test_two_training_passes_and_a_clip_in_graphs():
+    """Two captured graphs, replayed in turn with eager work in between: neither disturbs the other's workspace."""
+    def build(seed):
+        t = {k: x.requires_grad_(True) for k, x in _scan_inputs(seed, "bf16", 1, 640, 48, 16).items()}
+        c = {k: x.requires_grad_(True) for k, x in _conv_inputs(seed, "bf16", 1, 640, 48, 4).items() if x is not None}
+        leaves = [*t.values(), *c.values()]
+        dy = torch.ones(1, 640, 48, dtype=torch.bfloat16, device="cuda")
+        outs = [torch.empty_like(x) for x in leaves]
+
+        def run():
+            y = ops.state_scan(**dict(t, x=ops.causal_conv(c["x"], c["w"], c["b"], "silu") + t["x"]), softplus=True)
+            grads = torch.autograd.grad(y, leaves, dy)
+            norm = ops.clip_gradients(grads, 1.0, out=outs)
+            return [y.detach(), norm, *outs]
+
+        return leaves, run
+
+    built = [build(s) for s in (40, 41)]
+    graphs = [_capture(run) for _, run in built]
+    for turn in range(4):
+        for (leaves, run), (graph, outs) in zip(built, graphs):
+            with torch.no_grad():
+                leaves[0].mul_(1.25 if turn % 2 else 0.75)
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [o.clone() for o in outs]
+            for o in outs[2:]:
+                o.zero_()
+            want = [o.clone() for o in run()]
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
+
+
+# ---- the operators together --------------------------------------------------------------------------------------------
+def _layer(t, c, x, lengths=None, states=(None, None)):
+    h, cs = ops.causal_conv(x, c["w"], c["b"], "silu", state=states[0], lengths=lengths, return_state=True)
+    y, ss = ops.state_scan(h, t["dt"], t["a"], t["b"], t["c"], d=t["d"], gate=t["gate"], dt_bias=t["dt_bias"], softplus=True,
+                           state=states[1], lengths=lengths, return_state=True)
+    return y, (cs, ss)
+
+
+def test_a_training_step_of_a_sequence_head():
+    """Convolution -> scan -> mean classifier -> loss -> backward -> clip inside Adam, against the formulas in float64."""
+    b, l, d, n = 4, 37, 24, 16
+    t = _scan_inputs(50, "fp32", b, l, d, n, state=False)
+    c = _conv_inputs(50, "fp32", b, l, d, 4)
+    g = torch.Generator().manual_seed(51)
+    wl, bl = _rnd(g, 2, d, scale=0.3), _rnd(g, 2)
+    params = {k: torch.nn.Parameter(v.clone()) for k, v in
+              dict(w=c["w"], cb=c["b"], a=t["a"], d=t["d"], dt_bias=t["dt_bias"], wl=wl, bl=bl).items()}
+    labels = torch.tensor([0, 1, 1, 0], device="cuda")
+    lengths = torch.tensor([37, 20, 1, 36], device="cuda")
+    opt = ops.FusedAdam(params.values(), lr=1e-2)
+    opt.zero_grad()
+    y, _ = _layer(dict(t, a=params["a"], d=params["d"], dt_bias=params["dt_bias"]), dict(w=params["w"], b=params["cb"]),
+                  c["x"], lengths)
+    logits = ops.linear_mean(y, params["wl"], params["bl"])
+    loss = ops.CrossEntropyLoss()(logits, labels)
+    loss.backward()
+    got = {k: p.grad.detach().clone() for k, p in params.items()}
+    opt.step(max_grad_norm=0.1)
+    # the same in float64
+    hc = ref.conv(c["x"], c["w"], c["b"], act="silu", lengths=lengths)["y"]
+    kw = dict(softplus=True, lengths=lengths)
+    y64 = ref.scan(hc, t["dt"], t["a"], t["b"], t["c"], t["d"], t["gate"], t["dt_bias"], **kw)["y"]
+    wl64, bl64 = wl.cpu().double(), bl.cpu().double()
+    lo = (y64 @ wl64.t() + bl64).mean(1)
+    p = torch.softmax(lo, -1)
+    dlo = (p - torch.nn.functional.one_hot(labels.cpu(), 2).double()) / b
+    assert abs(float(loss) + float(torch.log_softmax(lo, -1)[torch.arange(b), labels.cpu()].mean())) <= 1e-5
+    dy = (dlo @ wl64)[:, None, :].expand(b, l, d) / l
+    gs = ref.scan(hc, t["dt"], t["a"], t["b"], t["c"], t["d"], t["gate"], t["dt_bias"], dy=dy, **kw)
+    gc = ref.conv(c["x"], c["w"], c["b"], act="silu", lengths=lengths, dy=gs["dx"])
+    want = dict(w=gc["dw"], cb=gc["db"], a=gs["da"], d=gs["dd"], dt_bias=gs["ddt_bias"],
+                wl=dlo.t() @ y64.mean(1), bl=dlo.sum(0))
+    for k, v in want.items():
+        scale = float(v.abs().max())
+        # chains of a few hundred float32 roundings (37 steps, twice), errors adding up: 1000 x 2^-24 of the largest value
+        assert float((got[k].cpu().double() - v).abs().max()) <= 1000 * 2.0 ** -24 * scale + 1e-9, k
+    norm = float(torch.sqrt(sum(v.square().sum() for v in want.values())))
+    assert abs(float(opt.last_grad_norm) - norm) <= 1000 * 2.0 ** -24 * norm
+    assert all(bool(torch.isfinite(p).all()) for p in params.values())
+
+
+def test_a_recording_scored_as_it_arrives():
+    """A ragged batch of prompts with their states, then frame by frame: what the whole recordings give."""
+    b, l, d, n = 3, 30, 40, 16
+    t = _scan_inputs(60, "fp32", b, l, d, n, state=False)
+    c = _conv_inputs(60, "fp32", b, l, d, 4)
+    starts = [12, 5, 0]
+    with torch.no_grad():
+        whole, _ = _layer(t, c, c["x"])
+        y, (cs, ss) = _layer(t, c, c["x"], lengths=torch.tensor(starts, device="cuda"))
+        for i, s in enumerate(starts):
+            assert torch.equal(y[i, :s], whole[i, :s])
+        for k in range(18):
+            at = [s + k for s in starts]
+
+            def rows(v):
+                return torch.stack([v[i, p] for i, p in enumerate(at)])
+
+            h = ops.causal_conv_step(rows(c["x"]), cs, c["w"], c["b"], "silu")
+            yk = ops.state_scan_step(h, ss, rows(t["dt"]), t["a"], rows(t["b"]), rows(t["c"]), d=t["d"], gate=rows(t["gate"]),
+                                     dt_bias=t["dt_bias"], softplus=True)
+            want = rows(whole)
+            # the same steps in another kernel: sums of 16 products in another order, 30 tokens of decay
+            assert float((yk - want).abs().max()) <= (64 + 5 * 30) * 2.0 ** -23 * float(whole.abs().max())

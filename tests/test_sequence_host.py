@@ -1,0 +1,228 @@
+"""Argument checks of the sequence-layer entry points (no GPU needed: every refusal comes before the first launch)."""
+
+import pytest
+import torch
+
+from audiofakedetect import _native, ops
+
+
+def _conv(**kw):
+    args = dict(x=torch.zeros(2, 5, 6), w=torch.zeros(6, 4), b=torch.zeros(6))
+    args.update(kw)
+    return args
+
+
+def _scan(**kw):
+    args = dict(x=torch.zeros(2, 5, 6), dt=torch.zeros(2, 5, 6), a=torch.zeros(6, 4), b=torch.zeros(2, 5, 4),
+                c=torch.zeros(2, 5, 4))
+    args.update(kw)
+    return args
+
+
+@pytest.mark.parametrize("kw, err", [
+    (dict(x=torch.zeros(5, 6)), ValueError),
+    (dict(x=torch.zeros(2, 5, 6, dtype=torch.float64)), TypeError),
+    (dict(x=[1.0]), TypeError),
+    (dict(w=torch.zeros(7, 4)), ValueError),
+    (dict(w=torch.zeros(6, 1)), ValueError),
+    (dict(w=torch.zeros(6, 9)), ValueError),
+    (dict(w=torch.zeros(6, 4, dtype=torch.bfloat16), b=None), TypeError),  # neither float32 nor the type of x
+    (dict(w=None), TypeError),
+    (dict(b=torch.zeros(5)), ValueError),
+    (dict(b=torch.zeros(6, dtype=torch.float16)), TypeError),
+    (dict(activation="gelu"), ValueError),
+    (dict(state=torch.zeros(2, 4, 6)), ValueError),
+    (dict(state=torch.zeros(2, 3, 6, dtype=torch.bfloat16)), TypeError),
+    (dict(lengths=torch.zeros(3, dtype=torch.int32)), ValueError),
+    (dict(lengths=torch.zeros(2)), TypeError),
+    (dict(lengths=[1, 2]), TypeError),
+    (dict(), RuntimeError),  # fine, but on the CPU
+])
+def test_causal_conv_refuses(kw, err):
+    with pytest.raises(err):
+        ops.causal_conv(**_conv(**kw))
+
+
+@pytest.mark.parametrize("kw, err", [
+    (dict(x=torch.zeros(2, 5, 6)), ValueError),
+    (dict(state=None), TypeError),
+    (dict(state=torch.zeros(2, 2, 6)), ValueError),
+    (dict(state=torch.zeros(2, 6, 3).transpose(1, 2)), ValueError),
+    (dict(state_out=torch.zeros(2, 4, 6)), ValueError),
+    (dict(x=torch.zeros(2, 6, requires_grad=True)), RuntimeError),
+    (dict(), RuntimeError),
+])
+def test_causal_conv_step_refuses(kw, err):
+    args = dict(x=torch.zeros(2, 6), state=torch.zeros(2, 3, 6), w=torch.zeros(6, 4))
+    args.update(kw)
+    with pytest.raises(err):
+        ops.causal_conv_step(**args)
+
+
+@pytest.mark.parametrize("kw, err", [
+    (dict(dt=torch.zeros(2, 5, 7)), ValueError),
+    (dict(dt=None), TypeError),
+    (dict(dt=torch.zeros(2, 5, 6, dtype=torch.bfloat16)), TypeError),
+    (dict(a=torch.zeros(5, 4)), ValueError),
+    (dict(a=torch.zeros(6, 0), b=torch.zeros(2, 5, 0), c=torch.zeros(2, 5, 0)), ValueError),
+    (dict(a=torch.zeros(6, 65), b=torch.zeros(2, 5, 65), c=torch.zeros(2, 5, 65)), ValueError),
+    (dict(a=torch.zeros(6, 4, dtype=torch.bfloat16)), TypeError),
+    (dict(b=torch.zeros(2, 5, 3)), ValueError),
+    (dict(c=torch.zeros(2, 4, 4)), ValueError),
+    (dict(d=torch.zeros(7)), ValueError),
+    (dict(gate=torch.zeros(2, 5, 5)), ValueError),
+    (dict(dt_bias=torch.zeros(6, dtype=torch.float16)), TypeError),
+    (dict(state=torch.zeros(2, 6, 5)), ValueError),
+    (dict(state=torch.zeros(2, 6, 4, dtype=torch.bfloat16)), TypeError),
+    (dict(lengths=torch.zeros((2, 1), dtype=torch.int64)), ValueError),
+    (dict(), RuntimeError),
+])
+def test_state_scan_refuses(kw, err):
+    with pytest.raises(err):
+        ops.state_scan(**_scan(**kw))
+
+
+def test_state_scan_step_refuses():
+    def args(**kw):
+        a = dict(x=torch.zeros(2, 6), state=torch.zeros(2, 6, 4), dt=torch.zeros(2, 6), a=torch.zeros(6, 4),
+                 b=torch.zeros(2, 4), c=torch.zeros(2, 4))
+        a.update(kw)
+        return a
+
+    flat = torch.zeros(2 * 6 * 4 + 4)
+    for kw, err in ((dict(state=None), TypeError), (dict(b=torch.zeros(2, 5)), ValueError),
+                    (dict(state=torch.zeros(2, 4, 6).transpose(1, 2)), ValueError),
+                    (dict(state=flat[:48].view(2, 6, 4), state_out=flat[4:].view(2, 6, 4)), ValueError),  # overlap
+                    (dict(a=torch.zeros(6, 4, requires_grad=True)), RuntimeError), (dict(), RuntimeError)):
+        with pytest.raises(err):
+            ops.state_scan_step(**args(**kw))
+
+
+def test_global_norm_and_clip_refuse():
+    z = torch.zeros(8)
+    for bad in ([z, None], [z.double()], [z.to_sparse()], [torch.zeros(8, dtype=torch.int32)]):
+        with pytest.raises(TypeError):
+            ops.global_norm(bad)
+    with pytest.raises(ValueError):
+        ops.global_norm([z], norm_type=1.0)
+    with pytest.raises(RuntimeError):
+        ops.global_norm([z])
+    for kw in (dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(max_norm=1.0, out=[]),
+               dict(max_norm=1.0, out=[torch.zeros(7)])):
+        with pytest.raises(ValueError):
+            ops.clip_gradients([z], **kw)
+    with pytest.raises(TypeError):
+        ops.clip_gradients([z], 1.0, out=[torch.zeros(8, dtype=torch.float16)])
+    with pytest.raises(ValueError):  # elements that share memory
+        ops.clip_gradients([torch.zeros(1).expand(8)], 1.0)
+    assert float(ops.global_norm([])) == 0.0 and float(ops.clip_gradients([], 1.0)) == 0.0
+
+
+def test_clip_refuses_tensors_that_overlap():
+    flat = torch.zeros(32)
+    a, b, c = flat[:16], flat[16:], flat[8:24]
+    ops._check_disjoint([a, b], [a, b])                       # in place, side by side
+    ops._check_disjoint([a], [torch.zeros(16)])
+    ops._check_disjoint([a, a], [torch.zeros(16), torch.zeros(16)])  # read twice, written apart
+    for src, dst in (([a, a], [a, a]), ([a, c], [a, c]), ([a], [c]), ([a, b], [b, a]), ([a, c], [torch.zeros(16), c])):
+        with pytest.raises(ValueError):
+            ops._check_disjoint(src, dst)
+
+
+def test_workspace_sizes_are_those_of_the_layout():
+    lib = _native.load()
+    # forward with enough rows: no time segments, no workspace; few rows and a long axis: segment states
+    assert lib.afd_state_scan_workspace_bytes(128, 101, 1024, 16, 0) == 0
+    assert lib.afd_state_scan_workspace_bytes(1, 16384, 1024, 16, 0) > 0
+    assert lib.afd_state_scan_workspace_bytes(0, 1, 1, 1, 0) == 0
+    assert lib.afd_state_scan_checkpoint_floats(2, 17, 5, 3) == 2 * 2 * 5 * 4
+    assert lib.afd_causal_conv_backward_workspace_bytes(2, 65, 6, 4) == 2 * 2 * 6 * 5 * 4
+
+
+def test_c_entries_refuse_bad_sizes():
+    lib = _native.load()
+    import ctypes
+
+    one = ctypes.c_void_p(16)  # never dereferenced: the sizes are refused first
+    strides = (_native.c_l * 12)()
+    assert lib.afd_causal_conv_forward(one, 1, 1, one, None, 1, None, None, one, None, 1, 1, 1, 9, 0, 0, None) == -1
+    assert b"9 (2..8)" in lib.afd_last_error()
+    assert lib.afd_causal_conv_forward(one, 1, 1, one, None, 1, None, None, one, None, 0, 1, 1, 4, 0, 0, None) == -1
+    assert lib.afd_causal_conv_backward(one, 1, 1, one, None, 1, None, None, one, 1, 1, None, one, one, None, None, 1, 1, 1,
+                                        4, 0, 0, None, 0, None) == -4
+    assert lib.afd_state_scan_forward(one, one, one, one, None, strides, one, None, None, None, None, one, None, None, 1, 1,
+                                      1, 65, 1, 0, None, 0, None) == -1
+    assert lib.afd_state_scan_forward(one, one, one, one, None, strides, one, None, None, None, None, one, None, None, 1,
+                                      16384, 64, 16, 1, 0, None, 0, None) == -4
+    assert lib.afd_state_scan_forward(one, one, one, one, None, strides, one, None, None, None, None, one, None, None, 1, 1,
+                                      1, 1, 1, 7, None, 0, None) == -1
+    assert lib.afd_global_norm(None, None, None, 1, 0, 1.0, 1.0, one, None, 0, None) == -1
+    assert lib.afd_global_norm(None, None, None, 0, 0, 1.0, 1.0, one, None, 0, None) == -4
+    assert lib.afd_adam_step_clipped(one, one, one, one, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, None, None) == -1
+
+
+def test_trainer_flag():
+    import argparse
+
+    from audiofakedetect.utils import add_default_parser_args
+
+    parser = add_default_parser_args(argparse.ArgumentParser())
+    assert parser.parse_args([]).clip_grad_norm is None
+    assert parser.parse_args(["--clip-grad-norm", "0.5"]).clip_grad_norm == 0.5
+
+
+# ---- the float64 restatements the GPU tests compare with: their gradients against differences ---------------------------
+def _differences(f, t, dy, eps=1e-6):
+    """d <dy, f> / dt by central differences, element by element."""
+    out = torch.zeros_like(t)
+    flat, o = t.view(-1), out.view(-1)
+    for i in range(flat.numel()):
+        keep = float(flat[i])
+        flat[i] = keep + eps
+        hi = float((f() * dy).sum())
+        flat[i] = keep - eps
+        lo = float((f() * dy).sum())
+        flat[i] = keep
+        o[i] = (hi - lo) / (2 * eps)
+    return out
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_reference_conv_gradients_are_the_differences(act):
+    import sequence_ref as ref
+
+    g = torch.Generator().manual_seed(1)
+    t = dict(x=torch.randn(2, 5, 3, generator=g).double(), w=torch.randn(3, 3, generator=g).double(),
+             b=torch.randn(3, generator=g).double(), state=torch.randn(2, 2, 3, generator=g).double())
+    dy = torch.randn(2, 5, 3, generator=g).double()
+    lengths = torch.tensor([5, 1])
+    got = ref.conv(**t, act=act, lengths=lengths, dy=dy)
+    for name in t:
+        diff = _differences(lambda: ref.conv(**t, act=act, lengths=lengths)["y"], t[name], dy)
+        assert (got["d" + name] - diff).abs().max() < 1e-7, name
+    ds = torch.randn(2, 2, 3, generator=g).double()
+    got = ref.conv(**t, act=act, lengths=lengths, dy=torch.zeros_like(dy), dstate_out=ds)
+    for name in ("x", "state"):
+        diff = _differences(lambda: ref.conv(**t, act=act, lengths=lengths)["state"], t[name], ds)
+        assert (got["d" + name] - diff).abs().max() < 1e-7, name
+
+
+def test_reference_scan_gradients_are_the_differences():
+    import sequence_ref as ref
+
+    g = torch.Generator().manual_seed(2)
+
+    def rnd(*s):
+        return torch.randn(*s, generator=g).double()
+
+    t = dict(x=rnd(2, 4, 3), dt=rnd(2, 4, 3), a=-rnd(3, 2).abs(), b=rnd(2, 4, 2), c=rnd(2, 4, 2), d=rnd(3), gate=rnd(2, 4, 3),
+             dt_bias=rnd(3), state=rnd(2, 3, 2))
+    dy, ds = rnd(2, 4, 3), rnd(2, 3, 2)
+    lengths = torch.tensor([4, 2])
+    got = ref.scan(**t, softplus=True, lengths=lengths, dy=dy)
+    late = ref.scan(**t, softplus=True, lengths=lengths, dy=torch.zeros_like(dy), dstate_out=ds)
+    for name in t:
+        diff = _differences(lambda: ref.scan(**t, softplus=True, lengths=lengths)["y"], t[name], dy)
+        assert (got["d" + name] - diff).abs().max() < 1e-7, name
+        diff = _differences(lambda: ref.scan(**t, softplus=True, lengths=lengths)["state"], t[name], ds)
+        assert (late["d" + name] - diff).abs().max() < 1e-7, name
