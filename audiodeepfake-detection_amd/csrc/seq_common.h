@@ -25,22 +25,18 @@ __device__ __forceinline__ float sigmoid_f32(float x) {
 }
 
 // log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1].  The step widths of a state-space layer start at
-// 1e-3 .. 1e-1, where log(1 + e) taken at face value has lost ten bits: log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3,
-// as its odd series up to s^15 (the next term is 2 s^17 / 17 < 1e-9 of the sum).
+// 1e-3 .. 1e-1, where log(1 + e) taken at face value has lost ten bits: log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, and
+// 2 atanh(s) / s as a polynomial in s^2 on [0, 1/9], fitted for the least relative error (8e-9, an eighth of a rounding).
 __device__ __forceinline__ float softplus_f32(float x) {
     const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(x));
     const float s = e * __builtin_amdgcn_rcpf(2.f + e);
     const float q = s * s;
-    float p = 1.f / 15.f;
-    p = fmaf(p, q, 1.f / 13.f);
-    p = fmaf(p, q, 1.f / 11.f);
-    p = fmaf(p, q, 1.f / 9.f);
-    p = fmaf(p, q, 1.f / 7.f);
-    p = fmaf(p, q, 1.f / 5.f);
-    p = fmaf(p, q, 1.f / 3.f);
-    p = fmaf(p, q, 1.f);
-    // (x = NaN: fmaxf would drop it)
-    return (x > 0.f ? x : 0.f * x) + 2.f * s * p;
+    float p = 0.28178325f;
+    p = fmaf(p, q, 0.27960604f);
+    p = fmaf(p, q, 0.40024909f);
+    p = fmaf(p, q, 0.66666317f);
+    p = fmaf(p, q, 2.f);
+    return fmaf(s, p, fmaxf(x, 0.f));  // (NaN comes in through e)
 }
 
 // Sums of the columns of part[rows][cols]: each workgroup takes 64 columns, its 16 waves take every 16th row and meet in LDS.

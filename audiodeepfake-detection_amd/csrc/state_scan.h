@@ -18,7 +18,9 @@
 
 namespace afd {
 
-constexpr int kTok = 16;       // tokens per block
+constexpr int kTokF = 16;      // tokens per block, forward
+constexpr int kTokB = 8;       // ... and backward, where a block's states and decays stay in registers
+constexpr int kCkpt = kTokB;   // tokens between the states that the forward keeps for the backward
 constexpr int kScanT = 256;    // threads per workgroup: 4 waves
 
 struct ScanArgs {
@@ -28,11 +30,11 @@ struct ScanArgs {
     const int* lengths;
     void* y;
     float* state_out;
-    float* ckpt;  // [B][ceil(L / 16)][D][NP]: the state in front of every block of 16 tokens (written for training)
+    float* ckpt;  // [B][ceil(L / kCkpt)][D][NP]: the state in front of every kCkpt tokens (written for training)
     float* seg_h;  // [B][S][D][NP]: what a time segment leaves on its own (forward: state, backward: gradient)
     float* seg_d;  // [B][S][D]: the segment's sum of delta
     int B, L, D, N, softplus;
-    int S, seg_blocks;  // time segments and blocks per segment
+    int S, seg;  // time segments and tokens per segment (a multiple of kTokF)
     int nb;             // workgroups per row of channels
     // backward only
     const float* dstate_out;
@@ -101,6 +103,33 @@ template <int Q> __device__ __forceinline__ float sum_lanes(float v) {
     return v;
 }
 
+// Sums of v[0 .. Q) over the Q lanes of a channel; lane q gets that of v[q].  Every step halves the values, so it takes
+// 3 (Q - 1) instructions where summing each in full and picking one's own takes Q (log2 Q + 1).
+template <int Q> __device__ __forceinline__ float scatter_lanes(float (&v)[Q]) {
+    const int q = threadIdx.x & (Q - 1);
+    if constexpr (Q == 16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // row_mirror: lane q meets lane 15 - q
+            const float lo = v[i] + dpp<0x140>(v[i]), hi = v[i + 8] + dpp<0x140>(v[i + 8]);
+            v[i] = (q & 8) ? hi : lo;
+        }
+    }
+    if constexpr (Q >= 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // row_half_mirror: q meets 7 - q
+            const float lo = v[i] + dpp<0x141>(v[i]), hi = v[i + 4] + dpp<0x141>(v[i + 4]);
+            v[i] = (q & 4) ? hi : lo;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // quad_perm [2, 3, 0, 1]
+        const float lo = v[i] + dpp<0x4e>(v[i]), hi = v[i + 2] + dpp<0x4e>(v[i + 2]);
+        v[i] = (q & 2) ? hi : lo;
+    }
+    const float lo = v[0] + dpp<0xb1>(v[0]), hi = v[1] + dpp<0xb1>(v[1]);  // quad_perm [1, 0, 3, 2]
+    return (q & 1) ? hi : lo;
+}
+
 template <int NS> struct Vec;
 template <> struct Vec<1> { typedef float type; };
 template <> struct Vec<2> { typedef float type __attribute__((ext_vector_type(2))); };
@@ -141,48 +170,73 @@ __device__ __forceinline__ int scan_rows(const int* lengths, int b, int L) {
     return n < 0 ? 0 : (n > L ? L : n);
 }
 
+// Loads go to a uniform base (advanced by scalar instructions) plus a 32-bit byte offset of the lane that never changes, so
+// an element costs one instruction.  A full block reads without looking; in the last block of a sequence rows behind it are
+// replaced by its last row, and the caller puts zeros in the place of what they give.
+template <typename T> __device__ __forceinline__ T load_at(const T* base, unsigned off) {
+    return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + off);
+}
+
 // The b and c rows of one block on their way into LDS: E values per thread, fetched early and written late.
-template <typename T, int NP> struct BcStage {
-    static constexpr int kAll = kTok * 2 * NP;
+template <typename T, int NP, int TOK> struct BcStage {
+    static constexpr int kAll = TOK * 2 * NP;
     static constexpr int E = (kAll + kScanT - 1) / kScanT;
     T v[E];
+    // thread's element e: token (e kScanT + tid) / (2 NP), column of [b | c] the rest
+    static __device__ __forceinline__ int tok(int e) { return (e * kScanT + (int)threadIdx.x) / (2 * NP); }
+    static __device__ __forceinline__ int col() { return (int)threadIdx.x % (2 * NP); }  // 2 NP divides kScanT
     __device__ __forceinline__ void fetch(const ScanArgs& p, const T* brow, const T* crow, int t0, int n) {
+        const bool is_c = col() >= NP;
+        const int s = min(is_c ? col() - NP : col(), p.N - 1);
+        const T* base = is_c ? crow : brow;
+        const long row = is_c ? p.cl : p.bl;
+        if (t0 + TOK <= n) {
+            base += (size_t)t0 * row;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = e * kScanT + (int)threadIdx.x;
-            const int tok = i / (2 * NP), col = i % (2 * NP);
-            const int s = col % NP;
-            v[e] = (T)0.f;
-            if (i < kAll && s < p.N && t0 + tok < n) {
-                v[e] = col < NP ? brow[(size_t)(t0 + tok) * p.bl + s] : crow[(size_t)(t0 + tok) * p.cl + s];
+            for (int e = 0; e < E; ++e) v[e] = base[(unsigned)min(tok(e), TOK - 1) * (unsigned)row + (unsigned)s];
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int t = min(t0 + min(tok(e), TOK - 1), n - 1);
+                v[e] = base[(size_t)t * row + s];
             }
         }
     }
-    __device__ __forceinline__ void put(float* lds) const {
+    __device__ __forceinline__ void put(float* lds, int t0, int n, int N) const {
+        const int s = col() >= NP ? col() - NP : col();
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int i = e * kScanT + (int)threadIdx.x;
-            if (i < kAll) lds[i] = to_f32(v[e]);
+            if (kAll % kScanT == 0 || i < kAll) lds[i] = (s < N && t0 + tok(e) < n) ? to_f32(v[e]) : 0.f;
         }
     }
 };
 
-// Tokens q, q + Q, ... of a block for this lane's channel (zero behind row n, so what lies there is never used).
-template <typename T, int Q> struct TokLoad {
-    static constexpr int R = kTok / Q;
+// Tokens q, q + Q, ... of a block for this lane's channel.
+template <typename T, int Q, int TOK> struct TokLoad {
+    static constexpr int R = TOK > Q ? TOK / Q : 1;
     T v[R];
-    __device__ __forceinline__ void fetch(const T* col, long row, int t0, int q, int n, bool live) {
+    // col: the row of token t0 (uniform); off: byte offset of (token q, channel); qr = the lane's token, row = row stride
+    __device__ __forceinline__ void full(const T* base, long row, unsigned off) {
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int t = t0 + i * Q + q;
-            v[i] = (T)0.f;
-            if (live && t < n) v[i] = col[(size_t)t * row];
-        }
+        for (int i = 0; i < R; ++i) v[i] = load_at(base + (size_t)(i * Q) * row, off);
+    }
+    __device__ __forceinline__ void tail(const T* base, long row, int left, int q, unsigned chan) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) v[i] = load_at(base + (size_t)min(i * Q + q, left - 1) * row, chan);
     }
 };
+
+// The loads under way have arrived.  Stores count with loads and complete in order: a block that starts right behind the
+// stores of the one before it would wait for those too when it takes its loaded values, so the wait comes in front of them.
+__device__ __forceinline__ void loads_arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+
+// No LDS access moves across: left to itself the compiler puts each token's rows right in front of their use and waits for
+// them there, once or twice a token.
+__device__ __forceinline__ void hold_lds() { __builtin_amdgcn_sched_barrier(0); }
 
 struct ScanPlace {
-    int b, s, cb, ch, q, n0, n;
+    int b, s, cb, ch, cl, q, n0, n;  // cl: the channel, or the last one for lanes behind it (they load and compute along)
     bool live;
 };
 // workgroup id -> (row of the batch, time segment, block of channels), channel blocks fastest
@@ -196,6 +250,7 @@ template <int Q, int NS> __device__ __forceinline__ ScanPlace scan_place(const S
     w.q = threadIdx.x & (Q - 1);
     w.ch = w.cb * (kScanT / Q) + (int)threadIdx.x / Q;
     w.live = w.ch < p.D;
+    w.cl = min(w.ch, p.D - 1);
     w.n0 = w.q * NS;
     w.n = scan_rows(p.lengths, w.b, p.L);
     return w;

@@ -7,30 +7,29 @@ using namespace afd;
 
 // LOCAL: the walk of a time segment from a zero state, leaving only its end state and its sum of delta (the decay over the
 // whole segment is exp(a sum delta)).  Otherwise the full walk; with more than one segment it first carries the state
-// over the segments in front of it, S fused multiply-adds per state.
+// over the segments in front of it, one exponential and one multiply-add per state and segment.
 template <typename T, int Q, int NS, bool LOCAL>
 __global__ void __launch_bounds__(kScanT) scan_fwd_kernel(const ScanArgs p) {
-    constexpr int NP = Q * NS, R = kTok / Q;
-    __shared__ float lds[2][kTok * 2 * NP];
+    constexpr int NP = Q * NS, R = kTokF / Q;
+    __shared__ float lds[2][kTokF * 2 * NP];
     const ScanPlace w = scan_place<Q, NS>(p);
-    const int nblk = (w.n + kTok - 1) / kTok;
-    const int blk0 = w.s * p.seg_blocks;
-    const int blk1 = min(blk0 + p.seg_blocks, nblk);
-    if (LOCAL && blk1 * kTok >= w.n) return;  // the last segment with tokens (and all behind it): nobody asks
-    const size_t seg = ((size_t)w.b * p.S + w.s) * p.D + w.ch;
+    const int start = w.s * p.seg;
+    const int end = min(start + p.seg, w.n);  // tokens [start, end) are this segment's
+    if (LOCAL && end >= w.n) return;  // the last segment with tokens (and all behind it): nobody asks
+    const size_t seg = ((size_t)w.b * p.S + w.s) * p.D + w.cl;
 
     float a2[NS], h[NS];
-    load_states<NS>(p.a + (size_t)w.ch * p.N, w.n0, p.N, w.live, a2);
+    load_states<NS>(p.a + (size_t)w.cl * p.N, w.n0, p.N, true, a2);
 #pragma unroll
     for (int k = 0; k < NS; ++k) {
         a2[k] *= kLog2e;
         h[k] = 0.f;
     }
     if (!LOCAL) {
-        load_states<NS>(p.state ? p.state + ((size_t)w.b * p.D + w.ch) * p.N : nullptr, w.n0, p.N, w.live, h);
-        if (w.live && blk0 < nblk) {
+        load_states<NS>(p.state ? p.state + ((size_t)w.b * p.D + w.cl) * p.N : nullptr, w.n0, p.N, true, h);
+        if (start < w.n) {
             for (int s = 0; s < w.s; ++s) {
-                const size_t at = ((size_t)w.b * p.S + s) * p.D + w.ch;
+                const size_t at = ((size_t)w.b * p.S + s) * p.D + w.cl;
                 float e[NS];
                 load_vec<NS>(p.seg_h + at * NP + w.n0, e);
                 const float sd = p.seg_d[at];
@@ -39,57 +38,86 @@ __global__ void __launch_bounds__(kScanT) scan_fwd_kernel(const ScanArgs p) {
             }
         }
     }
-    const float bias = (p.dt_bias && w.live) ? p.dt_bias[w.ch] : 0.f;
-    const float dskip = (!LOCAL && p.d && w.live) ? p.d[w.ch] : 0.f;
-    const T* xc = static_cast<const T*>(p.x) + (size_t)w.b * p.xb + w.ch;
-    const T* tc = static_cast<const T*>(p.dt) + (size_t)w.b * p.tb + w.ch;
-    const T* gc = p.gate ? static_cast<const T*>(p.gate) + (size_t)w.b * p.gb + w.ch : nullptr;
+    const float bias = p.dt_bias ? p.dt_bias[w.cl] : 0.f;
+    const float dskip = (!LOCAL && p.d) ? p.d[w.cl] : 0.f;
+    const bool gated = !LOCAL && p.gate;
+    const T* xb = static_cast<const T*>(p.x) + (size_t)w.b * p.xb;
+    const T* tb = static_cast<const T*>(p.dt) + (size_t)w.b * p.tb;
+    const T* gb = gated ? static_cast<const T*>(p.gate) + (size_t)w.b * p.gb : nullptr;
     const T* br = static_cast<const T*>(p.b) + (size_t)w.b * p.bb;
     const T* cr = static_cast<const T*>(p.c) + (size_t)w.b * p.cb;
-    T* yc = LOCAL ? nullptr : static_cast<T*>(p.y) + (size_t)w.b * p.L * p.D + w.ch;
+    T* yb = LOCAL ? nullptr : static_cast<T*>(p.y) + (size_t)w.b * p.L * p.D;
+    const unsigned chan = (unsigned)w.cl * sizeof(T);
+    const unsigned xo = chan + (unsigned)(w.q * p.xl * sizeof(T)), to = chan + (unsigned)(w.q * p.tl * sizeof(T));
+    const unsigned go = gated ? chan + (unsigned)(w.q * p.gl * sizeof(T)) : 0u;
+    const unsigned yo = chan + (unsigned)(w.q * p.D * sizeof(T));
     float sum_delta = 0.f;
 
-    BcStage<T, NP> bc;
-    TokLoad<T, Q> nx, nt, ng;
-    if (blk0 < blk1) {
-        bc.fetch(p, br, cr, blk0 * kTok, w.n);
-        nx.fetch(xc, p.xl, blk0 * kTok, w.q, w.n, w.live);
-        nt.fetch(tc, p.tl, blk0 * kTok, w.q, w.n, w.live);
-        if (!LOCAL && gc) ng.fetch(gc, p.gl, blk0 * kTok, w.q, w.n, w.live);
-        bc.put(lds[0]);
+    BcStage<T, NP, kTokF> bc;
+    TokLoad<T, Q, kTokF> nx, nt, ng;
+    auto fetch = [&](int t0) {
+        bc.fetch(p, br, cr, t0, w.n);
+        const int left = w.n - t0;
+        if (left >= kTokF) {
+            nx.full(xb + (size_t)t0 * p.xl, p.xl, xo);
+            nt.full(tb + (size_t)t0 * p.tl, p.tl, to);
+            if (gated) ng.full(gb + (size_t)t0 * p.gl, p.gl, go);
+        } else {
+            nx.tail(xb + (size_t)t0 * p.xl, p.xl, left, w.q, chan);
+            nt.tail(tb + (size_t)t0 * p.tl, p.tl, left, w.q, chan);
+            if (gated) ng.tail(gb + (size_t)t0 * p.gl, p.gl, left, w.q, chan);
+        }
+    };
+    if (start < end) {
+        fetch(start);
+        bc.put(lds[0], start, w.n, p.N);
     }
     __syncthreads();
-    for (int blk = blk0; blk < blk1; ++blk) {
-        const int t0 = blk * kTok;
-        const float* row = lds[(blk - blk0) & 1] + w.n0;
+    int turn = 0;
+    for (int t0 = start; t0 < end; t0 += kTokF, turn ^= 1) {
+        const float* row = lds[turn] + w.n0;
         float dl[R], dx[R], xv[R], gv[R], yv[R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const bool in = t0 + i * Q + w.q < w.n;
             xv[i] = to_f32(nx.v[i]);
             const float raw = to_f32(nt.v[i]) + bias;
-            const float de = p.softplus ? softplus_f32(raw) : raw;
-            dl[i] = in ? de : 0.f;  // exp(0) = 1 and nothing added: the state holds behind row n
+            dl[i] = p.softplus ? softplus_f32(raw) : raw;
             dx[i] = dl[i] * xv[i];
-            sum_delta += dl[i];
-            yv[i] = 0.f;
-            if (!LOCAL && gc) gv[i] = to_f32(ng.v[i]);
+            if (gated) gv[i] = to_f32(ng.v[i]);
         }
-        if (blk + 1 < blk1) {
-            bc.fetch(p, br, cr, t0 + kTok, w.n);
-            nx.fetch(xc, p.xl, t0 + kTok, w.q, w.n, w.live);
-            nt.fetch(tc, p.tl, t0 + kTok, w.q, w.n, w.live);
-            if (!LOCAL && gc) ng.fetch(gc, p.gl, t0 + kTok, w.q, w.n, w.live);
-        }
-        if (!LOCAL && p.ckpt && w.live)
-            store_vec<NS>(p.ckpt + (((size_t)w.b * ((p.L + kTok - 1) / kTok) + blk) * p.D + w.ch) * NP + w.n0, h);
+        if (t0 + kTokF > w.n) {  // exp(0) = 1 and nothing added: the state holds behind row n
 #pragma unroll
-        for (int j = 0; j < kTok; ++j) {
+            for (int i = 0; i < R; ++i) {
+                const bool in = t0 + i * Q + w.q < w.n;
+                dl[i] = in ? dl[i] : 0.f;
+                dx[i] = in ? dx[i] : 0.f;
+            }
+        }
+        if (LOCAL) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) sum_delta += dl[i];
+        }
+        if (t0 + kTokF < end) fetch(t0 + kTokF);
+        float part[Q], nb[NS], nc[NS];  // nb, nc: the next token's rows, asked for one token ahead
+        load_vec<NS>(row, nb);
+        if (!LOCAL) load_vec<NS>(row + NP, nc);
+#pragma unroll
+        for (int j = 0; j < kTokF; ++j) {
+            if (!LOCAL && j % kCkpt == 0 && p.ckpt && w.live && t0 + j < w.n)
+                store_vec<NS>(p.ckpt + (((size_t)w.b * ((p.L + kCkpt - 1) / kCkpt) + (t0 + j) / kCkpt) * p.D + w.ch) * NP + w.n0, h);
             const int i = j / Q, ql = j % Q;
             const float de = from_lane<Q>(dl[i], ql), dxj = from_lane<Q>(dx[i], ql);
             float bv[NS], cv[NS], y = 0.f;
-            load_vec<NS>(row + j * 2 * NP, bv);
-            if (!LOCAL) load_vec<NS>(row + j * 2 * NP + NP, cv);
+#pragma unroll
+            for (int k = 0; k < NS; ++k) {
+                bv[k] = nb[k];
+                if (!LOCAL) cv[k] = nc[k];
+            }
+            if (j + 1 < kTokF) {
+                load_vec<NS>(row + (j + 1) * 2 * NP, nb);
+                if (!LOCAL) load_vec<NS>(row + (j + 1) * 2 * NP + NP, nc);
+                hold_lds();
+            }
 #pragma unroll
             for (int k = 0; k < NS; ++k) {
                 const float e = __builtin_amdgcn_exp2f(de * a2[k]);
@@ -97,20 +125,35 @@ __global__ void __launch_bounds__(kScanT) scan_fwd_kernel(const ScanArgs p) {
                 if (!LOCAL) y = fmaf(cv[k], h[k], y);
             }
             if (!LOCAL) {
-                y = sum_lanes<Q>(y);
-                yv[i] = w.q == ql ? y : yv[i];
+                part[ql] = y;
+                if (ql == Q - 1) yv[i] = scatter_lanes<Q>(part);
             }
         }
         if (!LOCAL) {
+            loads_arrived();
+            T out[R];
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                const int t = t0 + i * Q + w.q;
                 float y = fmaf(dskip, xv[i], yv[i]);
-                if (gc) y *= gv[i] * sigmoid_f32(gv[i]);
-                if (w.live && t < p.L) yc[(size_t)t * p.D] = from_f32<T>(t < w.n ? y : 0.f);
+                if (gated) y *= gv[i] * sigmoid_f32(gv[i]);
+                out[i] = from_f32<T>(y);
+            }
+            T* yt = yb + (size_t)t0 * p.D;
+            if (t0 + kTokF <= w.n) {
+                if (w.live) {
+#pragma unroll
+                    for (int i = 0; i < R; ++i)
+                        *reinterpret_cast<T*>(reinterpret_cast<char*>(yt + (size_t)(i * Q) * p.D) + yo) = out[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const int t = t0 + i * Q + w.q;
+                    if (w.live && t < p.L) yb[(size_t)t * p.D + w.ch] = t < w.n ? out[i] : from_f32<T>(0.f);
+                }
             }
         }
-        if (blk + 1 < blk1) bc.put(lds[(blk + 1 - blk0) & 1]);
+        if (t0 + kTokF < end) bc.put(lds[turn ^ 1], t0 + kTokF, w.n, p.N);
         __syncthreads();
     }
     if (LOCAL) {
@@ -122,12 +165,13 @@ __global__ void __launch_bounds__(kScanT) scan_fwd_kernel(const ScanArgs p) {
         return;
     }
     // rows behind the last token, and the state behind it (by the segment that holds it, or the first if there is none)
-    const int tail0 = max(blk0, blk1) * kTok, tail1 = min((blk0 + p.seg_blocks) * kTok, p.L);
-    for (int t = tail0 + w.q; t < tail1; t += Q)
-        if (w.live) yc[(size_t)t * p.D] = from_f32<T>(0.f);
-    const int last = nblk > 0 ? (nblk - 1) / p.seg_blocks : 0;
+    const int done = start < end ? start + (end - start + kTokF - 1) / kTokF * kTokF : start;
+    const int stop = min(start + p.seg, p.L);
+    for (int t = done + w.q; t < stop; t += Q)
+        if (w.live) yb[(size_t)t * p.D + w.ch] = from_f32<T>(0.f);
+    const int last = w.n > 0 ? (w.n - 1) / p.seg : 0;
     if (p.state_out && w.s == last)
-        store_states<NS>(p.state_out + ((size_t)w.b * p.D + w.ch) * p.N, w.n0, p.N, w.live, h);
+        store_states<NS>(p.state_out + ((size_t)w.b * p.D + w.cl) * p.N, w.n0, p.N, w.live, h);
 }
 
 template <typename T, int Q, int NS> int launch(const ScanArgs& p, hipStream_t s) {
@@ -155,7 +199,7 @@ __global__ void __launch_bounds__(kScanT) scan_step_kernel(const ScanArgs p) {
     float a2[NS], h[NS], bv[NS], cv[NS];
     const T* br = static_cast<const T*>(p.b) + (size_t)w.b * p.bb;
     const T* cr = static_cast<const T*>(p.c) + (size_t)w.b * p.cb;
-    if (p.N == Q * NS && p.seg_blocks) {  // unpadded rows on 16-byte boundaries (seg_blocks: what the host found)
+    if (p.N == Q * NS && p.seg) {  // unpadded rows on 16-byte boundaries (seg: what the host found)
         load_vec<NS>(p.state + st + w.n0, h);
         load_vec<NS>(p.a + (size_t)w.ch * p.N + w.n0, a2);
     } else {
@@ -177,7 +221,7 @@ __global__ void __launch_bounds__(kScanT) scan_step_kernel(const ScanArgs p) {
         y = fmaf(cv[k], h[k], y);
     }
     y = sum_lanes<Q>(y);
-    if (p.N == Q * NS && p.seg_blocks) store_vec<NS>(p.state_out + st + w.n0, h);
+    if (p.N == Q * NS && p.seg) store_vec<NS>(p.state_out + st + w.n0, h);
     else store_states<NS>(p.state_out + st, w.n0, p.N, true, h);
     if (w.q == 0) {
         y = fmaf(p.d ? p.d[w.ch] : 0.f, x, y);
@@ -204,13 +248,15 @@ template <typename T> int step_n(const ScanArgs& p, hipStream_t s) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Time segments: batch and channels give B nb workgroups; below two per CU the time axis is split until there are
-// about that many, in segments of at least 8 blocks (each costs a second, lighter walk over its tokens).
+// Time segments: batch and channels give `have` workgroups.  From one per CU on the axis is walked in one piece; below that
+// it is split into about 4 workgroups per CU, in segments of at least 128 tokens, which costs a second, lighter walk.
+// 4 x 4096 x 2048 bf16, 128 workgroups, forward (both walks) / backward (both): 424 / 1018 us in 2 segments, 339 / 688 in 4,
+// 305 / 659 in 8, 305 / 667 in 16; one walk alone at 256 workgroups takes 125 ns a token (backward 385) whatever the split
+// would make of it: 512 us for 4096 tokens against 610 in 4 segments.
 int segments(int B, int nb, int nblk) {
     const long have = (long)B * nb;
     if (have >= 256 || nblk < 16) return 1;
-    long want = (512 + have - 1) / have;
-    const long most = nblk / 8;
+    const long want = (1024 + have - 1) / have, most = nblk / 8;
     return (int)(want < most ? want : most);
 }
 
@@ -218,17 +264,16 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 struct ScanPlan {
     ScanShape g;
-    int nb, nblk, S, seg_blocks;
+    int nb, S, seg;
     size_t seg_h, seg_d, part_bc, part_p;  // bytes
 };
 ScanPlan scan_plan(int B, int L, int D, int N, bool backward) {
     ScanPlan q;
     q.g = scan_shape(N);
     q.nb = ceil_div(D, kScanT / q.g.Q);
-    q.nblk = ceil_div(L, kTok);
-    const int want = segments(B, q.nb, q.nblk);
-    q.seg_blocks = ceil_div(q.nblk, want);
-    q.S = ceil_div(q.nblk, q.seg_blocks);
+    const int nblk = ceil_div(L, kTokF);
+    q.seg = ceil_div(nblk, segments(B, q.nb, nblk)) * kTokF;
+    q.S = ceil_div(L, q.seg);
     q.seg_h = q.S > 1 ? align256((size_t)B * q.S * D * q.g.NP * 4) : 0;
     q.seg_d = q.S > 1 ? align256((size_t)B * q.S * D * 4) : 0;
     q.part_bc = backward ? align256((size_t)q.nb * B * L * 2 * q.g.NP * 4) : 0;
@@ -240,8 +285,17 @@ int check(const char* what, int B, int L, int D, int N, int dtype) {
     if (B < 1 || L < 1 || D < 1 || N < 1 || N > 64 || !dtype_ok(dtype))
         return fail(AFD_ERR_ARG, "%s: B=%d L=%d D=%d N=%d (1..64) dtype=%d", what, B, L, D, N, dtype);
     const ScanPlan q = scan_plan(B, L, D, N, false);
-    if ((long)B * q.S * q.nb > 0x7fffffffL || (long)D * (q.g.NP + 2) > 0x7fffffc0L || L > 0x7fffff00)
+    if ((long)B * q.S * q.nb > 0x7fffffffL || (long)D * (q.g.NP + 2) > 0x7fffffc0L || L > 0x7fff0000 ||
+        (long)D * kTokF * 4 > 0x7fffffffL)
         return fail(AFD_ERR_UNSUPPORTED, "%s: B=%d L=%d D=%d is too large", what, B, L, D);
+    return AFD_OK;
+}
+
+// the lanes' offsets inside a block of tokens are 32-bit
+int check_rows(const char* what, const long long* st, int n, int dtype) {
+    for (int i = 1; i < n; i += 2)
+        if (st[i] < 0 || st[i] * kTokF * (long long)dtype_bytes(dtype) > 0x3fffffffLL)
+            return fail(AFD_ERR_UNSUPPORTED, "%s: row stride %lld", what, st[i]);
     return AFD_OK;
 }
 
@@ -268,7 +322,7 @@ extern "C" size_t afd_state_scan_workspace_bytes(int B, int L, int D, int N, int
 
 extern "C" size_t afd_state_scan_checkpoint_floats(int B, int L, int D, int N) {
     if (B < 1 || L < 1 || D < 1 || N < 1 || N > 64) return 0;
-    return (size_t)B * ceil_div(L, kTok) * D * scan_shape(N).NP;
+    return (size_t)B * ceil_div(L, kCkpt) * D * scan_shape(N).NP;
 }
 
 extern "C" int afd_state_scan_forward(const void* x, const void* dt, const void* b, const void* c, const void* gate,
@@ -278,6 +332,7 @@ extern "C" int afd_state_scan_forward(const void* x, const void* dt, const void*
                                       afd_stream_t stream) {
     if (!x || !dt || !b || !c || !a || !y || !strides) return fail(AFD_ERR_ARG, "state scan: missing tensor");
     if (int rc = check("state scan", B, L, D, N, dtype)) return rc;
+    if (int rc = check_rows("state scan", strides, 10, dtype)) return rc;
     const ScanPlan q = scan_plan(B, L, D, N, false);
     if (q.seg_h + q.seg_d > 0 && (!ws || ws_bytes < q.seg_h + q.seg_d))
         return fail(AFD_ERR_WORKSPACE, "state scan: workspace of %zu bytes, %zu needed", ws_bytes, q.seg_h + q.seg_d);
@@ -286,7 +341,7 @@ extern "C" int afd_state_scan_forward(const void* x, const void* dt, const void*
     set_inputs(p, x, dt, b, c, gate, strides);
     p.a = a; p.d = d; p.dt_bias = dt_bias; p.state = state; p.lengths = lengths; p.y = y; p.state_out = state_out;
     p.ckpt = checkpoints;
-    p.B = B; p.L = L; p.D = D; p.N = N; p.softplus = softplus; p.S = q.S; p.seg_blocks = q.seg_blocks; p.nb = q.nb;
+    p.B = B; p.L = L; p.D = D; p.N = N; p.softplus = softplus; p.S = q.S; p.seg = q.seg; p.nb = q.nb;
     p.seg_h = static_cast<float*>(ws);
     p.seg_d = reinterpret_cast<float*>(static_cast<char*>(ws) + q.seg_h);
     ScopedBytes timing(AFD_K_SEQUENCE, dtype_bytes(dtype) * (gate ? 4.0 : 3.0) * B * L * D, s);
@@ -309,7 +364,7 @@ extern "C" int afd_state_scan_step(const void* x, const void* dt, const void* b,
     const ScanShape g = scan_shape(N);
     p.nb = ceil_div(D, kScanT / g.Q);
     p.S = 1;
-    p.seg_blocks = aligned16(a) && aligned16(state) && aligned16(state_out);
+    p.seg = aligned16(a) && aligned16(state) && aligned16(state_out);
     ScopedBytes timing(AFD_K_SEQUENCE, 8.0 * B * D * N, s);
     if (dtype == AFD_T_F32) return step_n<float>(p, s);
     if (dtype == AFD_T_BF16) return step_n<bf16_t>(p, s);
@@ -325,6 +380,7 @@ extern "C" int afd_state_scan_backward(const void* x, const void* dt, const void
     if (!x || !dt || !b || !c || !a || !dy || !strides || !checkpoints || !dx || !ddt || !db || !dc || !da || (gate && !dgate))
         return fail(AFD_ERR_ARG, "state scan backward: missing tensor");
     if (int rc = check("state scan backward", B, L, D, N, dtype)) return rc;
+    if (int rc = check_rows("state scan backward", strides, 12, dtype)) return rc;
     const ScanPlan q = scan_plan(B, L, D, N, true);
     const size_t need = q.seg_h + q.seg_d + q.part_bc + q.part_p;
     if (!ws || ws_bytes < need)
@@ -335,7 +391,7 @@ extern "C" int afd_state_scan_backward(const void* x, const void* dt, const void
     p.dy = dy; p.yb = strides[10]; p.yl = strides[11];
     p.a = a; p.d = d; p.dt_bias = dt_bias; p.lengths = lengths; p.ckpt = const_cast<float*>(checkpoints);
     p.dstate_out = dstate_out; p.dx = dx; p.ddt = ddt; p.dgate = dgate; p.dstate = dstate;
-    p.B = B; p.L = L; p.D = D; p.N = N; p.softplus = softplus; p.S = q.S; p.seg_blocks = q.seg_blocks; p.nb = q.nb;
+    p.B = B; p.L = L; p.D = D; p.N = N; p.softplus = softplus; p.S = q.S; p.seg = q.seg; p.nb = q.nb;
     char* at = static_cast<char*>(ws);
     p.seg_h = reinterpret_cast<float*>(at);
     p.seg_d = reinterpret_cast<float*>(at + q.seg_h);

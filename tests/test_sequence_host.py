@@ -135,7 +135,7 @@ def test_workspace_sizes_are_those_of_the_layout():
     assert lib.afd_state_scan_workspace_bytes(128, 101, 1024, 16, 0) == 0
     assert lib.afd_state_scan_workspace_bytes(1, 16384, 1024, 16, 0) > 0
     assert lib.afd_state_scan_workspace_bytes(0, 1, 1, 1, 0) == 0
-    assert lib.afd_state_scan_checkpoint_floats(2, 17, 5, 3) == 2 * 2 * 5 * 4
+    assert lib.afd_state_scan_checkpoint_floats(2, 17, 5, 3) == 2 * 3 * 5 * 4
     assert lib.afd_causal_conv_backward_workspace_bytes(2, 65, 6, 4) == 2 * 2 * 6 * 5 * 4
 
 
