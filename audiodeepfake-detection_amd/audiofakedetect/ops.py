@@ -1814,39 +1814,46 @@ def state_scan_step(x, state, dt, a, b, c, d=None, gate=None, dt_bias=None, soft
 
 
 # --------------------------------------------------------------------------------------
+def _gapless(t: torch.Tensor) -> bool:
+    """Does `t` fill its memory without gaps or repeats, in whatever order of its axes?"""
+    return t.is_contiguous() or t.permute(sorted(range(t.dim()), key=lambda k: -t.stride(k))).is_contiguous()
+
+
 def _norm_tables(what: str, tensors, norm_type):
-    """(tensors in dense memory, pointers, counts, types) of a list for `afd_global_norm`."""
+    """The list as tensors in dense memory (the order of the elements is of no interest to a norm: a permuted but gapless
+    tensor is taken as it lies), ready for `afd_global_norm`."""
     _need(norm_type in (2, 2.0, float("inf")), f"{what}: norm_type {norm_type}; 2 or inf expected")
     dense, device = [], None
     for i, t in enumerate(tensors):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: entry {i} is a {type(t).__name__}, not a tensor")
-        if t.layout != torch.strided or t.dtype not in _SEQ_DTYPES:
+        if t.dtype not in _SEQ_DTYPES or t.layout is not torch.strided:
             raise TypeError(f"{what}: entry {i} is {t.layout} {t.dtype}; dense float32, bfloat16 or float16 expected")
-        device = t.device if device is None else device
-        _need(t.device == device, f"{what}: entry {i} is on {t.device}, entry 0 on {device}")
-        t = t.detach()
-        # (the order of the elements is of no interest: a permuted but gapless tensor is taken as it lies in memory)
-        by_stride = t.permute(sorted(range(t.dim()), key=lambda k: -t.stride(k)))
-        dense.append(t if t.is_contiguous() or by_stride.is_contiguous() else t.contiguous())
-    return dense, device
+        if t.device != device:
+            _need(device is None, f"{what}: entry {i} is on {t.device}, entry 0 on {device}")
+            device = t.device
+        dense.append(t if _gapless(t) else t.detach().contiguous())
+    return dense
 
 
 def _norm_arrays(dense):
+    """(pointers, counts, types) of the tensors as host arrays, and the pointers and sizes in bytes as lists."""
     n = len(dense)
-    return ((_native.c_p * n)(*[t.data_ptr() for t in dense]), (_native.c_l * n)(*[t.numel() for t in dense]),
-            (_native.c_i * n)(*[_SEQ_DTYPES[t.dtype] for t in dense]))
+    ptrs, counts = [t.data_ptr() for t in dense], [t.numel() for t in dense]
+    types = [_SEQ_DTYPES[t.dtype] for t in dense]
+    return ((_native.c_p * n)(*ptrs), (_native.c_l * n)(*counts), (_native.c_i * n)(*types)), ptrs, \
+        [c * (2 if k else 4) for c, k in zip(counts, types)]
 
 
-def _launch_norm(dense, arrays, norm_type, max_norm: float, scale: float) -> torch.Tensor:
+def _launch_norm(arrays, n: int, device, norm_type, max_norm: float, scale: float) -> torch.Tensor:
     """[norm, factor] of `afd_global_norm` on the device of the tensors (which is the current one)."""
     lib = _lib()
     ptrs, counts, types = arrays
-    n = len(dense)
-    stats = torch.empty(2, dtype=torch.float32, device=dense[0].device)
-    ws = torch.empty(lib.afd_global_norm_workspace_bytes(counts, n), dtype=torch.uint8, device=stats.device)
+    stats = torch.empty(2, dtype=torch.float32, device=device)
+    nbytes = lib.afd_global_norm_workspace_bytes(counts, n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _native.check(lib.afd_global_norm(ptrs, counts, types, n, int(norm_type == float("inf")), max_norm, scale,
-                                      stats.data_ptr(), ws.data_ptr(), ws.numel(), _native.stream_ptr()), "afd_global_norm")
+                                      stats.data_ptr(), ws.data_ptr(), nbytes, _native.stream_ptr()), "afd_global_norm")
     return stats
 
 
@@ -1854,30 +1861,27 @@ def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """Norm of all elements of all `tensors` (float32 / bfloat16 / float16, mixed as they come) as one float32 scalar on their
     device, without a host synchronisation: the root of the sum of squares, taken in float64, or the largest magnitude
     (norm_type inf).  NaN if an element is; zero for an empty list."""
-    dense, device = _norm_tables("global_norm", list(tensors), norm_type)
+    dense = _norm_tables("global_norm", tensors, norm_type)
     if not dense:
         return torch.zeros(())
     _seq_gpu("global_norm", dense[0])
     with _OnDevice(dense[0]):
-        return _launch_norm(dense, _norm_arrays(dense), norm_type, 1.0, 1.0)[0]
+        return _launch_norm(_norm_arrays(dense)[0], len(dense), dense[0].device, norm_type, 1.0, 1.0)[0]
 
 
-def _check_disjoint(src, dst) -> None:
-    """No element may be scaled twice, nor be read after it was written for another tensor."""
-    spans = []
-    for s, o in zip(src, dst):
-        n = s.numel() * s.element_size()
-        if n == 0:
-            continue
-        spans.append((o.data_ptr(), o.data_ptr() + n, True))
-        if s.data_ptr() != o.data_ptr():
-            spans.append((s.data_ptr(), s.data_ptr() + n, False))
+def _check_disjoint(src, dst, sizes) -> None:
+    """No element may be scaled twice, nor be read after it was written for another tensor (addresses and bytes)."""
+    spans = [(o, o + n, True) for o, n in zip(dst, sizes) if n]
+    spans += [(s, s + n, False) for s, o, n in zip(src, dst, sizes) if n and s != o]
     spans.sort()
     end_any = end_written = 0
     for lo, hi, written in spans:
-        _need(lo >= (end_any if written else end_written), "clip_gradients: tensors to be scaled overlap in memory")
-        end_any = max(end_any, hi)
-        end_written = max(end_written, hi) if written else end_written
+        if lo < (end_any if written else end_written):
+            raise ValueError("clip_gradients: tensors to be scaled overlap in memory")
+        if hi > end_any:
+            end_any = hi
+        if written and hi > end_written:
+            end_written = hi
 
 
 def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
@@ -1888,33 +1892,33 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     max_norm = float(max_norm)
     _need(max_norm >= 0.0, f"{what}: max_norm {max_norm} has to be a number from 0 on")
     grads = list(grads)
-    dense, _ = _norm_tables(what, grads, norm_type)
+    dense = _norm_tables(what, grads, norm_type)
     back = []  # (gradient, dense copy) where the gradient's memory has gaps
     if out is None:
+        into = dense
         for g, t in zip(grads, dense):
-            if t.data_ptr() != g.data_ptr():
+            if t is not g:
                 _need(all(s != 0 or k <= 1 for s, k in zip(g.stride(), g.shape)),
                       f"{what}: a gradient with elements that share memory cannot be scaled in place")
                 back.append((g, t))
-        into = dense
     else:
         into = list(out)
         _need(len(into) == len(grads), f"{what}: {len(into)} tensors in out for {len(grads)} gradients")
         for i, (g, o) in enumerate(zip(grads, into)):
             _seq_check(what, f"out[{i}]", o, g.shape, g.dtype, g.device)
-            if o.stride() != dense[i].stride():
+            if o.stride() != dense[i].stride() and not (o.is_contiguous() and dense[i].is_contiguous()):
                 dense[i] = g.detach().contiguous()
-            _need(o.stride() == dense[i].stride(), f"{what}: out[{i}] has to be contiguous, or strided as its gradient")
-            into[i] = o.detach()
+                _need(o.is_contiguous(), f"{what}: out[{i}] has to be contiguous, or strided as its gradient")
     if not dense:
         return torch.zeros(())
     _seq_gpu(what, dense[0])
-    _check_disjoint(dense, into)
+    n = len(dense)
+    arrays, src, sizes = _norm_arrays(dense)
+    dst = src if out is None else [t.data_ptr() for t in into]
+    _check_disjoint(src, dst, sizes)
     with _OnDevice(dense[0]):
-        arrays = _norm_arrays(dense)
-        stats = _launch_norm(dense, arrays, norm_type, max_norm, 1.0)
-        dst = (_native.c_p * len(into))(*[t.data_ptr() for t in into])
-        _native.check(_lib().afd_multi_scale(arrays[0], dst, arrays[1], arrays[2], len(dense), stats.data_ptr(),
+        stats = _launch_norm(arrays, n, dense[0].device, norm_type, max_norm, 1.0)
+        _native.check(_lib().afd_multi_scale(arrays[0], (_native.c_p * n)(*dst), arrays[1], arrays[2], n, stats.data_ptr(),
                                              _native.stream_ptr()), "afd_multi_scale")
         for g, t in back:
             g.detach().copy_(t)
@@ -2017,8 +2021,8 @@ class FusedAdam(torch.optim.Optimizer):
         self.step_count += 1
         self.gather_grads()
         if max_grad_norm is not None:
-            arena = [self._flat_grad]
-            stats = _launch_norm(arena, _norm_arrays(arena), 2.0, float(max_grad_norm), float(grad_scale))
+            stats = _launch_norm(_norm_arrays([self._flat_grad])[0], 1, self.flat.device, 2.0, float(max_grad_norm),
+                                 float(grad_scale))
             _native.check(_lib().afd_adam_step_clipped(
                 _native.ptr(self.flat), _native.ptr(self._flat_grad), _native.ptr(self.m), _native.ptr(self.v),
                 self.flat.numel(), g["lr"], g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"], self.step_count,

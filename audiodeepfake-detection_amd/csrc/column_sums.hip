@@ -28,7 +28,7 @@ column_sums_kernel(const float* __restrict__ part, long rows, int cols, const af
         if (col < o.begin || col >= o.end || !o.out) continue;
         const int i = col - o.begin, g = i / o.width, j = i - g * o.width;
         if (j >= o.keep) continue;
-        const size_t at = (size_t)g * o.keep + j;
+        const size_t at = (size_t)g * o.gs + (size_t)j * o.js;
         if (o.dtype == AFD_T_F32) static_cast<float*>(o.out)[at] = v;
         else if (o.dtype == AFD_T_BF16) static_cast<afd::bf16_t*>(o.out)[at] = afd::from_f32<afd::bf16_t>(v);
         else static_cast<afd::f16_t*>(o.out)[at] = afd::from_f32<afd::f16_t>(v);

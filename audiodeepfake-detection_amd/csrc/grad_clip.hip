@@ -48,8 +48,6 @@ template <typename Table> __device__ __forceinline__ int owner(const Table& t, i
     return lo;
 }
 
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-
 // NaN stays: fmax would drop it.
 __device__ __forceinline__ double larger(double a, double b) { return (a > b || a != a) ? a : b; }
 
@@ -141,37 +139,34 @@ __global__ void __launch_bounds__(kT) norm_finish_kernel(const double* __restric
     }
 }
 
+// 16 bytes at a time, on the destination's 16-byte boundaries (the source may lie anywhere: gradients go into an arena, one
+// behind the other; element by element such a pair ran at 3.0 TB/s).
 template <typename T> __device__ void piece_scale(const T* p, T* o, int n, float f) {
     constexpr int V = 16 / (int)sizeof(T);
-    const int ma = (int)(reinterpret_cast<uintptr_t>(p) & 15), mo = (int)(reinterpret_cast<uintptr_t>(o) & 15);
-    int done = 0;
-    // 16-byte accesses where source and destination sit the same way on 16-byte boundaries, single elements otherwise
-    if (ma == mo) {
-        int head = (int)(((16 - ma) & 15) / sizeof(T));
-        head = head < n ? head : n;
-        if ((int)threadIdx.x < head) o[threadIdx.x] = from_f32<T>(to_f32(p[threadIdx.x]) * f);
-        const int nv = (n - head) / V;
-        const u32x4* q = reinterpret_cast<const u32x4*>(p + head);
-        u32x4* w = reinterpret_cast<u32x4*>(o + head);
-        auto one = [&](u32x4 r) {
-            struct Pk { T v[V]; };
-            Pk k = __builtin_bit_cast(Pk, r);
+    int head = (int)(((16 - (reinterpret_cast<uintptr_t>(o) & 15)) & 15) / sizeof(T));
+    head = head < n ? head : n;
+    if ((int)threadIdx.x < head) o[threadIdx.x] = from_f32<T>(to_f32(p[threadIdx.x]) * f);
+    const int nv = (n - head) / V;
+    const T* q = p + head;
+    u32x4* w = reinterpret_cast<u32x4*>(o + head);
+    auto get = [&](int i) { return (u32x4)*reinterpret_cast<const u32x4_any*>(q + (size_t)i * V); };
+    auto one = [&](u32x4 r) {
+        Pack<T, V> k = __builtin_bit_cast(Pack<T, V>, r);
 #pragma unroll
-            for (int j = 0; j < V; ++j) k.v[j] = from_f32<T>(to_f32(k.v[j]) * f);
-            return __builtin_bit_cast(u32x4, k);
-        };
-        int i = threadIdx.x;
-        for (; i + 3 * kT < nv; i += 4 * kT) {
-            u32x4 r[4];
+        for (int j = 0; j < V; ++j) k.v[j] = from_f32<T>(to_f32(k.v[j]) * f);
+        return __builtin_bit_cast(u32x4, k);
+    };
+    int i = threadIdx.x;
+    for (; i + 3 * kT < nv; i += 4 * kT) {
+        u32x4 r[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) r[u] = q[i + u * kT];
+        for (int u = 0; u < 4; ++u) r[u] = get(i + u * kT);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) w[i + u * kT] = one(r[u]);
-        }
-        for (; i < nv; i += kT) w[i] = one(q[i]);
-        done = head + nv * V;
+        for (int u = 0; u < 4; ++u) w[i + u * kT] = one(r[u]);
     }
-    for (int i = done + threadIdx.x; i < n; i += kT) o[i] = from_f32<T>(to_f32(p[i]) * f);
+    for (; i < nv; i += kT) w[i] = one(get(i));
+    const int done = head + nv * V;
+    if (done + (int)threadIdx.x < n) o[done + threadIdx.x] = from_f32<T>(to_f32(p[done + threadIdx.x]) * f);
 }
 
 __global__ void __launch_bounds__(kT) scale_pieces_kernel(const ScaleTable t, const float* __restrict__ stats) {

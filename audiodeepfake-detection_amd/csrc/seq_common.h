@@ -39,13 +39,46 @@ __device__ __forceinline__ float softplus_f32(float x) {
     return fmaf(s, p, fmaxf(x, 0.f));  // (NaN comes in through e)
 }
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+// 16 bytes from or to any element's address: global memory takes them on every alignment, aligned ones fastest
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+template <typename T, int V> struct Pack { T v[V]; };
+
+template <typename T, int V> __device__ __forceinline__ void load_row(const T* p, float (&r)[V]) {
+    if constexpr (V == 1) {
+        r[0] = to_f32(*p);
+    } else {
+        static_assert(V * sizeof(T) == 16 || V * sizeof(T) == 8, "vector rows");
+        Pack<T, V> k;
+        if constexpr (V * sizeof(T) == 16) k = __builtin_bit_cast(Pack<T, V>, (u32x4)*reinterpret_cast<const u32x4_any*>(p));
+        else k = __builtin_bit_cast(Pack<T, V>, (u32x2)*reinterpret_cast<const u32x2_any*>(p));
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[i] = to_f32(k.v[i]);
+    }
+}
+
+template <typename T, int V> __device__ __forceinline__ void store_row(T* p, const float (&r)[V]) {
+    if constexpr (V == 1) {
+        *p = from_f32<T>(r[0]);
+    } else {
+        Pack<T, V> k;
+#pragma unroll
+        for (int i = 0; i < V; ++i) k.v[i] = from_f32<T>(r[i]);
+        if constexpr (V * sizeof(T) == 16) *reinterpret_cast<u32x4_any*>(p) = __builtin_bit_cast(u32x4, k);
+        else *reinterpret_cast<u32x2_any*>(p) = __builtin_bit_cast(u32x2, k);
+    }
+}
+
 // Sums of the columns of part[rows][cols]: each workgroup takes 64 columns, its 16 waves take every 16th row and meet in LDS.
 // Column c goes to the output that owns it (fixed order: no atomics, the same bits every time).  The partial rows are
 // written just before by the same stream: L2-resident in most cases, a tenth or less of the main kernel's bytes.
 struct ColumnOut {
-    void* out;       // NULL: dropped
-    int begin, end;  // the columns [begin, end) of a row belong to this output
-    int width, keep; // inside it, column i = (i / width, i % width) is kept where i % width < keep, at i / width * keep + i % width
+    void* out;        // NULL: dropped
+    int begin, end;   // the columns [begin, end) of a row belong to this output
+    int width, keep;  // inside it, column i = (g, j) = (i / width, i % width) is kept where j < keep
+    int gs, js;       // ... and goes to g gs + j js
     int dtype;
 };
 struct ColumnOuts {

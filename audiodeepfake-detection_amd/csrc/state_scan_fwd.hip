@@ -402,8 +402,8 @@ extern "C" int afd_state_scan_backward(const void* x, const void* dt, const void
     if (int rc = scan_bc_gradients(p, db, dc, dtype, s)) return rc;
     ColumnOuts o{};
     o.n = 3;
-    o.o[0] = {da, 0, D * q.g.NP, q.g.NP, N, AFD_T_F32};
-    o.o[1] = {dd, D * q.g.NP, D * q.g.NP + D, 1, 1, AFD_T_F32};
-    o.o[2] = {ddt_bias, D * q.g.NP + D, D * q.g.NP + 2 * D, 1, 1, AFD_T_F32};
+    o.o[0] = {da, 0, D * q.g.NP, q.g.NP, N, N, 1, AFD_T_F32};
+    o.o[1] = {dd, D * q.g.NP, D * q.g.NP + D, 1, 1, 1, 0, AFD_T_F32};
+    o.o[2] = {ddt_bias, D * q.g.NP + D, D * q.g.NP + 2 * D, 1, 1, 1, 0, AFD_T_F32};
     return launch_column_sums(p.part_p, (long)B * q.S, D * (q.g.NP + 2), o, s);
 }

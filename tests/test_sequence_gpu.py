@@ -4,7 +4,7 @@ restatements of sequence_ref.py.
 Tolerances (sequence_ref.close): half a step of the result's type, plus a count of float32 roundings times 2^-24 of the sums
 of magnitudes behind the result.  The counts, worst case, errors adding up linearly:
   convolution          W products and sums, sigmoid and product (10)                       -> 2 W + 32
-    dw, db             plus 64 rows in a thread's sum and the partial rows behind it       -> + 64 + B ceil(L / 64)
+    dw, db             plus 32 rows in a thread's sum and the partial rows behind it       -> + 64 + B ceil(L / 16)
   scan                 per step 5 (decay: exponent and exponential 3, product and sum 2); the error of delta (softplus: 20)
                        reaches a decay exp(-s) as 22 s <= 22 / e of it; c . h and gate 40   -> 64 + 5 L
     gradients          the same again backwards, sums over channels or rows                 -> 160 + 12 L + B + D / 16
@@ -73,7 +73,7 @@ def test_conv_forward_and_gradients(dtype, b, l, d, w, act, bias, state, lens, w
     k = 2 * w + 32
     ref.close(y, want["y"], bound["y"], k, "y")
     assert torch.equal(so.cpu().double(), want["state"]), "state: a copy of rows"
-    rows = 64 + b * ((l + 63) // 64)
+    rows = 64 + b * ((l + 15) // 16)
     for name in names:
         ref.close(grads[name], want["d" + name], bound["d" + name], k + (rows if name in ("w", "b") else 0), "d" + name)
 

@@ -120,13 +120,18 @@ def test_global_norm_and_clip_refuse():
 
 def test_clip_refuses_tensors_that_overlap():
     flat = torch.zeros(32)
-    a, b, c = flat[:16], flat[16:], flat[8:24]
-    ops._check_disjoint([a, b], [a, b])                       # in place, side by side
-    ops._check_disjoint([a], [torch.zeros(16)])
-    ops._check_disjoint([a, a], [torch.zeros(16), torch.zeros(16)])  # read twice, written apart
-    for src, dst in (([a, a], [a, a]), ([a, c], [a, c]), ([a], [c]), ([a, b], [b, a]), ([a, c], [torch.zeros(16), c])):
+    a, b, c, o1, o2 = flat[:16], flat[16:], flat[8:24], torch.zeros(16), torch.zeros(16)
+
+    def check(src, dst):
+        ops._check_disjoint([t.data_ptr() for t in src], [t.data_ptr() for t in dst], [4 * t.numel() for t in src])
+
+    check([a, b], [a, b])       # in place, side by side
+    check([a], [o1])
+    check([a, a], [o1, o2])     # read twice, written apart
+    check([a[:0], a], [c[:0], a])
+    for src, dst in (([a, a], [a, a]), ([a, c], [a, c]), ([a], [c]), ([a, b], [b, a]), ([a, c], [o1, c]), ([a, b], [o1, o1])):
         with pytest.raises(ValueError):
-            ops._check_disjoint(src, dst)
+            check(src, dst)
 
 
 def test_workspace_sizes_are_those_of_the_layout():
@@ -136,7 +141,7 @@ def test_workspace_sizes_are_those_of_the_layout():
     assert lib.afd_state_scan_workspace_bytes(1, 16384, 1024, 16, 0) > 0
     assert lib.afd_state_scan_workspace_bytes(0, 1, 1, 1, 0) == 0
     assert lib.afd_state_scan_checkpoint_floats(2, 17, 5, 3) == 2 * 3 * 5 * 4
-    assert lib.afd_causal_conv_backward_workspace_bytes(2, 65, 6, 4) == 2 * 2 * 6 * 5 * 4
+    assert lib.afd_causal_conv_backward_workspace_bytes(2, 65, 6, 4) == 2 * 5 * 6 * 5 * 4  # five tiles of 16 rows
 
 
 def test_c_entries_refuse_bad_sizes():
