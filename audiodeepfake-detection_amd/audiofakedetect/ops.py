@@ -1489,16 +1489,13 @@ _SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {"none": 0, "silu": 1}
 
 
-def _need(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
-
-
+# (Messages are put together only when something is wrong: a check costs less than a microsecond, a formatted shape more.)
 def _seq_input(what: str, x, ndim: int) -> None:
     """The tensor that fixes type, device and sizes of a call."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what}: x is a {type(x).__name__}, not a tensor")
-    _need(x.dim() == ndim, f"{what}: x has {x.dim()} dimensions, {ndim} expected")
+    if x.dim() != ndim:
+        raise ValueError(f"{what}: x has {x.dim()} dimensions, {ndim} expected")
     if x.dtype not in _SEQ_DTYPES:
         raise TypeError(f"{what}: x is {x.dtype}; float32, bfloat16 or float16 expected")
 
@@ -1508,10 +1505,12 @@ def _seq_check(what: str, name: str, t, shape, dtype, device) -> None:
         return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: {name} is a {type(t).__name__}, not a tensor")
-    _need(tuple(t.shape) == tuple(shape), f"{what}: {name} has shape {tuple(t.shape)}, {tuple(shape)} expected")
-    if t.dtype != dtype:
+    if t.shape != shape:
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, {tuple(shape)} expected")
+    if t.dtype is not dtype:
         raise TypeError(f"{what}: {name} is {t.dtype}, {dtype} expected")
-    _need(t.device == device, f"{what}: {name} is on {t.device}, x on {device}")
+    if t.device != device:
+        raise ValueError(f"{what}: {name} is on {t.device}, x on {device}")
 
 
 def _seq_gpu(what: str, x) -> None:
@@ -1520,19 +1519,26 @@ def _seq_gpu(what: str, x) -> None:
 
 
 class _OnDevice:
-    """Launches go to the device of the tensors, whatever the current one is."""
+    """Launches go to the device of the tensors, whatever the current one is; `with` gives that device's current stream."""
+
+    __slots__ = ("index", "guard")
 
     def __init__(self, t: torch.Tensor) -> None:
-        i = t.device.index
-        self.guard = torch.cuda.device(i) if i != torch.cuda.current_device() else None
+        self.index = t.get_device()
+        self.guard = torch.cuda.device(self.index) if self.index != torch.cuda.current_device() else None
 
-    def __enter__(self):
+    def __enter__(self) -> int:
         if self.guard is not None:
             self.guard.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.guard is not None:
             self.guard.__exit__(*exc)
+
+
+def _at(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -1549,15 +1555,21 @@ def _seq_lengths(what: str, lengths, x) -> Optional[torch.Tensor]:
         return None
     if not isinstance(lengths, torch.Tensor) or lengths.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{what}: lengths has to be an int32 or int64 tensor")
-    _need(tuple(lengths.shape) == (x.shape[0],), f"{what}: lengths has shape {tuple(lengths.shape)}, ({x.shape[0]},) expected")
-    _need(lengths.device == x.device, f"{what}: lengths is on {lengths.device}, x on {x.device}")
+    if lengths.shape != (x.shape[0],):
+        raise ValueError(f"{what}: lengths has shape {tuple(lengths.shape)}, ({x.shape[0]},) expected")
+    if lengths.device != x.device:
+        raise ValueError(f"{what}: lengths is on {lengths.device}, x on {x.device}")
     if lengths.dtype == torch.int64:
         lengths = lengths.clamp(0, x.shape[1]).to(torch.int32)
     return _dense(lengths)
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _step_state(what: str, state, state_out, tensors) -> torch.Tensor:
@@ -1565,13 +1577,16 @@ def _step_state(what: str, state, state_out, tensors) -> torch.Tensor:
     if _wants_grad(*tensors):
         raise RuntimeError(f"{what}: single steps have no backward pass: call it under torch.no_grad() (the whole-sequence "
                            "form is differentiable)")
-    _need(state.is_contiguous(), f"{what}: state has to be contiguous (it is updated in place)")
+    if not state.is_contiguous():
+        raise ValueError(f"{what}: state has to be contiguous (it is updated in place)")
     if state_out is None:
         return state
     _seq_check(what, "state_out", state_out, state.shape, state.dtype, state.device)
-    _need(state_out.is_contiguous(), f"{what}: state_out has to be contiguous")
+    if not state_out.is_contiguous():
+        raise ValueError(f"{what}: state_out has to be contiguous")
     p, q, n = state.data_ptr(), state_out.data_ptr(), state.numel() * state.element_size()
-    _need(p == q or p + n <= q or q + n <= p, f"{what}: state_out overlaps state without being it")
+    if p != q and p < q + n and q < p + n:
+        raise ValueError(f"{what}: state_out overlaps state without being it")
     return state_out
 
 
@@ -1579,36 +1594,43 @@ def _conv_check(what: str, x, w, b, activation, ndim: int):
     _seq_input(what, x, ndim)
     if not isinstance(w, torch.Tensor):
         raise TypeError(f"{what}: w is a {type(w).__name__}, not a tensor")
-    _need(w.dim() == 2 and w.shape[0] == x.shape[-1], f"{what}: w has shape {tuple(w.shape)}, ({x.shape[-1]}, taps) expected")
-    _need(2 <= w.shape[1] <= 8, f"{what}: {w.shape[1]} taps; 2 to 8 are supported")
-    if w.dtype not in (torch.float32, x.dtype):
+    if w.dim() != 2 or w.shape[0] != x.shape[-1]:
+        raise ValueError(f"{what}: w has shape {tuple(w.shape)}, ({x.shape[-1]}, taps) expected")
+    if not 2 <= w.shape[1] <= 8:
+        raise ValueError(f"{what}: {w.shape[1]} taps; 2 to 8 are supported")
+    if w.dtype is not torch.float32 and w.dtype is not x.dtype:
         raise TypeError(f"{what}: w is {w.dtype}; float32 or the type of x ({x.dtype}) expected")
-    _need(w.device == x.device, f"{what}: w is on {w.device}, x on {x.device}")
+    if w.device != x.device:
+        raise ValueError(f"{what}: w is on {w.device}, x on {x.device}")
     _seq_check(what, "b", b, (x.shape[-1],), w.dtype, x.device)
-    _need(activation in _ACTIVATIONS, f"{what}: activation {activation!r}; one of {sorted(_ACTIVATIONS)} expected")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{what}: activation {activation!r}; one of {sorted(_ACTIVATIONS)} expected")
     return _ACTIVATIONS[activation]
+
+
+def _conv_forward(x, w, b, state, lengths, act, return_state):
+    bsz, steps, d = x.shape
+    taps = w.shape[1]
+    y = torch.empty((bsz, steps, d), dtype=x.dtype, device=x.device)
+    state_out = torch.empty((bsz, taps - 1, d), dtype=x.dtype, device=x.device) if return_state else None
+    if y.numel() > 0:
+        with _OnDevice(x) as stream:
+            _native.check(_lib().afd_causal_conv_forward(
+                x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _at(b), int(w.dtype is torch.float32), _at(state),
+                _at(lengths), y.data_ptr(), _at(state_out), bsz, steps, d, taps, act, _SEQ_DTYPES[x.dtype], stream),
+                "afd_causal_conv_forward")
+    elif state_out is not None:
+        state_out.copy_(state) if state is not None else state_out.zero_()
+    return y, state_out
 
 
 class _CausalConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, state, lengths, act, return_state):
         ctx.set_materialize_grads(False)
-        bsz, steps, d = x.shape
-        taps = w.shape[1]
-        x, w, b, state = _rows(x), _dense(w), _dense(b), _dense(state)
-        y = torch.empty((bsz, steps, d), dtype=x.dtype, device=x.device)
-        state_out = torch.empty((bsz, taps - 1, d), dtype=x.dtype, device=x.device) if return_state else None
-        if y.numel() > 0:
-            with _OnDevice(x):
-                _native.check(_lib().afd_causal_conv_forward(
-                    x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _native.ptr(b), int(w.dtype == torch.float32),
-                    _native.ptr(state), _native.ptr(lengths), y.data_ptr(), _native.ptr(state_out), bsz, steps, d, taps, act,
-                    _SEQ_DTYPES[x.dtype], _native.stream_ptr()), "afd_causal_conv_forward")
-        elif state_out is not None:
-            state_out.copy_(state) if state is not None else state_out.zero_()
         ctx.save_for_backward(x, w, b, state, lengths)
         ctx.act = act
-        return y, state_out
+        return _conv_forward(x, w, b, state, lengths, act, return_state)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -1629,15 +1651,14 @@ class _CausalConv(torch.autograd.Function):
         dw = torch.empty_like(w)
         db = torch.empty_like(b) if b is not None else None
         dstate = torch.empty_like(state) if need[3] else None
-        with _OnDevice(x):
+        with _OnDevice(x) as stream:
             lib = _lib()
-            ws = torch.empty(lib.afd_causal_conv_backward_workspace_bytes(bsz, steps, d, taps), dtype=torch.uint8,
-                             device=x.device)
+            nbytes = lib.afd_causal_conv_backward_workspace_bytes(bsz, steps, d, taps)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
             _native.check(lib.afd_causal_conv_backward(
-                x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _native.ptr(b), int(w.dtype == torch.float32),
-                _native.ptr(state), _native.ptr(lengths), dy.data_ptr(), dy.stride(0), dy.stride(1),
-                _native.ptr(dstate_out), dx.data_ptr(), dw.data_ptr(), _native.ptr(db), _native.ptr(dstate), bsz, steps, d,
-                taps, ctx.act, _SEQ_DTYPES[x.dtype], ws.data_ptr(), ws.numel(), _native.stream_ptr()),
+                x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _at(b), int(w.dtype is torch.float32), _at(state),
+                _at(lengths), dy.data_ptr(), dy.stride(0), dy.stride(1), _at(dstate_out), dx.data_ptr(), dw.data_ptr(),
+                _at(db), _at(dstate), bsz, steps, d, taps, ctx.act, _SEQ_DTYPES[x.dtype], ws.data_ptr(), nbytes, stream),
                 "afd_causal_conv_backward")
         return dx, dw, db, dstate, None, None, None
 
@@ -1655,7 +1676,9 @@ def causal_conv(x, w, b=None, activation: str = "none", state=None, lengths=None
     _seq_check("causal_conv", "state", state, (x.shape[0], w.shape[1] - 1, x.shape[2]), x.dtype, x.device)
     lengths = _seq_lengths("causal_conv", lengths, x)
     _seq_gpu("causal_conv", x)
-    y, state_out = _CausalConv.apply(x, w, b, state, lengths, act, bool(return_state))
+    x, w, b, state = _rows(x), _dense(w), _dense(b), _dense(state)
+    run = _CausalConv.apply if _wants_grad(x, w, b, state) else _conv_forward
+    y, state_out = run(x, w, b, state, lengths, act, bool(return_state))
     return (y, state_out) if return_state else y
 
 
@@ -1671,67 +1694,73 @@ def causal_conv_step(x, state, w, b=None, activation: str = "none", state_out=No
     x, w, b = _rows(x), _dense(w), _dense(b)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if y.numel() > 0:
-        with _OnDevice(x):
+        with _OnDevice(x) as stream:
             _native.check(_lib().afd_causal_conv_step(
-                x.data_ptr(), x.stride(0), w.data_ptr(), _native.ptr(b), int(w.dtype == torch.float32), state.data_ptr(),
-                y.data_ptr(), into.data_ptr(), x.shape[0], x.shape[1], w.shape[1], act, _SEQ_DTYPES[x.dtype],
-                _native.stream_ptr()), "afd_causal_conv_step")
+                x.data_ptr(), x.stride(0), w.data_ptr(), _at(b), int(w.dtype is torch.float32), state.data_ptr(),
+                y.data_ptr(), into.data_ptr(), x.shape[0], x.shape[1], w.shape[1], act, _SEQ_DTYPES[x.dtype], stream),
+                "afd_causal_conv_step")
     return y
 
 
 def _scan_check(what: str, x, dt, a, b, c, d, gate, dt_bias, state, ndim: int) -> None:
     _seq_input(what, x, ndim)
-    chans, lead = x.shape[-1], tuple(x.shape[:-1])
+    lead, chans, dtype, device = x.shape[:-1], x.shape[-1], x.dtype, x.device
     if not isinstance(a, torch.Tensor):
         raise TypeError(f"{what}: a is a {type(a).__name__}, not a tensor")
-    _need(a.dim() == 2 and a.shape[0] == chans, f"{what}: a has shape {tuple(a.shape)}, ({chans}, states) expected")
+    if a.dim() != 2 or a.shape[0] != chans:
+        raise ValueError(f"{what}: a has shape {tuple(a.shape)}, ({chans}, states) expected")
     n = a.shape[1]
-    _need(1 <= n <= 64, f"{what}: {n} states per channel; 1 to 64 are supported")
-    for name, t in (("dt", dt), ("b", b), ("c", c)):
-        if t is None:
-            raise TypeError(f"{what}: {name} has to be a tensor")
-    for name, t, shape in (("dt", dt, lead + (chans,)), ("b", b, lead + (n,)), ("c", c, lead + (n,)),
-                           ("gate", gate, lead + (chans,))):
-        _seq_check(what, name, t, shape, x.dtype, x.device)
-    for name, t, shape in (("a", a, (chans, n)), ("d", d, (chans,)), ("dt_bias", dt_bias, (chans,)),
-                           ("state", state, (x.shape[0], chans, n))):
-        _seq_check(what, name, t, shape, torch.float32, x.device)
+    if not 1 <= n <= 64:
+        raise ValueError(f"{what}: {n} states per channel; 1 to 64 are supported")
+    if dt is None or b is None or c is None:
+        raise TypeError(f"{what}: dt, b and c have to be tensors")
+    _seq_check(what, "dt", dt, x.shape, dtype, device)
+    _seq_check(what, "b", b, (*lead, n), dtype, device)
+    _seq_check(what, "c", c, (*lead, n), dtype, device)
+    _seq_check(what, "gate", gate, x.shape, dtype, device)
+    _seq_check(what, "a", a, (chans, n), torch.float32, device)
+    _seq_check(what, "d", d, (chans,), torch.float32, device)
+    _seq_check(what, "dt_bias", dt_bias, (chans,), torch.float32, device)
+    _seq_check(what, "state", state, (x.shape[0], chans, n), torch.float32, device)
 
 
 def _scan_strides(tensors, axes):
-    out = []
-    for t in tensors:
-        out += [t.stride(i) if t is not None else 0 for i in axes]
+    out = [t.stride(i) if t is not None else 0 for t in tensors for i in axes]
     return (_native.c_l * len(out))(*out)
+
+
+def _scan_forward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, softplus, return_state, keep=False):
+    """(y, state behind the last token or None, checkpoints for the backward or None)"""
+    bsz, steps, chans = x.shape
+    n = a.shape[1]
+    device = x.device
+    y = torch.empty((bsz, steps, chans), dtype=x.dtype, device=device)
+    state_out = torch.empty((bsz, chans, n), dtype=torch.float32, device=device) if return_state else None
+    ckpt = ws = None
+    if y.numel() > 0:
+        with _OnDevice(x) as stream:
+            lib = _lib()
+            if keep:
+                ckpt = torch.empty(lib.afd_state_scan_checkpoint_floats(bsz, steps, chans, n), dtype=torch.float32,
+                                   device=device)
+            nbytes = lib.afd_state_scan_workspace_bytes(bsz, steps, chans, n, 0)
+            if nbytes:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            _native.check(lib.afd_state_scan_forward(
+                x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _at(gate),
+                _scan_strides((x, dt, b, c, gate), (0, 1)), a.data_ptr(), _at(d), _at(dt_bias), _at(state), _at(lengths),
+                y.data_ptr(), _at(state_out), _at(ckpt), bsz, steps, chans, n, softplus, _SEQ_DTYPES[x.dtype], _at(ws),
+                nbytes, stream), "afd_state_scan_forward")
+    elif state_out is not None:
+        state_out.copy_(state) if state is not None else state_out.zero_()
+    return y, state_out, ckpt
 
 
 class _StateScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, dt, a, b, c, d, gate, dt_bias, state, lengths, softplus, return_state, keep):
+    def forward(ctx, x, dt, a, b, c, d, gate, dt_bias, state, lengths, softplus, return_state):
         ctx.set_materialize_grads(False)
-        bsz, steps, chans = x.shape
-        n = a.shape[1]
-        x, dt, b, c, gate = _rows(x), _rows(dt), _rows(b), _rows(c), _rows(gate)
-        a, d, dt_bias, state = _dense(a), _dense(d), _dense(dt_bias), _dense(state)
-        y = torch.empty((bsz, steps, chans), dtype=x.dtype, device=x.device)
-        state_out = torch.empty((bsz, chans, n), dtype=torch.float32, device=x.device) if return_state else None
-        ckpt = None
-        if y.numel() > 0:
-            with _OnDevice(x):
-                lib = _lib()
-                if keep:
-                    ckpt = torch.empty(lib.afd_state_scan_checkpoint_floats(bsz, steps, chans, n), dtype=torch.float32,
-                                       device=x.device)
-                nbytes = lib.afd_state_scan_workspace_bytes(bsz, steps, chans, n, 0)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-                _native.check(lib.afd_state_scan_forward(
-                    x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _native.ptr(gate),
-                    _scan_strides((x, dt, b, c, gate), (0, 1)), a.data_ptr(), _native.ptr(d), _native.ptr(dt_bias),
-                    _native.ptr(state), _native.ptr(lengths), y.data_ptr(), _native.ptr(state_out), _native.ptr(ckpt), bsz,
-                    steps, chans, n, softplus, _SEQ_DTYPES[x.dtype], _native.ptr(ws), nbytes, _native.stream_ptr()),
-                    "afd_state_scan_forward")
-        elif state_out is not None:
-            state_out.copy_(state) if state is not None else state_out.zero_()
+        y, state_out, ckpt = _scan_forward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, softplus, return_state, True)
         ctx.save_for_backward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, ckpt)
         ctx.softplus = softplus
         return y, state_out
@@ -1754,21 +1783,21 @@ class _StateScan(torch.autograd.Function):
                     g.zero_()
             if grads[8] is not None and dstate_out is not None:
                 grads[8].copy_(dstate_out)
-            return (*grads, None, None, None, None)
+            return (*grads, None, None, None)
         dx, ddt, da, db, dc, dd, dgate, dbias, dstate = grads
         dy = _rows(dy) if dy is not None else torch.zeros_like(x)
         dstate_out = _dense(dstate_out)
-        with _OnDevice(x):
+        with _OnDevice(x) as stream:
             lib = _lib()
-            ws = torch.empty(lib.afd_state_scan_workspace_bytes(bsz, steps, chans, n, 1), dtype=torch.uint8, device=x.device)
+            nbytes = lib.afd_state_scan_workspace_bytes(bsz, steps, chans, n, 1)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
             _native.check(lib.afd_state_scan_backward(
-                x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _native.ptr(gate), dy.data_ptr(),
-                _scan_strides((x, dt, b, c, gate, dy), (0, 1)), a.data_ptr(), _native.ptr(d), _native.ptr(dt_bias),
-                _native.ptr(lengths), ckpt.data_ptr(), _native.ptr(dstate_out), dx.data_ptr(), ddt.data_ptr(),
-                db.data_ptr(), dc.data_ptr(), _native.ptr(dgate), da.data_ptr(), _native.ptr(dd), _native.ptr(dbias),
-                _native.ptr(dstate), bsz, steps, chans, n, ctx.softplus, _SEQ_DTYPES[x.dtype], ws.data_ptr(), ws.numel(),
-                _native.stream_ptr()), "afd_state_scan_backward")
-        return (*grads, None, None, None, None)
+                x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _at(gate), dy.data_ptr(),
+                _scan_strides((x, dt, b, c, gate, dy), (0, 1)), a.data_ptr(), _at(d), _at(dt_bias), _at(lengths),
+                ckpt.data_ptr(), _at(dstate_out), dx.data_ptr(), ddt.data_ptr(), db.data_ptr(), dc.data_ptr(), _at(dgate),
+                da.data_ptr(), _at(dd), _at(dbias), _at(dstate), bsz, steps, chans, n, ctx.softplus, _SEQ_DTYPES[x.dtype],
+                ws.data_ptr(), nbytes, stream), "afd_state_scan_backward")
+        return (*grads, None, None, None)
 
 
 def state_scan(x, dt, a, b, c, d=None, gate=None, dt_bias=None, softplus: bool = False, state=None, lengths=None,
@@ -1786,9 +1815,10 @@ def state_scan(x, dt, a, b, c, d=None, gate=None, dt_bias=None, softplus: bool =
     _scan_check("state_scan", x, dt, a, b, c, d, gate, dt_bias, state, 3)
     lengths = _seq_lengths("state_scan", lengths, x)
     _seq_gpu("state_scan", x)
-    keep = _wants_grad(x, dt, a, b, c, d, gate, dt_bias, state)
-    y, state_out = _StateScan.apply(x, dt, a, b, c, d, gate, dt_bias, state, lengths, int(bool(softplus)),
-                                    bool(return_state), keep)
+    x, dt, b, c, gate = _rows(x), _rows(dt), _rows(b), _rows(c), _rows(gate)
+    a, d, dt_bias, state = _dense(a), _dense(d), _dense(dt_bias), _dense(state)
+    run = _StateScan.apply if _wants_grad(x, dt, a, b, c, d, gate, dt_bias, state) else _scan_forward
+    y, state_out = run(x, dt, a, b, c, d, gate, dt_bias, state, lengths, int(bool(softplus)), bool(return_state))[:2]
     return (y, state_out) if return_state else y
 
 
@@ -1804,35 +1834,36 @@ def state_scan_step(x, state, dt, a, b, c, d=None, gate=None, dt_bias=None, soft
     a, d, dt_bias = _dense(a), _dense(d), _dense(dt_bias)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if y.numel() > 0:
-        with _OnDevice(x):
+        with _OnDevice(x) as stream:
             _native.check(_lib().afd_state_scan_step(
-                x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _native.ptr(gate),
-                _scan_strides((x, dt, b, c, gate), (0,)), a.data_ptr(), _native.ptr(d), _native.ptr(dt_bias),
-                state.data_ptr(), y.data_ptr(), into.data_ptr(), x.shape[0], x.shape[1], a.shape[1], int(bool(softplus)),
-                _SEQ_DTYPES[x.dtype], _native.stream_ptr()), "afd_state_scan_step")
+                x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _at(gate), _scan_strides((x, dt, b, c, gate), (0,)),
+                a.data_ptr(), _at(d), _at(dt_bias), state.data_ptr(), y.data_ptr(), into.data_ptr(), x.shape[0], x.shape[1],
+                a.shape[1], int(bool(softplus)), _SEQ_DTYPES[x.dtype], stream), "afd_state_scan_step")
     return y
 
 
 # --------------------------------------------------------------------------------------
 def _gapless(t: torch.Tensor) -> bool:
     """Does `t` fill its memory without gaps or repeats, in whatever order of its axes?"""
-    return t.is_contiguous() or t.permute(sorted(range(t.dim()), key=lambda k: -t.stride(k))).is_contiguous()
+    return t.permute(sorted(range(t.dim()), key=lambda k: -t.stride(k))).is_contiguous()
 
 
 def _norm_tables(what: str, tensors, norm_type):
     """The list as tensors in dense memory (the order of the elements is of no interest to a norm: a permuted but gapless
     tensor is taken as it lies), ready for `afd_global_norm`."""
-    _need(norm_type in (2, 2.0, float("inf")), f"{what}: norm_type {norm_type}; 2 or inf expected")
+    if norm_type not in (2, 2.0, float("inf")):
+        raise ValueError(f"{what}: norm_type {norm_type}; 2 or inf expected")
     dense, device = [], None
-    for i, t in enumerate(tensors):
+    for t in tensors:
         if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{what}: entry {i} is a {type(t).__name__}, not a tensor")
+            raise TypeError(f"{what}: entry {len(dense)} is a {type(t).__name__}, not a tensor")
         if t.dtype not in _SEQ_DTYPES or t.layout is not torch.strided:
-            raise TypeError(f"{what}: entry {i} is {t.layout} {t.dtype}; dense float32, bfloat16 or float16 expected")
+            raise TypeError(f"{what}: entry {len(dense)} is {t.layout} {t.dtype}; dense float32, bfloat16 or float16 expected")
         if t.device != device:
-            _need(device is None, f"{what}: entry {i} is on {t.device}, entry 0 on {device}")
+            if device is not None:
+                raise ValueError(f"{what}: entry {len(dense)} is on {t.device}, entry 0 on {device}")
             device = t.device
-        dense.append(t if _gapless(t) else t.detach().contiguous())
+        dense.append(t if t.is_contiguous() or _gapless(t) else t.detach().contiguous())
     return dense
 
 
@@ -1845,7 +1876,7 @@ def _norm_arrays(dense):
         [c * (2 if k else 4) for c, k in zip(counts, types)]
 
 
-def _launch_norm(arrays, n: int, device, norm_type, max_norm: float, scale: float) -> torch.Tensor:
+def _launch_norm(arrays, n: int, device, norm_type, max_norm: float, scale: float, stream: int) -> torch.Tensor:
     """[norm, factor] of `afd_global_norm` on the device of the tensors (which is the current one)."""
     lib = _lib()
     ptrs, counts, types = arrays
@@ -1853,7 +1884,7 @@ def _launch_norm(arrays, n: int, device, norm_type, max_norm: float, scale: floa
     nbytes = lib.afd_global_norm_workspace_bytes(counts, n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _native.check(lib.afd_global_norm(ptrs, counts, types, n, int(norm_type == float("inf")), max_norm, scale,
-                                      stats.data_ptr(), ws.data_ptr(), nbytes, _native.stream_ptr()), "afd_global_norm")
+                                      stats.data_ptr(), ws.data_ptr(), nbytes, stream), "afd_global_norm")
     return stats
 
 
@@ -1865,8 +1896,8 @@ def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     if not dense:
         return torch.zeros(())
     _seq_gpu("global_norm", dense[0])
-    with _OnDevice(dense[0]):
-        return _launch_norm(_norm_arrays(dense)[0], len(dense), dense[0].device, norm_type, 1.0, 1.0)[0]
+    with _OnDevice(dense[0]) as stream:
+        return _launch_norm(_norm_arrays(dense)[0], len(dense), dense[0].device, norm_type, 1.0, 1.0, stream)[0]
 
 
 def _check_disjoint(src, dst, sizes) -> None:
@@ -1890,7 +1921,8 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     scaling, a float32 scalar on the device; nothing waits for it on the host.  A norm of inf gives zeros, NaN gives NaN."""
     what = "clip_gradients"
     max_norm = float(max_norm)
-    _need(max_norm >= 0.0, f"{what}: max_norm {max_norm} has to be a number from 0 on")
+    if not max_norm >= 0.0:
+        raise ValueError(f"{what}: max_norm {max_norm} has to be a number from 0 on")
     grads = list(grads)
     dense = _norm_tables(what, grads, norm_type)
     back = []  # (gradient, dense copy) where the gradient's memory has gaps
@@ -1898,17 +1930,20 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
         into = dense
         for g, t in zip(grads, dense):
             if t is not g:
-                _need(all(s != 0 or k <= 1 for s, k in zip(g.stride(), g.shape)),
-                      f"{what}: a gradient with elements that share memory cannot be scaled in place")
+                if any(s == 0 and k > 1 for s, k in zip(g.stride(), g.shape)):
+                    raise ValueError(f"{what}: a gradient with elements that share memory cannot be scaled in place")
                 back.append((g, t))
     else:
         into = list(out)
-        _need(len(into) == len(grads), f"{what}: {len(into)} tensors in out for {len(grads)} gradients")
-        for i, (g, o) in enumerate(zip(grads, into)):
-            _seq_check(what, f"out[{i}]", o, g.shape, g.dtype, g.device)
-            if o.stride() != dense[i].stride() and not (o.is_contiguous() and dense[i].is_contiguous()):
-                dense[i] = g.detach().contiguous()
-                _need(o.is_contiguous(), f"{what}: out[{i}] has to be contiguous, or strided as its gradient")
+        if len(into) != len(grads):
+            raise ValueError(f"{what}: {len(into)} tensors in out for {len(grads)} gradients")
+        for i, o in enumerate(into):
+            t = dense[i]
+            _seq_check(what, "an entry of out", o, t.shape, t.dtype, t.device)
+            if not (o.is_contiguous() and t.is_contiguous()) and o.stride() != t.stride():
+                if not o.is_contiguous():
+                    raise ValueError(f"{what}: out[{i}] has to be contiguous, or strided as its gradient")
+                dense[i] = t.detach().contiguous()
     if not dense:
         return torch.zeros(())
     _seq_gpu(what, dense[0])
@@ -1916,10 +1951,10 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     arrays, src, sizes = _norm_arrays(dense)
     dst = src if out is None else [t.data_ptr() for t in into]
     _check_disjoint(src, dst, sizes)
-    with _OnDevice(dense[0]):
-        stats = _launch_norm(arrays, n, dense[0].device, norm_type, max_norm, 1.0)
+    with _OnDevice(dense[0]) as stream:
+        stats = _launch_norm(arrays, n, dense[0].device, norm_type, max_norm, 1.0, stream)
         _native.check(_lib().afd_multi_scale(arrays[0], (_native.c_p * n)(*dst), arrays[1], arrays[2], n, stats.data_ptr(),
-                                             _native.stream_ptr()), "afd_multi_scale")
+                                             stream), "afd_multi_scale")
         for g, t in back:
             g.detach().copy_(t)
     return stats[0]
@@ -2016,17 +2051,19 @@ class FusedAdam(torch.optim.Optimizer):
         device, in `last_grad_norm`."""
         g = self.param_groups[0]
         if max_grad_norm is not None:
-            _need(float(max_grad_norm) >= 0.0, f"max_grad_norm {max_grad_norm} has to be a number from 0 on")
+            if not float(max_grad_norm) >= 0.0:
+                raise ValueError(f"max_grad_norm {max_grad_norm} has to be a number from 0 on")
             _seq_gpu("FusedAdam.step", self.flat)
         self.step_count += 1
         self.gather_grads()
         if max_grad_norm is not None:
-            stats = _launch_norm(_norm_arrays([self._flat_grad])[0], 1, self.flat.device, 2.0, float(max_grad_norm),
-                                 float(grad_scale))
-            _native.check(_lib().afd_adam_step_clipped(
-                _native.ptr(self.flat), _native.ptr(self._flat_grad), _native.ptr(self.m), _native.ptr(self.v),
-                self.flat.numel(), g["lr"], g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"], self.step_count,
-                _native.ptr(stats), _native.stream_ptr()), "afd_adam_step_clipped")
+            with _OnDevice(self.flat) as stream:
+                stats = _launch_norm(_norm_arrays([self._flat_grad])[0], 1, self.flat.device, 2.0, float(max_grad_norm),
+                                     float(grad_scale), stream)
+                _native.check(_lib().afd_adam_step_clipped(
+                    _native.ptr(self.flat), _native.ptr(self._flat_grad), _native.ptr(self.m), _native.ptr(self.v),
+                    self.flat.numel(), g["lr"], g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"], self.step_count,
+                    _native.ptr(stats), stream), "afd_adam_step_clipped")
             self.last_grad_norm = stats[0]
             return None
         _native.check(_lib().afd_adam_step(

@@ -190,51 +190,84 @@ template <typename T> int launch_n(const ScanArgs& p, hipStream_t s) {
     return launch<T, 16, 4>(p, s);
 }
 
-// One token.  Every lane reads its NS states before it writes them: state_out may be the state.
-template <typename T, int Q, int NS>
-__global__ void __launch_bounds__(kScanT) scan_step_kernel(const ScanArgs p) {
-    const ScanPlace w = scan_place<Q, NS>(p);
-    if (!w.live) return;  // (whole channels: the Q lanes that meet below are all there or all gone)
-    const size_t st = ((size_t)w.b * p.D + w.ch) * p.N;
-    float a2[NS], h[NS], bv[NS], cv[NS];
-    const T* br = static_cast<const T*>(p.b) + (size_t)w.b * p.bb;
-    const T* cr = static_cast<const T*>(p.c) + (size_t)w.b * p.cb;
-    if (p.N == Q * NS && p.seg) {  // unpadded rows on 16-byte boundaries (seg: what the host found)
-        load_vec<NS>(p.state + st + w.n0, h);
-        load_vec<NS>(p.a + (size_t)w.ch * p.N + w.n0, a2);
-    } else {
-        load_states<NS>(p.state + st, w.n0, p.N, true, h);
-        load_states<NS>(p.a + (size_t)w.ch * p.N, w.n0, p.N, true, a2);
-    }
+// NS neighbouring elements, in one load where there are 8 or 16 bytes of them
+template <typename T, int NS> __device__ __forceinline__ void load_few(const T* p, float (&r)[NS]) {
+    if constexpr (NS * sizeof(T) >= 8) load_row<T, NS>(p, r);
+    else {
 #pragma unroll
-    for (int k = 0; k < NS; ++k) {
-        bv[k] = w.n0 + k < p.N ? to_f32(br[w.n0 + k]) : 0.f;
-        cv[k] = w.n0 + k < p.N ? to_f32(cr[w.n0 + k]) : 0.f;
-    }
-    const float x = to_f32(static_cast<const T*>(p.x)[(size_t)w.b * p.xb + w.ch]);
-    const float raw = to_f32(static_cast<const T*>(p.dt)[(size_t)w.b * p.tb + w.ch]) + (p.dt_bias ? p.dt_bias[w.ch] : 0.f);
-    const float de = p.softplus ? softplus_f32(raw) : raw;
-    float y = 0.f;
-#pragma unroll
-    for (int k = 0; k < NS; ++k) {
-        h[k] = fmaf(__builtin_amdgcn_exp2f(de * (a2[k] * kLog2e)), h[k], de * x * bv[k]);
-        y = fmaf(cv[k], h[k], y);
-    }
-    y = sum_lanes<Q>(y);
-    if (p.N == Q * NS && p.seg) store_vec<NS>(p.state_out + st + w.n0, h);
-    else store_states<NS>(p.state_out + st, w.n0, p.N, true, h);
-    if (w.q == 0) {
-        y = fmaf(p.d ? p.d[w.ch] : 0.f, x, y);
-        if (p.gate) {
-            const float g = to_f32(static_cast<const T*>(p.gate)[(size_t)w.b * p.gb + w.ch]);
-            y *= g * sigmoid_f32(g);
-        }
-        static_cast<T*>(p.y)[(size_t)w.b * p.D + w.ch] = from_f32<T>(y);
+        for (int k = 0; k < NS; ++k) r[k] = to_f32(p[k]);
     }
 }
 
+// One token for RB rows of the batch at a time.  Bound by the state, 8 bytes read and written per channel and state.  With
+// RB = 4 a channel's lanes share the rows' per-token work as they share a sequence's tokens (lane q: softplus and gate of
+// row q), a is loaded once and four state loads are under way per lane; RB = 1 where there are too few rows for that to
+// fill the card.  Every lane reads its states before it writes them: state_out may be the state.
+template <typename T, int Q, int NS, int RB>
+__global__ void __launch_bounds__(kScanT) scan_step_kernel(const ScanArgs p) {
+    const int cb = blockIdx.x % p.nb, b0 = (int)(blockIdx.x / p.nb) * RB;
+    const int q = threadIdx.x & (Q - 1), ch = cb * (kScanT / Q) + (int)threadIdx.x / Q, n0 = q * NS;
+    if (ch >= p.D) return;  // (whole channels: the Q lanes that meet below are all there or all gone)
+    const bool vec = p.N == Q * NS && p.seg;  // unpadded rows on 16-byte boundaries (seg: what the host found)
+    const int r = RB > 1 ? q & (RB - 1) : 0, own = min(b0 + r, p.B - 1);
+    const float x = to_f32(static_cast<const T*>(p.x)[(size_t)own * p.xb + ch]);
+    const float raw = to_f32(static_cast<const T*>(p.dt)[(size_t)own * p.tb + ch]) + (p.dt_bias ? p.dt_bias[ch] : 0.f);
+    const float gt = p.gate ? to_f32(static_cast<const T*>(p.gate)[(size_t)own * p.gb + ch]) : 0.f;
+    float a2[NS], h[RB][NS], bv[RB][NS], cv[RB][NS];
+    if (vec) load_vec<NS>(p.a + (size_t)ch * p.N + n0, a2);
+    else load_states<NS>(p.a + (size_t)ch * p.N, n0, p.N, true, a2);
+#pragma unroll
+    for (int j = 0; j < RB; ++j) {
+        const int b = min(b0 + j, p.B - 1);
+        const float* st = p.state + ((size_t)b * p.D + ch) * p.N;
+        const T* br = static_cast<const T*>(p.b) + (size_t)b * p.bb;
+        const T* cr = static_cast<const T*>(p.c) + (size_t)b * p.cb;
+        if (vec) {
+            load_vec<NS>(st + n0, h[j]);
+            load_few<T, NS>(br + n0, bv[j]);
+            load_few<T, NS>(cr + n0, cv[j]);
+        } else {
+            load_states<NS>(st, n0, p.N, true, h[j]);
+#pragma unroll
+            for (int k = 0; k < NS; ++k) {
+                bv[j][k] = n0 + k < p.N ? to_f32(br[n0 + k]) : 0.f;
+                cv[j][k] = n0 + k < p.N ? to_f32(cr[n0 + k]) : 0.f;
+            }
+        }
+    }
+    const float de = p.softplus ? softplus_f32(raw) : raw, dx = de * x;
+    float yown = 0.f;
+#pragma unroll
+    for (int j = 0; j < RB; ++j) {
+        const float dej = RB > 1 ? from_lane<Q>(de, j) : de, dxj = RB > 1 ? from_lane<Q>(dx, j) : dx;
+        float y = 0.f;
+#pragma unroll
+        for (int k = 0; k < NS; ++k) {
+            h[j][k] = fmaf(__builtin_amdgcn_exp2f(dej * (a2[k] * kLog2e)), h[j][k], dxj * bv[j][k]);
+            y = fmaf(cv[j][k], h[j][k], y);
+        }
+        y = sum_lanes<Q>(y);
+        yown = r == j ? y : yown;
+        if (b0 + j < p.B) {
+            float* so = p.state_out + ((size_t)(b0 + j) * p.D + ch) * p.N;
+            if (vec) store_vec<NS>(so + n0, h[j]);
+            else store_states<NS>(so, n0, p.N, true, h[j]);
+        }
+    }
+    if (q < RB && b0 + q < p.B) {
+        float y = fmaf(p.d ? p.d[ch] : 0.f, x, yown);
+        if (p.gate) y *= gt * sigmoid_f32(gt);
+        static_cast<T*>(p.y)[(size_t)(b0 + q) * p.D + ch] = from_f32<T>(y);
+    }
+}
+
+// Four rows at a time from 8 workgroups per CU on.
 template <typename T, int Q, int NS> int step(const ScanArgs& p, hipStream_t s) {
-    hipLaunchKernelGGL((scan_step_kernel<T, Q, NS>), dim3((unsigned)((long)p.B * p.nb)), dim3(kScanT), 0, s, p);
+    const long one = (long)p.B * p.nb;
+    if (one >= 2048)
+        hipLaunchKernelGGL((scan_step_kernel<T, Q, NS, 4>), dim3((unsigned)((long)((p.B + 3) / 4) * p.nb)), dim3(kScanT), 0, s, p);
+    else
+        hipLaunchKernelGGL((scan_step_kernel<T, Q, NS, 1>), dim3((unsigned)one), dim3(kScanT), 0, s, p);
     return check_launch("scan_step_kernel");
 }
 template <typename T> int step_n(const ScanArgs& p, hipStream_t s) {

@@ -234,6 +234,20 @@ def test_scan_step_takes_unaligned_states_and_strided_rows():
         assert torch.equal(y, want) and torch.equal(st, other)
 
 
+@pytest.mark.parametrize("dtype, b, d, n", [("fp32", 700, 200, 16), ("bf16", 2050, 33, 13), ("fp16", 1031, 130, 32),
+                                            ("bf16", 2049, 64, 8), ("fp32", 2051, 20, 64), ("fp16", 2050, 65, 4)])
+def test_scan_step_of_many_rows(dtype, b, d, n):
+    """Batches large enough to be taken four rows at a time, with rows left over."""
+    t = _scan_inputs(b, dtype, b, 1, d, n)
+    one = {k: t[k][:, 0] for k in ("x", "dt", "b", "c", "gate")}
+    par = {k: t[k] for k in ("a", "d", "dt_bias")}
+    st = t["state"].clone()
+    y = ops.state_scan_step(state=st, **one, **par, softplus=True)
+    want, bound = ref.scan(**t, softplus=True), ref.scan(**t, softplus=True, absolute=True)
+    ref.close(y, want["y"][:, 0], bound["y"][:, 0], 64 + 5, "y")
+    ref.close(st, want["state"], bound["state"], 64 + 5, "state")
+
+
 @pytest.mark.parametrize("l, d", [(40, 48), (400, 10)])
 def test_scan_padding_is_never_read(l, d):
     t = _scan_inputs(11, "bf16", 4, l, d, 16)
