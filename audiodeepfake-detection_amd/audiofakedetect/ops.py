@@ -1842,6 +1842,102 @@ def state_scan_step(x, state, dt, a, b, c, d=None, gate=None, dt_bias=None, soft
     return y
 
 
+_LINEAR_ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _linear_forward(x, w, b, residual, act, keep=False):
+    """(y, pre-activation for the backward or None) for x [M, K]"""
+    m, k = x.shape
+    n = w.shape[0]
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    z = torch.empty((m, n), dtype=x.dtype, device=x.device) if keep and act else None
+    if m > 0:
+        dtype = _SEQ_DTYPES[x.dtype]
+        with _OnDevice(x) as stream:
+            lib = _lib()
+            nbytes = lib.afd_linear_workspace_bytes(m, n, k, dtype)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            _native.check(lib.afd_linear_forward(
+                x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), _at(b), int(b is not None and b.dtype is torch.float32),
+                _at(residual), residual.stride(0) if residual is not None else 0, y.data_ptr(), _at(z), m, n, k, act, dtype,
+                ws.data_ptr(), nbytes, stream), "afd_linear_forward")
+    return y, z
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, residual, act):
+        y, z = _linear_forward(x, w, b, residual, act, ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+                               or ctx.needs_input_grad[2])
+        ctx.save_for_backward(x, w, b, z)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, b, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        m, k = x.shape
+        n = w.shape[0]
+        dx = torch.empty((m, k), dtype=x.dtype, device=x.device) if need[0] else None
+        dw = torch.empty((n, k), dtype=w.dtype, device=x.device) if need[1] else None
+        db = torch.empty_like(b) if need[2] else None
+        if m == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        elif need[0] or need[1] or need[2]:
+            rows, dtype = _rows(dy), _SEQ_DTYPES[x.dtype]
+            with _OnDevice(x) as stream:
+                lib = _lib()
+                nbytes = lib.afd_linear_backward_workspace_bytes(m, n, k, dtype)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+                _native.check(lib.afd_linear_backward(
+                    x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), _at(z), rows.data_ptr(), rows.stride(0), _at(dx),
+                    _at(dw), _at(db), int(b is not None and b.dtype is torch.float32), m, n, k, ctx.act, dtype,
+                    ws.data_ptr(), nbytes, stream), "afd_linear_backward")
+        return dx, dw, db, dy if need[3] else None, None
+
+
+def linear(x, w, b=None, activation: str = "none", residual=None):
+    """act(x @ w.T + b) + residual in one pass: x [..., K], w [N, K] and residual [..., N] of one type (float32 / bfloat16 /
+    float16), b [N] float32 or of that type; `activation` "none", "relu", "silu" or "gelu" (with the error function).  float32
+    products are exact, all sums are float32, the result is rounded once.  Differentiable in every tensor; the backward
+    takes the activation's slope at x @ w.T + b rounded to the type of x, and rounds the gradient in front of its two
+    products to it."""
+    what = "linear"
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{what}: x is a {type(x).__name__}, not a tensor")
+    if x.dim() < 1:
+        raise ValueError(f"{what}: x has no dimensions")
+    if x.dtype not in _SEQ_DTYPES:
+        raise TypeError(f"{what}: x is {x.dtype}; float32, bfloat16 or float16 expected")
+    if not isinstance(w, torch.Tensor):
+        raise TypeError(f"{what}: w is a {type(w).__name__}, not a tensor")
+    k = x.shape[-1]
+    if w.dim() != 2 or w.shape[1] != k or w.shape[0] < 1 or k < 1:
+        raise ValueError(f"{what}: w has shape {tuple(w.shape)}, (outputs, {k}) expected, neither of them zero")
+    n = w.shape[0]
+    _seq_check(what, "w", w, w.shape, x.dtype, x.device)
+    if b is not None:
+        if not isinstance(b, torch.Tensor):
+            raise TypeError(f"{what}: b is a {type(b).__name__}, not a tensor")
+        _seq_check(what, "b", b, (n,), torch.float32 if b.dtype is torch.float32 else x.dtype, x.device)
+    _seq_check(what, "residual", residual, (*x.shape[:-1], n), x.dtype, x.device)
+    if activation not in _LINEAR_ACTIVATIONS:
+        raise ValueError(f"{what}: activation {activation!r}; one of {sorted(_LINEAR_ACTIVATIONS)} expected")
+    _seq_gpu(what, x)
+    rows = _rows(x.reshape(-1, k))
+    res = _rows(residual.reshape(-1, n)) if residual is not None else None
+    w, b = _rows(w), _dense(b)
+    if _wants_grad(rows, w, b, res):
+        y = _Linear.apply(rows, w, b, res, _LINEAR_ACTIVATIONS[activation])
+    else:
+        y = _linear_forward(rows, w, b, res, _LINEAR_ACTIVATIONS[activation])[0]
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
+
+
 # --------------------------------------------------------------------------------------
 def _gapless(t: torch.Tensor) -> bool:
     """Does `t` fill its memory without gaps or repeats, in whatever order of its axes?"""

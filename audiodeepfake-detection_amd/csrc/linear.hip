@@ -1,0 +1,587 @@
+// y = act(x w^T + bias) + residual and its backward, on the matrix cores: fp32 (v_mfma_f32_32x32x2_f32, exact products),
+// bf16 and fp16 (32x32x16, sums in fp32).
+//
+// One kernel computes C[m][n] = sum_k A[m][k] B[n][k] for operands whose rows are contiguous along k: the forward as it
+// stands, dx with w transposed, dw with dz and x transposed (small passes of this file, which also take operands whose
+// rows do not start on 16-byte boundaries or do not end on them).  A workgroup owns a TM x TN tile; 128 bytes of k per row
+// are staged in LDS, double buffered: the next slab's global loads are issued before the current slab's products and
+// written to LDS behind them, one barrier per slab.  Both operands of a lane are 16-byte reads: lane l holds row l % 32 and the
+// (2 s + l / 32)-th 16 bytes of its slab, which are 8 bf16 (one 32x32x16 product) or 4 fp32 (four 32x32x2 products, whose k
+// order does not matter as long as both operands agree).  Chunks are XORed with the row, so 8 rows' reads of one chunk
+// number spread over all banks.
+// Few tiles: the k axis is split over workgroups, which leave fp32 partial tiles for a second kernel with the same epilogue.
+#include "seq_common.h"
+
+namespace {
+
+using namespace afd;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kSlab = 128;  // bytes of k per row and slab
+
+enum Act { kNone, kRelu, kSilu, kGelu };
+
+__device__ __forceinline__ float activate(float z, int act) {
+    if (act == kRelu) return z < 0.f ? 0.f : z;  // (NaN stays)
+    if (act == kSilu) return z * sigmoid_f32(z);
+    if (act == kGelu) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    return z;
+}
+__device__ __forceinline__ float activate_slope(float z, int act) {
+    if (act == kRelu) return z > 0.f ? 1.f : 0.f;
+    if (act == kSilu) {
+        const float s = sigmoid_f32(z);
+        return s * (1.f + z * (1.f - s));
+    }
+    if (act == kGelu)
+        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * z * z);
+    return 1.f;
+}
+
+struct Epi {
+    const void* bias;  // [N], NULL: none
+    int bias_f32;
+    const void* residual;  // rows of ldr elements, NULL: none
+    long ldr;
+    void* out;  // rows of ldo elements
+    long ldo;
+    void* z;  // pre-activation, rows of N elements, NULL: not kept
+    int act;
+};
+
+struct Gemm {
+    const void *a, *b;
+    long lda, ldb;
+    int M, N, K;
+    Epi e;
+    float* part;  // split k: [S][M][ldp] partial sums
+    long ldp;
+    int S, ksplit;  // splits and slabs per split
+    int tm, tn;     // tiles
+};
+
+// The pre-activation is kept in the type of the tensors.  A value that rounds to zero there would lose the side of relu's
+// corner it is on, one beyond fp16's range would become inf and give NaN as inf times the 0 of a slope: both stay
+// just inside.
+template <typename T> __device__ __forceinline__ T keep_z(float z) {
+    if constexpr (sizeof(T) == 2 && __is_same(T, f16_t)) {
+        if (fabsf(z) > 65504.f) return z > 0.f ? (T)65504.f : (z < 0.f ? (T)-65504.f : (T)z);
+        if (z != 0.f && fabsf(z) < 5.9604645e-8f) return z > 0.f ? (T)5.9604645e-8f : (T)-5.9604645e-8f;
+    }
+    return from_f32<T>(z);
+}
+
+// V consecutive columns n .. n + V of row m
+template <typename T, int V>
+__device__ __forceinline__ void finish(const Epi& e, int m, int n, int N, float (&v)[V], const float (&bias)[V]) {
+    T* out = static_cast<T*>(e.out) + (size_t)m * e.ldo + n;
+    const T* res = e.residual ? static_cast<const T*>(e.residual) + (size_t)m * e.ldr + n : nullptr;
+    T* zp = e.z ? static_cast<T*>(e.z) + (size_t)m * N + n : nullptr;
+    constexpr int W = 16 / (int)sizeof(T);
+    if (n + V <= N) {
+#pragma unroll
+        for (int g = 0; g < V; g += W) {
+            float r[W], o[W];
+            if (res) load_row<T, W>(res + g, r);
+            Pack<T, W> zk;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const float z = v[g + i] + bias[g + i];
+                if (zp) zk.v[i] = keep_z<T>(z);
+                o[i] = activate(z, e.act);
+                if (res) o[i] += r[i];
+            }
+            if (zp) *reinterpret_cast<u32x4_any*>(zp + g) = __builtin_bit_cast(u32x4, zk);
+            store_row<T, W>(out + g, o);
+        }
+    } else {
+        for (int i = 0; i < V && n + i < N; ++i) {
+            const float z = v[i] + bias[i];
+            if (zp) zp[i] = keep_z<T>(z);
+            const float o = activate(z, e.act);
+            out[i] = from_f32<T>(res ? o + to_f32(res[i]) : o);
+        }
+    }
+}
+
+template <typename T, int V> __device__ __forceinline__ void load_bias(const Epi& e, int n, int N, float (&b)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        b[i] = 0.f;
+        if (e.bias && n + i < N)
+            b[i] = e.bias_f32 ? static_cast<const float*>(e.bias)[n + i] : to_f32(static_cast<const T*>(e.bias)[n + i]);
+    }
+}
+
+template <typename T> __device__ __forceinline__ void mma(const u32x4& a, const u32x4& b, f32x16& c) {
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
+    } else if constexpr (__is_same(T, bf16_t)) {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+}
+
+// Tile of this workgroup.  Workgroups go to the 8 XCDs in turn; each XCD takes a contiguous run of tiles, in groups of 8 tile
+// rows walked column by column, so the rows of A and B that its workgroups share stay in its L2.
+__device__ __forceinline__ void tile_of(const Gemm& g, int id, int& tm, int& tn) {
+    const int total = g.tm * g.tn, each = total / 8, left = total % 8;
+    const int x = id % 8, i = id / 8;
+    const int t = x * each + min(x, left) + i;
+    const int per = 8 * g.tn, grp = t / per, in = t - grp * per;
+    const int rows = min(8, g.tm - grp * 8);
+    tm = grp * 8 + in % rows;
+    tn = in / rows;
+}
+
+template <typename T, int TM, int TN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(const Gemm g) {
+    constexpr int kThreads = 64 * WM * WN, MI = TM / WM / 32, NI = TN / WN / 32;
+    constexpr int EPC = 16 / (int)sizeof(T), KS = kSlab / (int)sizeof(T);  // elements per chunk and per slab
+    constexpr int CA = TM * 8 / kThreads, CB = TN * 8 / kThreads;          // chunks a thread stages
+    constexpr int kBuf = (TM + TN) * kSlab;
+    extern __shared__ char lds[];
+    int tm, tn;
+    tile_of(g, blockIdx.x, tm, tn);
+    const int m0 = tm * TM, n0 = tn * TN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave % WM, wn = wave / WM, l31 = lane & 31, half = lane >> 5;
+    const int kbeg = blockIdx.y * g.ksplit * KS, kend = min(kbeg + g.ksplit * KS, g.K);
+
+    // operands: a uniform base that moves along k plus a fixed 32-bit offset per chunk; rows behind the matrix repeat its last
+    const T* ab = static_cast<const T*>(g.a) + (size_t)m0 * g.lda + kbeg;
+    const T* bb = static_cast<const T*>(g.b) + (size_t)n0 * g.ldb + kbeg;
+    unsigned oa[CA], ob[CB], la[CA], lb[CB];
+    int chunk[CA > CB ? CA : CB];
+#pragma unroll
+    for (int e = 0; e < (CA > CB ? CA : CB); ++e) chunk[e] = (e * kThreads + tid) & 7;
+#pragma unroll
+    for (int e = 0; e < CA; ++e) {
+        const int row = (e * kThreads + tid) >> 3;
+        oa[e] = (unsigned)((size_t)min(row, g.M - 1 - m0) * g.lda * sizeof(T)) + chunk[e] * 16;
+        la[e] = row * kSlab + ((chunk[e] ^ (row & 7)) * 16);
+    }
+#pragma unroll
+    for (int e = 0; e < CB; ++e) {
+        const int row = (e * kThreads + tid) >> 3;
+        ob[e] = (unsigned)((size_t)min(row, g.N - 1 - n0) * g.ldb * sizeof(T)) + chunk[e] * 16;
+        lb[e] = TM * kSlab + row * kSlab + ((chunk[e] ^ (row & 7)) * 16);
+    }
+    u32x4 ra[CA], rb[CB];
+    auto fetch = [&](int k) {
+        const T* pa = ab + (k - kbeg);
+        const T* pb = bb + (k - kbeg);
+        auto at = [](const T* p, unsigned off) { return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p) + off); };
+        if (k + KS <= kend) {
+#pragma unroll
+            for (int e = 0; e < CA; ++e) ra[e] = at(pa, oa[e]);
+#pragma unroll
+            for (int e = 0; e < CB; ++e) rb[e] = at(pb, ob[e]);
+        } else {  // (kend is a multiple of a chunk)
+#pragma unroll
+            for (int e = 0; e < CA; ++e) ra[e] = k + chunk[e] * EPC < kend ? at(pa, oa[e]) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < CB; ++e) rb[e] = k + chunk[e] * EPC < kend ? at(pb, ob[e]) : u32x4{0, 0, 0, 0};
+        }
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int e = 0; e < CA; ++e) *reinterpret_cast<u32x4*>(lds + buf * kBuf + la[e]) = ra[e];
+#pragma unroll
+        for (int e = 0; e < CB; ++e) *reinterpret_cast<u32x4*>(lds + buf * kBuf + lb[e]) = rb[e];
+    };
+
+    f32x16 acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+    const int arow = wm * (TM / WM) + l31, brow = wn * (TN / WN) + l31;
+    if (kbeg < kend) {
+        fetch(kbeg);
+        put(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int k = kbeg; k < kend; k += KS, buf ^= 1) {
+        const bool more = k + KS < kend;
+        if (more) fetch(k + KS);
+        const char* base = lds + buf * kBuf;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            u32x4 fa[MI], fb[NI];
+            const int c = 2 * s + half;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+                fa[i] = *reinterpret_cast<const u32x4*>(base + (arow + i * 32) * kSlab + ((c ^ (l31 & 7)) * 16));
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+                fb[j] = *reinterpret_cast<const u32x4*>(base + TM * kSlab + (brow + j * 32) * kSlab + ((c ^ (l31 & 7)) * 16));
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) mma<T>(fa[i], fb[j], acc[i][j]);
+        }
+        if (more) put(buf ^ 1);
+        __syncthreads();
+    }
+
+    // Epilogue, wave by wave through LDS (nobody reads the slabs any more): 32 rows of the wave's columns at a time, then
+    // 8 columns per lane in row order.
+    constexpr int WC = NI * 32, kPitch = WC + 4;
+    float* tile = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
+    constexpr int LPR = WC / 8, RPP = 64 / LPR;  // lanes per row, rows per pass
+    const int col = (lane % LPR) * 8, n = n0 + wn * WC + col;
+    float bias[8];
+    if (g.S == 1) load_bias<T, 8>(g.e, n, g.N, bias);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) tile[((r & 3) + 8 * (r >> 2) + 4 * half) * kPitch + j * 32 + l31] = acc[i][j][r];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int p = 0; p < 32; p += RPP) {
+            const int row = p + lane / LPR, m = m0 + wm * (TM / WM) + i * 32 + row;
+            float v[8];
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + row * kPitch + col);
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(tile + row * kPitch + col + 4);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                v[c] = lo[c];
+                v[4 + c] = hi[c];
+            }
+            if (m < g.M && n < g.N) {
+                if (g.S > 1) {  // (ldp is a multiple of 8)
+                    float* dst = g.part + ((size_t)blockIdx.y * g.M + m) * g.ldp + n;
+                    *reinterpret_cast<f32x4*>(dst) = lo;
+                    *reinterpret_cast<f32x4*>(dst + 4) = hi;
+                } else {
+                    finish<T, 8>(g.e, m, n, g.N, v, bias);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Sum of the k splits' partial tiles, and the epilogue.
+template <typename T> __global__ void __launch_bounds__(256) join_kernel(const Gemm g) {
+    const long groups = g.ldp / 8, all = (long)g.M * groups;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
+        const int m = (int)(i / groups), n = (int)(i - (long)m * groups) * 8;
+        if (n >= g.N) continue;
+        float v[8], bias[8];
+        load_bias<T, 8>(g.e, n, g.N, bias);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = 0.f;
+        for (int s = 0; s < g.S; ++s) {
+            const float* src = g.part + ((size_t)s * g.M + m) * g.ldp + n;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(src), hi = *reinterpret_cast<const f32x4*>(src + 4);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                v[c] += lo[c];
+                v[4 + c] += hi[c];
+            }
+        }
+        finish<T, 8>(g.e, m, n, g.N, v, bias);
+    }
+}
+
+// dst[c][r] = src[r][c] for R x C elements, rows of dst padded with zeros to ldd (a multiple of 16 bytes).  64 x 64 tiles
+// through LDS.
+template <typename T>
+__global__ void __launch_bounds__(256) turn_kernel(const T* __restrict__ src, long lds_, int R, int C, T* __restrict__ dst, long ldd) {
+    __shared__ T t[64][64 + 4 / sizeof(T)];
+    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < 64; i += 4) {
+        const int r = r0 + i + y, c = c0 + x;
+        t[i + y][x] = r < R && c < C ? src[(size_t)r * lds_ + c] : (T)0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 64; i += 4) {
+        const int c = c0 + i + y, r = r0 + x;
+        if (c < C && r < ldd) dst[(size_t)c * ldd + r] = t[x][i + y];
+    }
+}
+
+// dst[r][0 .. ldd) = src[r][0 .. C), zeros behind it
+template <typename T>
+__global__ void __launch_bounds__(256) pad_kernel(const T* __restrict__ src, long lds_, int R, int C, T* __restrict__ dst, long ldd) {
+    const long all = (long)R * ldd;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
+        const long r = i / ldd, c = i - r * ldd;
+        dst[i] = c < C ? src[(size_t)r * lds_ + c] : (T)0.f;
+    }
+}
+
+// dz = dy act'(z) as rows (ldz, zeros behind N; NULL: not wanted) and turned (ldt, zeros behind M), and its column sums over
+// the tile's rows.
+template <typename T>
+__global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ dy, long ldy, const T* __restrict__ z, int act, int M, int N,
+                                                 T* __restrict__ dz, long ldz, T* __restrict__ turned, long ldt,
+                                                 float* __restrict__ sums) {
+    __shared__ float t[64][65];
+    const int m0 = blockIdx.x * 64, n0 = blockIdx.y * 64;
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 64; i += 4) {
+        const int m = m0 + i + y, n = n0 + x;
+        float v = 0.f;
+        if (m < M && n < N) {
+            v = to_f32(dy[(size_t)m * ldy + n]);
+            if (act != kNone) v *= activate_slope(to_f32(z[(size_t)m * N + n]), act);
+        }
+        s += v;
+        t[i + y][x] = v;
+        if (dz && m < M && n < ldz) dz[(size_t)m * ldz + n] = from_f32<T>(v);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 64; i += 4) {
+        const int n = n0 + i + y, m = m0 + x;
+        if (n < N && m < ldt) turned[(size_t)n * ldt + m] = from_f32<T>(t[x][i + y]);
+    }
+    if (!sums) return;
+    __shared__ float red[4][64];
+    red[y][x] = s;
+    __syncthreads();
+    if (y == 0 && n0 + x < N) sums[(size_t)blockIdx.x * N + n0 + x] = (red[0][x] + red[1][x]) + (red[2][x] + red[3][x]);
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+long pad_to(long n, long k) { return (n + k - 1) / k * k; }
+
+struct Shape {
+    int kind;  // 0: 32 x 128, 1: 128 x 128 tiles
+    int tm, tn, S, ksplit;
+    size_t part;
+};
+Shape gemm_shape(int M, int N, int K, int dtype) {
+    Shape s;
+    const int ks = kSlab / (int)dtype_bytes(dtype);
+    s.kind = M <= 32 ? 0 : 1;
+    s.tm = ceil_div(M, s.kind ? 128 : 32);
+    s.tn = ceil_div(N, 128);
+    const long tiles = (long)s.tm * s.tn;
+    const int slabs = ceil_div(K, ks);
+    int want = 1;
+    if (tiles < 256) {
+        want = (int)((512 + tiles - 1) / tiles);
+        const int most = slabs / (s.kind ? 4 : 2);
+        if (want > most) want = most;
+        if (want < 1) want = 1;
+    }
+    s.ksplit = ceil_div(slabs, want);
+    s.S = ceil_div(slabs, s.ksplit);
+    s.part = s.S > 1 ? align256((size_t)s.S * M * pad_to(N, 8) * 4) : 0;
+    return s;
+}
+
+template <typename T, int TM, int TN, int WM, int WN> void launch_tile(const Gemm& g, hipStream_t s) {
+    constexpr int kBuf = 2 * (TM + TN) * kSlab, kEpi = WM * WN * 32 * (TN / WN + 4) * 4;
+    constexpr unsigned lds = kBuf > kEpi ? kBuf : kEpi;
+    hipLaunchKernelGGL((gemm_kernel<T, TM, TN, WM, WN>), dim3((unsigned)(g.tm * g.tn), (unsigned)g.S), dim3(64 * WM * WN), lds, s, g);
+}
+
+template <typename T> int gemm_t(const Gemm& g, int kind, hipStream_t s) {
+    if (kind == 0) launch_tile<T, 32, 128, 1, 4>(g, s);
+    else launch_tile<T, 128, 128, 2, 2>(g, s);
+    if (g.S > 1) {
+        const long all = (long)g.M * (g.ldp / 8), grid = (all + 255) / 256;
+        hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0, s, g);
+    }
+    return check_launch("gemm_kernel");
+}
+
+// C = A B^T with the epilogue; operands on 16-byte boundaries, K a multiple of 16 bytes.
+int gemm(const void* a, long lda, const void* b, long ldb, int M, int N, int K, const Epi& e, int dtype, float* part, hipStream_t s) {
+    const Shape q = gemm_shape(M, N, K, dtype);
+    Gemm g{};
+    g.a = a; g.b = b; g.lda = lda; g.ldb = ldb; g.M = M; g.N = N; g.K = K; g.e = e; g.part = part; g.ldp = pad_to(N, 8);
+    g.S = q.S; g.ksplit = q.ksplit; g.tm = q.tm; g.tn = q.tn;
+    if (dtype == AFD_T_F32) return gemm_t<float>(g, q.kind, s);
+    if (dtype == AFD_T_BF16) return gemm_t<bf16_t>(g, q.kind, s);
+    return gemm_t<f16_t>(g, q.kind, s);
+}
+
+template <typename T> int turn_t(const void* src, long ld, int R, int C, void* dst, long ldd, hipStream_t s) {
+    hipLaunchKernelGGL(turn_kernel<T>, dim3((unsigned)ceil_div(ldd, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, s,
+                       static_cast<const T*>(src), ld, R, C, static_cast<T*>(dst), ldd);
+    return check_launch("turn_kernel");
+}
+// (types of one size move alike)
+int turn(const void* src, long ld, int R, int C, void* dst, long ldd, int dtype, hipStream_t s) {
+    return dtype == AFD_T_F32 ? turn_t<float>(src, ld, R, C, dst, ldd, s) : turn_t<bf16_t>(src, ld, R, C, dst, ldd, s);
+}
+int pad(const void* src, long ld, int R, int C, void* dst, long ldd, int dtype, hipStream_t s) {
+    const long grid = ((long)R * ldd + 255) / 256;
+    const dim3 d((unsigned)(grid < 65536 ? grid : 65536));
+    if (dtype == AFD_T_F32)
+        hipLaunchKernelGGL(pad_kernel<float>, d, dim3(256), 0, s, static_cast<const float*>(src), ld, R, C, static_cast<float*>(dst), ldd);
+    else
+        hipLaunchKernelGGL(pad_kernel<bf16_t>, d, dim3(256), 0, s, static_cast<const bf16_t*>(src), ld, R, C, static_cast<bf16_t*>(dst), ldd);
+    return check_launch("pad_kernel");
+}
+
+// May the product's kernel read these rows as they are?
+bool direct(const void* p, long ld, int K, int dtype) {
+    const long epc = 16 / (long)dtype_bytes(dtype);
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % epc == 0 && K % epc == 0 && ld <= (1 << 20);
+}
+
+int check(const char* what, long M, int N, int K, int act, int dtype) {
+    if (M < 1 || N < 1 || K < 1 || act < 0 || act > 3 || !dtype_ok(dtype))
+        return fail(AFD_ERR_ARG, "%s: M=%ld N=%d K=%d act=%d dtype=%d", what, M, N, K, act, dtype);
+    if (M > 0x7fffff00L || N > (1 << 20) - 64 || K > (1 << 20) - 64 || (long)ceil_div(M, 128) * ceil_div(N, 128) > 0x7fffffffL)
+        return fail(AFD_ERR_UNSUPPORTED, "%s: M=%ld N=%d K=%d is too large", what, M, N, K);
+    return AFD_OK;
+}
+
+struct Arena {
+    char* base;
+    size_t at, size;
+    void* take(size_t n) {
+        void* p = base + at;
+        at += align256(n);
+        return p;
+    }
+};
+
+}  // namespace
+
+extern "C" size_t afd_linear_workspace_bytes(long long M, int N, int K, int dtype) {
+    if (M < 1 || N < 1 || K < 1 || !dtype_ok(dtype)) return 0;
+    const size_t e = dtype_bytes(dtype);
+    const long kp = pad_to(K, 16 / (long)e);
+    // (copies of operands that cannot be read as they are: counted always, one size for a shape)
+    return align256((size_t)M * kp * e) + align256((size_t)N * kp * e) + gemm_shape((int)M, N, K, dtype).part;
+}
+
+extern "C" int afd_linear_forward(const void* x, long long ldx, const void* w, long long ldw, const void* bias, int bias_f32,
+                                  const void* residual, long long ldr, void* y, void* z, long long M, int N, int K, int act,
+                                  int dtype, void* ws, size_t ws_bytes, afd_stream_t stream) {
+    if (!x || !w || !y) return fail(AFD_ERR_ARG, "linear: missing tensor");
+    if (int rc = check("linear", M, N, K, act, dtype)) return rc;
+    const size_t e = dtype_bytes(dtype);
+    const long kp = pad_to(K, 16 / (long)e);
+    const bool dx = direct(x, ldx, K, dtype), dw = direct(w, ldw, K, dtype);
+    const size_t need = (dx ? 0 : align256((size_t)M * kp * e)) + (dw ? 0 : align256((size_t)N * kp * e)) +
+                        gemm_shape((int)M, N, (int)kp, dtype).part;
+    if (need > 0 && (!ws || ws_bytes < need)) return fail(AFD_ERR_WORKSPACE, "linear: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    ScopedTiming timing(AFD_K_SEQUENCE, 2.0 * (double)M * N * K, s);
+    Arena ar{static_cast<char*>(ws), 0, ws_bytes};
+    if (!dx) {
+        void* c = ar.take((size_t)M * kp * e);
+        if (int rc = pad(x, ldx, (int)M, K, c, kp, dtype, s)) return rc;
+        x = c;
+        ldx = kp;
+    }
+    if (!dw) {
+        void* c = ar.take((size_t)N * kp * e);
+        if (int rc = pad(w, ldw, N, K, c, kp, dtype, s)) return rc;
+        w = c;
+        ldw = kp;
+    }
+    Epi ep{bias, bias_f32, residual, ldr, y, N, z, act};
+    return gemm(x, ldx, w, ldw, (int)M, N, (int)kp, ep, dtype, reinterpret_cast<float*>(ar.base + ar.at), s);
+}
+
+namespace {
+struct BackPlan {
+    long mp, np;  // padded lengths of the k axes
+    size_t dz, dzt, xt, wt, sums, part, total;
+};
+BackPlan back_plan(long M, int N, int K, int dtype) {
+    BackPlan b;
+    const size_t e = dtype_bytes(dtype);
+    const long epc = 16 / (long)e;
+    b.mp = pad_to(M, epc);
+    b.np = pad_to(N, epc);
+    b.dz = align256((size_t)M * b.np * e);
+    b.dzt = align256((size_t)N * b.mp * e);
+    b.xt = align256((size_t)K * b.mp * e);
+    b.wt = align256((size_t)K * b.np * e);
+    b.sums = align256((size_t)ceil_div(b.mp, 64) * N * 4);
+    const size_t p1 = gemm_shape((int)M, K, (int)b.np, dtype).part, p2 = gemm_shape(N, K, (int)b.mp, dtype).part;
+    b.part = p1 > p2 ? p1 : p2;
+    b.total = b.dz + b.dzt + b.xt + b.wt + b.sums + b.part;
+    return b;
+}
+template <typename T>
+int dz_t(const void* dy, long ldy, const void* z, int act, int M, int N, void* dz, long ldz, void* t, long ldt, float* sums, hipStream_t s) {
+    const long rows = ldt > M ? ldt : M;
+    const long cols = dz && ldz > N ? ldz : N;
+    hipLaunchKernelGGL(dz_kernel<T>, dim3((unsigned)ceil_div(rows, 64), (unsigned)ceil_div(cols, 64)), dim3(256), 0, s,
+                       static_cast<const T*>(dy), ldy, static_cast<const T*>(z), act, M, N, static_cast<T*>(dz), ldz,
+                       static_cast<T*>(t), ldt, sums);
+    return check_launch("dz_kernel");
+}
+}  // namespace
+
+extern "C" size_t afd_linear_backward_workspace_bytes(long long M, int N, int K, int dtype) {
+    if (M < 1 || N < 1 || K < 1 || !dtype_ok(dtype)) return 0;
+    return back_plan(M, N, K, dtype).total;
+}
+
+extern "C" int afd_linear_backward(const void* x, long long ldx, const void* w, long long ldw, const void* z, const void* dy,
+                                   long long ldy, void* dx, void* dw, void* dbias, int bias_f32, long long M, int N, int K,
+                                   int act, int dtype, void* ws, size_t ws_bytes, afd_stream_t stream) {
+    if (!x || !w || !dy || (act != kNone && !z)) return fail(AFD_ERR_ARG, "linear backward: missing tensor");
+    if (int rc = check("linear backward", M, N, K, act, dtype)) return rc;
+    // (a tile's rows of the turned operands have to be within a 32-bit offset of each other)
+    if (M > 8000000) return fail(AFD_ERR_UNSUPPORTED, "linear backward: M=%lld, at most 8000000 rows", M);
+    const BackPlan b = back_plan(M, N, K, dtype);
+    if (!ws || ws_bytes < b.total)
+        return fail(AFD_ERR_WORKSPACE, "linear backward: workspace of %zu bytes, %zu needed", ws_bytes, b.total);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    ScopedTiming timing(AFD_K_SEQUENCE, 2.0 * (double)M * N * K * ((dx != nullptr) + (dw != nullptr)), s);
+    Arena ar{static_cast<char*>(ws), 0, ws_bytes};
+    void* dz = ar.take(b.dz);
+    void* dzt = ar.take(b.dzt);
+    void* xt = ar.take(b.xt);
+    void* wt = ar.take(b.wt);
+    float* sums = static_cast<float*>(ar.take(b.sums));
+    float* part = reinterpret_cast<float*>(ar.base + ar.at);
+    // without an activation dy is dz, and can be read as it is where its rows allow
+    const bool rows = act != kNone || !direct(dy, ldy, N, dtype);
+    void* rz = dx && rows ? dz : nullptr;
+    int rc = dtype == AFD_T_F32 ? dz_t<float>(dy, ldy, z, act, (int)M, N, rz, b.np, dzt, b.mp, dbias ? sums : nullptr, s)
+             : dtype == AFD_T_BF16 ? dz_t<bf16_t>(dy, ldy, z, act, (int)M, N, rz, b.np, dzt, b.mp, dbias ? sums : nullptr, s)
+                                   : dz_t<f16_t>(dy, ldy, z, act, (int)M, N, rz, b.np, dzt, b.mp, dbias ? sums : nullptr, s);
+    if (rc) return rc;
+    if (dbias) {
+        ColumnOuts o{};
+        o.n = 1;
+        o.o[0] = {dbias, 0, N, 1, 1, 1, 0, bias_f32 ? AFD_T_F32 : dtype};
+        if (int r = launch_column_sums(sums, ceil_div(b.mp, 64), N, o, s)) return r;
+    }
+    if (dx) {
+        if (int r = turn(w, ldw, N, K, wt, b.np, dtype, s)) return r;
+        Epi e{nullptr, 0, nullptr, 0, dx, K, nullptr, kNone};
+        if (int r = gemm(rows ? dz : dy, rows ? b.np : ldy, wt, b.np, (int)M, K, (int)b.np, e, dtype, part, s)) return r;
+    }
+    if (dw) {
+        if (int r = turn(x, ldx, (int)M, K, xt, b.mp, dtype, s)) return r;
+        Epi e{nullptr, 0, nullptr, 0, dw, K, nullptr, kNone};
+        if (int r = gemm(dzt, b.mp, xt, b.mp, N, K, (int)b.mp, e, dtype, part, s)) return r;
+    }
+    return AFD_OK;
+}

@@ -130,3 +130,22 @@ def close(got, ref, bound, roundings, what=""):
         raise AssertionError(f"{what}: {int((over > 0).sum())} of {over.numel()} outside; worst at {i}: "
                              f"got {float(g.flatten()[i])!r}, ref {float(ref.flatten()[i])!r}, "
                              f"allowed {float(tol.flatten()[i])!r}")
+
+
+def linear(x, w, b=None, act="none", residual=None, dy=None, absolute=False):
+    """dict of y and, with dy, dx / dw / db; x [M, K].  absolute: the sums of magnitudes, through slopes of at most 1.13 and
+    the change of the slope (at most 1 per unit of z) under an error of z."""
+    f = (lambda t: t.abs()) if absolute else (lambda t: t)
+    x, w = d64(x), d64(w)
+    z = x @ w.t() + (0 if b is None else d64(b))
+    za = f(x) @ f(w).t() + (0 if b is None else f(d64(b)))
+    s, cdf = torch.sigmoid(z), 0.5 * torch.erfc(-z * 0.5 ** 0.5)
+    y, slope = {"none": (z, torch.ones_like(z)), "relu": (z.clamp(min=0), (z > 0).double()), "silu": (z * s, s + z * s * (1 - s)),
+                "gelu": (z * cdf, cdf + z * torch.exp(-0.5 * z * z) / (2 * torch.pi) ** 0.5)}[act]
+    if absolute:
+        y, slope = 1.13 * za, 1.13 + za
+    out = {"y": y if residual is None else y + f(d64(residual)), "z": z}
+    if dy is not None:
+        dz = f(d64(dy)) * slope
+        out.update(dx=dz @ f(w), dw=dz.t() @ f(x), db=dz.sum(0), dz=dz)
+    return out

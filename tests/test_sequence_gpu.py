@@ -695,3 +695,157 @@ def test_a_recording_scored_as_it_arrives():
             want = rows(whole)
             # the same steps in another kernel: sums of 16 products in another order, 30 tokens of decay
             assert float((yk - want).abs().max()) <= (64 + 5 * 30) * 2.0 ** -23 * float(whole.abs().max())
+
+
+# ---- projections -------------------------------------------------------------------------------------------------------
+LINEAR = [
+    # dtype, M, K, N, act, bias, residual
+    ("fp32", 1, 1, 1, "none", None, False),
+    ("fp32", 3, 5, 7, "silu", "fp32", True),
+    ("fp32", 33, 64, 128, "gelu", "fp32", False),
+    ("fp32", 130, 100, 257, "relu", "fp32", True),
+    ("fp32", 200, 1031, 90, "silu", None, False),
+    ("bf16", 1, 64, 64, "gelu", "fp32", True),
+    ("bf16", 17, 8, 300, "silu", "same", False),
+    ("bf16", 129, 264, 136, "none", "fp32", True),
+    ("bf16", 300, 1000, 131, "gelu", "fp32", True),
+    ("bf16", 5, 2048, 520, "silu", "fp32", False),   # few rows: the k axis is split
+    ("bf16", 256, 4096, 128, "none", None, True),
+    ("fp16", 31, 33, 65, "gelu", "same", False),
+    ("fp16", 140, 513, 250, "relu", "fp32", True),
+    ("fp16", 64, 72, 1000, "silu", None, False),
+    ("fp16", 1000, 16, 16, "none", "same", False),
+]
+
+
+@pytest.mark.parametrize("dtype, m, k, n, act, bias, residual", LINEAR)
+def test_linear_forward_and_gradients(dtype, m, k, n, act, bias, residual):
+    """y: K products and sums, then 10 (erf 4 ulp of a value up to 2, slope 1.13); a partial tile per split is one of the
+    sums.  dz is rounded to the type and its slope taken at a rounded z: two half steps relative to dy's magnitude (and |z|
+    for the second, whose slope changes by at most 1 per unit), which enter the two products like any other error."""
+    g = torch.Generator().manual_seed(m + k + n)
+    t = TYPES[dtype]
+    v = dict(x=_rnd(g, m, k, dtype=t), w=_rnd(g, n, k, scale=k ** -0.5, dtype=t),
+             b=None if bias is None else _rnd(g, n, dtype=t if bias == "same" else torch.float32),
+             residual=_rnd(g, m, n, dtype=t) if residual else None)
+    if act == "relu":  # no pre-activation within its rounding errors of the corner
+        z = ref.linear(v["x"], v["w"], v["b"])["z"]
+        near = (z.abs() < 1e-3).any(1)
+        v["x"][near.cuda()] = 0
+        if bias is None:
+            v["x"][near.cuda()] = 0
+    for x in v.values():
+        if x is not None:
+            x.requires_grad_(True)
+    y = ops.linear(v["x"], v["w"], v["b"], act, residual=v["residual"])
+    with torch.no_grad():
+        assert torch.equal(ops.linear(v["x"], v["w"], v["b"], act, residual=v["residual"]), y)
+    dy = _rnd(g, m, n, dtype=t)
+    names = [key for key, x in v.items() if x is not None]
+    grads = dict(zip(names, torch.autograd.grad(y, [v[key] for key in names], dy)))
+    want, bound = ref.linear(**v, act=act, dy=dy), ref.linear(**v, act=act, dy=dy, absolute=True)
+    ref.close(y, want["y"], bound["y"], k + 10, "y")
+    half = ref.HALF_STEP[t]
+    dz_err = half * want["dz"].abs() + (0 if act == "none" else half * want["z"].abs() * dy.cpu().double().abs())
+    xa, wa = v["x"].detach().cpu().double().abs(), v["w"].detach().cpu().double().abs()
+    extra = {"x": dz_err @ wa, "w": dz_err.t() @ xa, "b": dz_err.sum(0) - half * want["dz"].abs().sum(0), "residual": 0}
+    for name in names:
+        r = dy.cpu().double() if name == "residual" else want["d" + name]
+        lim = r.abs() if name == "residual" else bound["d" + name]
+        e = torch.as_tensor(extra[name])
+        # (close()'s bound in units of 2^-24: the rounding of dz is added to it)
+        ref.close(grads[name], r, lim * (m + n + k + 20) + e * 2.0 ** 24, 1, "d" + name)
+
+
+def test_linear_views_leading_axes_and_unaligned_rows():
+    g = torch.Generator().manual_seed(77)
+    for t in (torch.bfloat16, torch.float32):
+        big, wide = _rnd(g, 4, 9, 2 * 72 + 1, dtype=t), _rnd(g, 50, 80, dtype=t)
+        w, b = wide[:, 5:77], _rnd(g, 50)
+        for x in (big[..., :72], big[..., 1:73], big[..., 73:], big[:, ::2, :72], big.transpose(0, 1)[..., :72],
+                  big[..., :144:2]):
+            res = _rnd(g, *x.shape[:-1], 2 * 50, dtype=t)[..., 50:]
+            got = ops.linear(x, w, b, "silu", residual=res)
+            assert torch.equal(got, ops.linear(x.contiguous(), w.contiguous(), b, "silu", residual=res.contiguous()))
+            assert got.shape == (*x.shape[:-1], 50)
+        one = ops.linear(big[0, 0, :72], w, b)
+        assert one.shape == (50,) and torch.equal(one, ops.linear(big[:1, 0, :72], w, b)[0])
+        x = big[..., :72].detach().requires_grad_(True)
+        y = ops.linear(x, w, b, "gelu")
+        (dx,) = torch.autograd.grad(y.float().sum(), [x])  # an expanded gradient
+        (dx2,) = torch.autograd.grad(ops.linear(x, w, b, "gelu"), [x], torch.ones_like(y))
+        assert torch.equal(dx, dx2)
+    empty = torch.zeros(0, 72, device="cuda", requires_grad=True)
+    w = torch.randn(5, 72, device="cuda", requires_grad=True)
+    y = ops.linear(empty, w, torch.zeros(5, device="cuda"), "silu")
+    dx, dw = torch.autograd.grad(y.sum(), [empty, w])
+    assert y.shape == (0, 5) and dx.shape == (0, 72) and not dw.any()
+
+
+def test_linear_rows_do_not_leak_into_each_other():
+    """A row of NaN or inf in x spoils its own row of y alone, and what lies behind a view's rows is never read."""
+    g = torch.Generator().manual_seed(78)
+    for t, k in ((torch.bfloat16, 100), (torch.float32, 66), (torch.float16, 128)):
+        x, w = _rnd(g, 150, k, dtype=t), _rnd(g, 140, k, dtype=t)
+        clean = ops.linear(x, w)
+        dirty = x.clone()
+        dirty[70], dirty[71] = float("nan"), float("inf")
+        y = ops.linear(dirty, w)
+        keep = [i for i in range(150) if i not in (70, 71)]
+        assert torch.equal(y[keep], clean[keep]) and bool(torch.isnan(y[70]).all())
+        wide = torch.full((150, k + 24), float("nan"), dtype=t, device="cuda")
+        wide[:, :k] = x
+        assert torch.equal(ops.linear(wide[:, :k], w), clean)
+        # a column of w's gradient sums over rows: a zero gradient times an infinite input is not zero, as ever
+        v = x.clone().requires_grad_(True)
+        dy = torch.zeros_like(clean)
+        dy[3] = 1
+        (dx,) = torch.autograd.grad(ops.linear(v, w), [v], dy)
+        assert not dx[:3].any() and not dx[4:].any() and dx[3].any()
+
+
+def test_linear_extremes_of_fp16_keep_their_slopes():
+    x = torch.tensor([[300.0], [-300.0], [2.0 ** -20], [-2.0 ** -20]], device="cuda", dtype=torch.float16, requires_grad=True)
+    w = torch.tensor([[300.0], [2.0 ** -20]], device="cuda", dtype=torch.float16)
+    for act in ("relu", "silu", "gelu"):
+        y = ops.linear(x, w, None, act)
+        (dx,) = torch.autograd.grad(y, [x], torch.ones_like(y))
+        assert bool(torch.isfinite(dx).all()), act
+        if act == "relu":  # 90000 and 2^-40 are positive, their negatives are not
+            want = torch.tensor([[300.0], [0.0], [300.0], [0.0]], device="cuda").half()
+            assert torch.equal(dx, want)
+    for act, want in (("relu", 0.0), ("none", float("-inf"))):
+        z = ops.linear(torch.full((1, 1), float("-inf"), device="cuda"), torch.ones(1, 1, device="cuda"), None, act)
+        assert float(z) == want
+
+
+def test_linear_same_bits_every_time_and_in_a_graph():
+    g = torch.Generator().manual_seed(79)
+    x, w, b = (_rnd(g, *s, dtype=torch.bfloat16).requires_grad_(True) for s in ((70, 2048), (96, 2048), (96,)))
+    dy = _rnd(g, 70, 96, dtype=torch.bfloat16)
+
+    def run():
+        y = ops.linear(x, w, b, "gelu")
+        return [y.detach(), *torch.autograd.grad(y, [x, w, b], dy)]
+
+    first = [t.clone() for t in run()]
+    assert all(torch.equal(a, c) for a, c in zip(first, run()))
+    graph, outs = _capture(run)
+    for turn in range(3):
+        with torch.no_grad():
+            x.mul_(0.5)
+        want = [t.clone() for t in run()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(outs, want)), turn
+
+
+def test_linear_past_32_bits():
+    """Rows behind 2^31 elements of x and of y equal a shorter call's (of enough rows that its k axis is not split either:
+    a split sums in another order)."""
+    m, k, n = 2200000, 1000, 1000
+    x = torch.empty(m, k, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    w = _rnd(torch.Generator().manual_seed(2), n, k, scale=0.03, dtype=torch.bfloat16)
+    y = ops.linear(x, w, None, "silu")
+    assert torch.equal(y[-40000:], ops.linear(x[-40000:], w, None, "silu"))
+    assert torch.equal(y[:40001], ops.linear(x[:40001], w, None, "silu"))

@@ -231,3 +231,54 @@ def test_reference_scan_gradients_are_the_differences():
         assert (got["d" + name] - diff).abs().max() < 1e-7, name
         diff = _differences(lambda: ref.scan(**t, softplus=True, lengths=lengths)["state"], t[name], ds)
         assert (late["d" + name] - diff).abs().max() < 1e-7, name
+
+
+@pytest.mark.parametrize("kw, err", [
+    (dict(x=torch.zeros(3, 5)), ValueError),
+    (dict(x=torch.tensor(1.0)), ValueError),
+    (dict(x=torch.zeros(3, 4, dtype=torch.float64)), TypeError),
+    (dict(x=None), TypeError),
+    (dict(w=torch.zeros(6, 4, dtype=torch.bfloat16)), TypeError),
+    (dict(w=torch.zeros(4)), ValueError),
+    (dict(w=torch.zeros(0, 4)), ValueError),
+    (dict(x=torch.zeros(3, 0), w=torch.zeros(6, 0)), ValueError),
+    (dict(b=torch.zeros(5)), ValueError),
+    (dict(b=torch.zeros(6, dtype=torch.float16)), TypeError),
+    (dict(residual=torch.zeros(2, 6)), ValueError),
+    (dict(residual=torch.zeros(3, 6, dtype=torch.float16)), TypeError),
+    (dict(activation="tanh"), ValueError),
+    (dict(), RuntimeError),
+])
+def test_linear_refuses(kw, err):
+    args = dict(x=torch.zeros(3, 4), w=torch.zeros(6, 4))
+    args.update(kw)
+    with pytest.raises(err):
+        ops.linear(**args)
+
+
+@pytest.mark.parametrize("act", ["none", "silu", "gelu"])
+def test_reference_linear_gradients_are_the_differences(act):
+    import sequence_ref as ref
+
+    g = torch.Generator().manual_seed(3)
+    t = dict(x=torch.randn(4, 3, generator=g).double(), w=torch.randn(5, 3, generator=g).double(),
+             b=torch.randn(5, generator=g).double())
+    dy = torch.randn(4, 5, generator=g).double()
+    got = ref.linear(**t, act=act, dy=dy)
+    for name in t:
+        diff = _differences(lambda: ref.linear(**t, act=act)["y"], t[name], dy)
+        assert (got["d" + name] - diff).abs().max() < 1e-7, name
+
+
+def test_linear_c_entries_refuse():
+    import ctypes
+
+    lib = _native.load()
+    one = ctypes.c_void_p(16)
+    assert lib.afd_linear_workspace_bytes(0, 4, 4, 0) == 0 and lib.afd_linear_workspace_bytes(4, 4, 4, 9) == 0
+    assert lib.afd_linear_forward(one, 4, one, 4, None, 0, None, 0, one, None, 4, 4, 4, 7, 0, None, 0, None) == -1
+    assert lib.afd_linear_forward(one, 4, one, 4, None, 0, None, 0, one, None, 4, 1 << 20, 4, 0, 0, None, 0, None) == -3
+    assert lib.afd_linear_forward(one, 3, one, 3, None, 0, None, 0, one, None, 4, 4, 3, 0, 0, None, 0, None) == -4
+    assert lib.afd_linear_backward(one, 4, one, 4, None, one, 4, one, one, None, 0, 4, 4, 4, 2, 0, None, 0, None) == -1
+    assert lib.afd_linear_backward(one, 4, one, 4, one, one, 4, one, one, None, 0, 4, 4, 4, 2, 0, None, 0, None) == -4
+    assert lib.afd_linear_backward(one, 4, one, 4, None, one, 4, one, one, None, 0, 9000000, 4, 4, 0, 0, one, 0, None) == -3
