@@ -25,20 +25,33 @@ constexpr int kSlab = 128;  // bytes of k per row and slab
 
 enum Act { kNone, kRelu, kSilu, kGelu };
 
-__device__ __forceinline__ float activate(float z, int act) {
+// The normal distribution's Phi.  fp32: the library's erf.  16-bit results: erf after Abramowitz and Stegun 7.1.26, off by at
+// most 1.5e-7, a fifth of the instructions and no branch (the library's took 50 us of a 16384 x 2048 forward's epilogue).
+template <typename T> __device__ __forceinline__ float phi(float z) {
+    if constexpr (sizeof(T) == 4) return 0.5f * (1.f + erff(z * 0.70710678118654752f));
+    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    float p = 1.061405429f;
+    p = fmaf(p, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float tail = 0.5f * p * t * __builtin_amdgcn_exp2f(-kLog2e * x * x);  // 1 - Phi(|z|)
+    return z < 0.f ? tail : 1.f - tail;
+}
+
+template <typename T> __device__ __forceinline__ float activate(float z, int act) {
     if (act == kRelu) return z < 0.f ? 0.f : z;  // (NaN stays)
     if (act == kSilu) return z * sigmoid_f32(z);
-    if (act == kGelu) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    if (act == kGelu) return z * phi<T>(z);
     return z;
 }
-__device__ __forceinline__ float activate_slope(float z, int act) {
+template <typename T> __device__ __forceinline__ float activate_slope(float z, int act) {
     if (act == kRelu) return z > 0.f ? 1.f : 0.f;
     if (act == kSilu) {
         const float s = sigmoid_f32(z);
         return s * (1.f + z * (1.f - s));
     }
-    if (act == kGelu)
-        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * z * z);
+    if (act == kGelu) return phi<T>(z) + z * 0.39894228040143268f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * z * z);
     return 1.f;
 }
 
@@ -92,7 +105,7 @@ __device__ __forceinline__ void finish(const Epi& e, int m, int n, int N, float 
             for (int i = 0; i < W; ++i) {
                 const float z = v[g + i] + bias[g + i];
                 if (zp) zk.v[i] = keep_z<T>(z);
-                o[i] = activate(z, e.act);
+                o[i] = activate<T>(z, e.act);
                 if (res) o[i] += r[i];
             }
             if (zp) *reinterpret_cast<u32x4_any*>(zp + g) = __builtin_bit_cast(u32x4, zk);
@@ -102,7 +115,7 @@ __device__ __forceinline__ void finish(const Epi& e, int m, int n, int N, float 
         for (int i = 0; i < V && n + i < N; ++i) {
             const float z = v[i] + bias[i];
             if (zp) zp[i] = keep_z<T>(z);
-            const float o = activate(z, e.act);
+            const float o = activate<T>(z, e.act);
             out[i] = from_f32<T>(res ? o + to_f32(res[i]) : o);
         }
     }
@@ -129,6 +142,10 @@ template <typename T> __device__ __forceinline__ void mma(const u32x4& a, const 
     }
 }
 
+// Where a chunk of 16 bytes sits in its 128-byte row: 16 lanes read one chunk number of 16 rows at a time, and two rows span
+// the 64 banks, so every other row has to turn to another place.
+__device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
+
 // Tile of this workgroup.  Workgroups go to the 8 XCDs in turn; each XCD takes a contiguous run of tiles, in groups of 8 tile
 // rows walked column by column, so the rows of A and B that its workgroups share stay in its L2.
 __device__ __forceinline__ void tile_of(const Gemm& g, int id, int& tm, int& tn) {
@@ -140,6 +157,8 @@ __device__ __forceinline__ void tile_of(const Gemm& g, int id, int& tm, int& tn)
     tm = grp * 8 + in % rows;
     tn = in / rows;
 }
+
+template <int N> struct Const { static constexpr int value = N; };
 
 template <typename T, int TM, int TN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(const Gemm g) {
@@ -166,13 +185,13 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(const Gemm g) {
     for (int e = 0; e < CA; ++e) {
         const int row = (e * kThreads + tid) >> 3;
         oa[e] = (unsigned)((size_t)min(row, g.M - 1 - m0) * g.lda * sizeof(T)) + chunk[e] * 16;
-        la[e] = row * kSlab + ((chunk[e] ^ (row & 7)) * 16);
+        la[e] = row * kSlab + ((chunk[e] ^ swizzle(row)) * 16);
     }
 #pragma unroll
     for (int e = 0; e < CB; ++e) {
         const int row = (e * kThreads + tid) >> 3;
         ob[e] = (unsigned)((size_t)min(row, g.N - 1 - n0) * g.ldb * sizeof(T)) + chunk[e] * 16;
-        lb[e] = TM * kSlab + row * kSlab + ((chunk[e] ^ (row & 7)) * 16);
+        lb[e] = TM * kSlab + row * kSlab + ((chunk[e] ^ swizzle(row)) * 16);
     }
     u32x4 ra[CA], rb[CB];
     auto fetch = [&](int k) {
@@ -207,34 +226,78 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(const Gemm g) {
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
     const int arow = wm * (TM / WM) + l31, brow = wn * (TN / WN) + l31;
-    if (kbeg < kend) {
+    // One slab: four steps of 32 bytes of k.  A step's fragments are read while the step before it is multiplied.  The next
+    // slab's registers, under way for a whole slab, go to LDS between the third step's products, the loads of the slab behind
+    // it start, and the barrier is passed in front of the last step, whose products cover the next slab's first reads.
+    u32x4 fa[2][MI], fb[2][NI];
+    auto read = [&](int buf, int st, int to) {
+        const char* base = lds + buf * kBuf;
+        const int c = ((2 * st + half) ^ swizzle(l31)) * 16;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[to][i] = *reinterpret_cast<const u32x4*>(base + (arow + i * 32) * kSlab + c);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) fb[to][j] = *reinterpret_cast<const u32x4*>(base + TM * kSlab + (brow + j * 32) * kSlab + c);
+    };
+    auto multiply = [&](int from) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) mma<T>(fa[from][i], fb[from][j], acc[i][j]);
+    };
+    // reads, writes and products of a step take turns
+    constexpr int kMma = MI * NI * (sizeof(T) == 4 ? 4 : 1);
+    auto weave = [&](auto writes) {
+        constexpr int kReads = MI + NI, kWrites = decltype(writes)::value, kAll = kReads + kWrites;
+        constexpr int kEach = kMma / kAll > 0 ? kMma / kAll : 1;
+#pragma unroll
+        for (int i = 0; i < kReads; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kWrites; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+        }
+    };
+    constexpr Const<0> none;
+    constexpr Const<CA + CB> all;
+    const int slabs = (kend - kbeg + KS - 1) / KS;
+    if (slabs > 0) {
         fetch(kbeg);
         put(0);
+        if (slabs > 1) fetch(kbeg + KS);
     }
     __syncthreads();
+    read(0, 0, 0);
     int buf = 0;
-    for (int k = kbeg; k < kend; k += KS, buf ^= 1) {
-        const bool more = k + KS < kend;
-        if (more) fetch(k + KS);
-        const char* base = lds + buf * kBuf;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            u32x4 fa[MI], fb[NI];
-            const int c = 2 * s + half;
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-                fa[i] = *reinterpret_cast<const u32x4*>(base + (arow + i * 32) * kSlab + ((c ^ (l31 & 7)) * 16));
-#pragma unroll
-            for (int j = 0; j < NI; ++j)
-                fb[j] = *reinterpret_cast<const u32x4*>(base + TM * kSlab + (brow + j * 32) * kSlab + ((c ^ (l31 & 7)) * 16));
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NI; ++j) mma<T>(fa[i], fb[j], acc[i][j]);
-        }
-        if (more) put(buf ^ 1);
+    for (int i = 1; i < slabs; ++i, buf ^= 1) {
+        read(buf, 1, 1);
+        multiply(0);
+        weave(none);
+        read(buf, 2, 0);
+        multiply(1);
+        weave(none);
+        read(buf, 3, 1);
+        put(buf ^ 1);
+        multiply(0);
+        weave(all);
+        if (i + 1 < slabs) fetch(kbeg + (i + 1) * KS);
         __syncthreads();
+        read(buf ^ 1, 0, 0);
+        multiply(1);
+        weave(none);
     }
+    read(buf, 1, 1);
+    multiply(0);
+    weave(none);
+    read(buf, 2, 0);
+    multiply(1);
+    weave(none);
+    read(buf, 3, 1);
+    multiply(0);
+    multiply(1);
+    __syncthreads();
 
     // Epilogue, wave by wave through LDS (nobody reads the slabs any more): 32 rows of the wave's columns at a time, then
     // 8 columns per lane in row order.
@@ -286,6 +349,7 @@ template <typename T> __global__ void __launch_bounds__(256) join_kernel(const G
         load_bias<T, 8>(g.e, n, g.N, bias);
 #pragma unroll
         for (int c = 0; c < 8; ++c) v[c] = 0.f;
+#pragma unroll 8
         for (int s = 0; s < g.S; ++s) {
             const float* src = g.part + ((size_t)s * g.M + m) * g.ldp + n;
             const f32x4 lo = *reinterpret_cast<const f32x4*>(src), hi = *reinterpret_cast<const f32x4*>(src + 4);
@@ -299,23 +363,50 @@ template <typename T> __global__ void __launch_bounds__(256) join_kernel(const G
     }
 }
 
-// dst[c][r] = src[r][c] for R x C elements, rows of dst padded with zeros to ldd (a multiple of 16 bytes).  64 x 64 tiles
-// through LDS.
-template <typename T>
-__global__ void __launch_bounds__(256) turn_kernel(const T* __restrict__ src, long lds_, int R, int C, T* __restrict__ dst, long ldd) {
-    __shared__ T t[64][64 + 4 / sizeof(T)];
-    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
-    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+// 64 x 64 tiles of the two transposing passes: a thread reads 8 columns of rows y and y + 32, and writes 8 rows of columns y
+// and y + 32 (x8 its first column or row); 16-byte accesses inside the matrix, single elements at its edges.
+template <typename T> __device__ __forceinline__ void load8(const T* p, int left, float (&v)[8]) {
+    constexpr int W = 16 / (int)sizeof(T);
+    if (left >= 8) {
 #pragma unroll
-    for (int i = 0; i < 64; i += 4) {
-        const int r = r0 + i + y, c = c0 + x;
-        t[i + y][x] = r < R && c < C ? src[(size_t)r * lds_ + c] : (T)0.f;
+        for (int g = 0; g < 8; g += W) load_row<T, W>(p + g, *reinterpret_cast<float(*)[W]>(&v[g]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, int left, const float (&v)[8]) {
+    constexpr int W = 16 / (int)sizeof(T);
+    if (left >= 8) {
+#pragma unroll
+        for (int g = 0; g < 8; g += W) store_row<T, W>(p + g, *reinterpret_cast<const float(*)[W]>(&v[g]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left) p[i] = from_f32<T>(v[i]);
+    }
+}
+
+// dst[c][r] = src[r][c] for R x C elements, rows of dst padded with zeros to ldd (a multiple of 16 bytes).
+template <typename T>
+__global__ void __launch_bounds__(256) turn_kernel(const T* __restrict__ src, long ld, int R, int C, T* __restrict__ dst, long ldd) {
+    __shared__ float t[64][65];
+    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+    const int x8 = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
+#pragma unroll
+    for (int i = y; i < 64; i += 32) {
+        float v[8];
+        load8<T>(src + (size_t)min(r0 + i, R - 1) * ld + c0 + x8, r0 + i < R ? C - c0 - x8 : 0, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[i][x8 + k] = v[k];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 64; i += 4) {
-        const int c = c0 + i + y, r = r0 + x;
-        if (c < C && r < ldd) dst[(size_t)c * ldd + r] = t[x][i + y];
+    for (int i = y; i < 64; i += 32) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = t[x8 + k][i];
+        if (c0 + i < C) store8<T>(dst + (size_t)(c0 + i) * ldd + r0 + x8, (int)min(ldd - r0 - x8, 8L), v);
     }
 }
 
@@ -337,54 +428,79 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ dy, long 
                                                  float* __restrict__ sums) {
     __shared__ float t[64][65];
     const int m0 = blockIdx.x * 64, n0 = blockIdx.y * 64;
-    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    float s = 0.f;
+    const int x8 = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
 #pragma unroll
-    for (int i = 0; i < 64; i += 4) {
-        const int m = m0 + i + y, n = n0 + x;
-        float v = 0.f;
-        if (m < M && n < N) {
-            v = to_f32(dy[(size_t)m * ldy + n]);
-            if (act != kNone) v *= activate_slope(to_f32(z[(size_t)m * N + n]), act);
+    for (int i = y; i < 64; i += 32) {
+        const int m = m0 + i, n = n0 + x8, left = m < M ? N - n : 0;
+        float v[8], zv[8];
+        load8<T>(dy + (size_t)min(m, M - 1) * ldy + n, left, v);
+        if (act != kNone) {
+            load8<T>(z + (size_t)min(m, M - 1) * N + n, left, zv);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = k < left ? v[k] * activate_slope<T>(zv[k], act) : 0.f;
         }
-        s += v;
-        t[i + y][x] = v;
-        if (dz && m < M && n < ldz) dz[(size_t)m * ldz + n] = from_f32<T>(v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[i][x8 + k] = v[k];
+        if (dz && m < M) store8<T>(dz + (size_t)m * ldz + n, (int)min(ldz - n, 8L), v);
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 64; i += 4) {
-        const int n = n0 + i + y, m = m0 + x;
-        if (n < N && m < ldt) turned[(size_t)n * ldt + m] = from_f32<T>(t[x][i + y]);
+    for (int i = y; i < 64; i += 32) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = t[x8 + k][i];
+        if (n0 + i < N) store8<T>(turned + (size_t)(n0 + i) * ldt + m0 + x8, (int)min(ldt - m0 - x8, 8L), v);
     }
     if (!sums) return;
     __shared__ float red[4][64];
-    red[y][x] = s;
+    const int col = threadIdx.x & 63, part = threadIdx.x >> 6;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += t[part * 16 + i][col];
+    red[part][col] = s;
     __syncthreads();
-    if (y == 0 && n0 + x < N) sums[(size_t)blockIdx.x * N + n0 + x] = (red[0][x] + red[1][x]) + (red[2][x] + red[3][x]);
+    if (part == 0 && n0 + col < N)
+        sums[(size_t)blockIdx.x * N + n0 + col] = (red[0][col] + red[1][col]) + (red[2][col] + red[3][col]);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 long pad_to(long n, long k) { return (n + k - 1) / k * k; }
 
+// Tiles by what they took (us) for the three products of a training step, forward / dx / dw:
+//   fp32 12928 x 512 x 1024: 128 x 128 166 / 152 / 129, 64 x 64 148 / 150 / 138, 128 x 64 144 / 139 / 132 (three workgroups
+//   per CU, and 1616 tiles where 808 leave a fifth of the card idle at the end; matrix instructions are busy 60 % of it);
+//   bf16 16384 x 2048 x 2048: 256 x 256 220 / 171 / 162, 128 x 128 263 / 211 / 186 (half the operand traffic per product).
+// Up to 32 rows there is one tile row of 32 and the weights are what is read.
 struct Shape {
-    int kind;  // 0: 32 x 128, 1: 128 x 128 tiles
+    int kind;
     int tm, tn, S, ksplit;
     size_t part;
 };
+enum { kTile32x128, kTile128x64, kTile128, kTile256 };
 Shape gemm_shape(int M, int N, int K, int dtype) {
     Shape s;
-    const int ks = kSlab / (int)dtype_bytes(dtype);
-    s.kind = M <= 32 ? 0 : 1;
-    s.tm = ceil_div(M, s.kind ? 128 : 32);
-    s.tn = ceil_div(N, 128);
+    const int slabs = ceil_div(K, kSlab / (int)dtype_bytes(dtype));
+    int rows = 128, cols = 128, fill = 512;  // fill: workgroups that keep the card busy
+    s.kind = kTile128;
+    if (M <= 32) {
+        s.kind = kTile32x128;
+        rows = 32;
+    } else if (dtype == AFD_T_F32) {
+        s.kind = kTile128x64;
+        cols = 64;
+        fill = 768;
+    } else if ((long)ceil_div(M, 256) * ceil_div(N, 256) * slabs >= 256 * 16) {  // 16 slabs for every CU
+        s.kind = kTile256;
+        rows = cols = fill = 256;
+    }
+    s.tm = ceil_div(M, rows);
+    s.tn = ceil_div(N, cols);
     const long tiles = (long)s.tm * s.tn;
-    const int slabs = ceil_div(K, ks);
     int want = 1;
-    if (tiles < 256) {
-        want = (int)((512 + tiles - 1) / tiles);
-        const int most = slabs / (s.kind ? 4 : 2);
+    if (tiles < fill) {
+        want = (int)((fill + tiles - 1) / tiles);
+        const int most = slabs / (s.kind == kTile32x128 ? 2 : 4);
         if (want > most) want = most;
         if (want < 1) want = 1;
     }
@@ -394,15 +510,29 @@ Shape gemm_shape(int M, int N, int K, int dtype) {
     return s;
 }
 
-template <typename T, int TM, int TN, int WM, int WN> void launch_tile(const Gemm& g, hipStream_t s) {
+template <typename T, int TM, int TN, int WM, int WN> int launch_tile(const Gemm& g, hipStream_t s) {
     constexpr int kBuf = 2 * (TM + TN) * kSlab, kEpi = WM * WN * 32 * (TN / WN + 4) * 4;
     constexpr unsigned lds = kBuf > kEpi ? kBuf : kEpi;
+    if constexpr (lds > 64 * 1024) {
+        static PerDeviceOnce once;
+        if (!once.done()) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<T, TM, TN, WM, WN>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess) return fail(AFD_ERR_HIP, "linear: %s", hipGetErrorString(e));
+            once.mark();
+        }
+    }
     hipLaunchKernelGGL((gemm_kernel<T, TM, TN, WM, WN>), dim3((unsigned)(g.tm * g.tn), (unsigned)g.S), dim3(64 * WM * WN), lds, s, g);
+    return AFD_OK;
 }
 
 template <typename T> int gemm_t(const Gemm& g, int kind, hipStream_t s) {
-    if (kind == 0) launch_tile<T, 32, 128, 1, 4>(g, s);
-    else launch_tile<T, 128, 128, 2, 2>(g, s);
+    int rc;
+    if (kind == kTile32x128) rc = launch_tile<T, 32, 128, 1, 4>(g, s);
+    else if constexpr (sizeof(T) == 4) rc = launch_tile<T, 128, 64, 2, 2>(g, s);
+    else if (kind == kTile256) rc = launch_tile<T, 256, 256, 2, 4>(g, s);
+    else rc = launch_tile<T, 128, 128, 2, 2>(g, s);
+    if (rc) return rc;
     if (g.S > 1) {
         const long all = (long)g.M * (g.ldp / 8), grid = (all + 255) / 256;
         hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0, s, g);

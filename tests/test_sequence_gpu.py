@@ -715,6 +715,9 @@ LINEAR = [
     ("fp16", 140, 513, 250, "relu", "fp32", True),
     ("fp16", 64, 72, 1000, "silu", None, False),
     ("fp16", 1000, 16, 16, "none", "same", False),
+    ("bf16", 2050, 1024, 1030, "silu", "fp32", True),  # 256 x 256 tiles, ragged in both directions
+    ("fp16", 4100, 520, 2056, "gelu", "fp32", False),
+    ("fp32", 2000, 260, 130, "gelu", "fp32", True),
 ]
 
 
