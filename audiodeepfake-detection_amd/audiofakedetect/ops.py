@@ -1850,7 +1850,7 @@ def _linear_forward(x, w, b, residual, act, keep=False):
     m, k = x.shape
     n = w.shape[0]
     y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    z = torch.empty((m, n), dtype=x.dtype, device=x.device) if keep and act else None
+    z = torch.empty((m, n), dtype=torch.float32, device=x.device) if keep and act else None
     if m > 0:
         dtype = _SEQ_DTYPES[x.dtype]
         with _OnDevice(x) as stream:
@@ -1904,8 +1904,8 @@ def linear(x, w, b=None, activation: str = "none", residual=None):
     """act(x @ w.T + b) + residual in one pass: x [..., K], w [N, K] and residual [..., N] of one type (float32 / bfloat16 /
     float16), b [N] float32 or of that type; `activation` "none", "relu", "silu" or "gelu" (with the error function).  float32
     products are exact, all sums are float32, the result is rounded once.  Differentiable in every tensor; the backward
-    takes the activation's slope at x @ w.T + b rounded to the type of x, and rounds the gradient in front of its two
-    products to it."""
+    keeps x @ w.T + b in float32 for the activation's slope, and rounds the gradient to the type of x in front of its two
+    products (not for b's)."""
     what = "linear"
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what}: x is a {type(x).__name__}, not a tensor")

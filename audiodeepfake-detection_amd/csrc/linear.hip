@@ -62,7 +62,7 @@ struct Epi {
     long ldr;
     void* out;  // rows of ldo elements
     long ldo;
-    void* z;  // pre-activation, rows of N elements, NULL: not kept
+    float* z;  // pre-activation, rows of N elements, NULL: not kept
     int act;
 };
 
@@ -77,44 +77,35 @@ struct Gemm {
     int tm, tn;     // tiles
 };
 
-// The pre-activation is kept in the type of the tensors.  A value that rounds to zero there would lose the side of relu's
-// corner it is on, one beyond fp16's range would become inf and give NaN as inf times the 0 of a slope: both stay
-// just inside.
-template <typename T> __device__ __forceinline__ T keep_z(float z) {
-    if constexpr (sizeof(T) == 2 && __is_same(T, f16_t)) {
-        if (fabsf(z) > 65504.f) return z > 0.f ? (T)65504.f : (z < 0.f ? (T)-65504.f : (T)z);
-        if (z != 0.f && fabsf(z) < 5.9604645e-8f) return z > 0.f ? (T)5.9604645e-8f : (T)-5.9604645e-8f;
-    }
-    return from_f32<T>(z);
-}
-
-// V consecutive columns n .. n + V of row m
+// V consecutive columns n .. n + V of row m.  The pre-activation is kept in fp32 whatever the tensors' type: the bias gradient
+// is a sum of dy times its slope and an fp32 parameter's; at a z rounded to bf16 it was off by 2e-3.
 template <typename T, int V>
 __device__ __forceinline__ void finish(const Epi& e, int m, int n, int N, float (&v)[V], const float (&bias)[V]) {
     T* out = static_cast<T*>(e.out) + (size_t)m * e.ldo + n;
     const T* res = e.residual ? static_cast<const T*>(e.residual) + (size_t)m * e.ldr + n : nullptr;
-    T* zp = e.z ? static_cast<T*>(e.z) + (size_t)m * N + n : nullptr;
+    float* zp = e.z ? e.z + (size_t)m * N + n : nullptr;
     constexpr int W = 16 / (int)sizeof(T);
     if (n + V <= N) {
 #pragma unroll
         for (int g = 0; g < V; g += W) {
             float r[W], o[W];
             if (res) load_row<T, W>(res + g, r);
-            Pack<T, W> zk;
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                const float z = v[g + i] + bias[g + i];
-                if (zp) zk.v[i] = keep_z<T>(z);
-                o[i] = activate<T>(z, e.act);
+                v[g + i] += bias[g + i];
+                o[i] = activate<T>(v[g + i], e.act);
                 if (res) o[i] += r[i];
             }
-            if (zp) *reinterpret_cast<u32x4_any*>(zp + g) = __builtin_bit_cast(u32x4, zk);
             store_row<T, W>(out + g, o);
+        }
+        if (zp) {
+#pragma unroll
+            for (int g = 0; g < V; g += 4) store_row<float, 4>(zp + g, *reinterpret_cast<float(*)[4]>(&v[g]));
         }
     } else {
         for (int i = 0; i < V && n + i < N; ++i) {
             const float z = v[i] + bias[i];
-            if (zp) zp[i] = keep_z<T>(z);
+            if (zp) zp[i] = z;
             const float o = activate<T>(z, e.act);
             out[i] = from_f32<T>(res ? o + to_f32(res[i]) : o);
         }
@@ -423,7 +414,7 @@ __global__ void __launch_bounds__(256) pad_kernel(const T* __restrict__ src, lon
 // dz = dy act'(z) as rows (ldz, zeros behind N; NULL: not wanted) and turned (ldt, zeros behind M), and its column sums over
 // the tile's rows.
 template <typename T>
-__global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ dy, long ldy, const T* __restrict__ z, int act, int M, int N,
+__global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ dy, long ldy, const float* __restrict__ z, int act, int M, int N,
                                                  T* __restrict__ dz, long ldz, T* __restrict__ turned, long ldt,
                                                  float* __restrict__ sums) {
     __shared__ float t[64][65];
@@ -435,7 +426,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ dy, long 
         float v[8], zv[8];
         load8<T>(dy + (size_t)min(m, M - 1) * ldy + n, left, v);
         if (act != kNone) {
-            load8<T>(z + (size_t)min(m, M - 1) * N + n, left, zv);
+            load8<float>(z + (size_t)min(m, M - 1) * N + n, left, zv);
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = k < left ? v[k] * activate_slope<T>(zv[k], act) : 0.f;
         }
@@ -605,7 +596,7 @@ extern "C" size_t afd_linear_workspace_bytes(long long M, int N, int K, int dtyp
 }
 
 extern "C" int afd_linear_forward(const void* x, long long ldx, const void* w, long long ldw, const void* bias, int bias_f32,
-                                  const void* residual, long long ldr, void* y, void* z, long long M, int N, int K, int act,
+                                  const void* residual, long long ldr, void* y, float* z, long long M, int N, int K, int act,
                                   int dtype, void* ws, size_t ws_bytes, afd_stream_t stream) {
     if (!x || !w || !y) return fail(AFD_ERR_ARG, "linear: missing tensor");
     if (int rc = check("linear", M, N, K, act, dtype)) return rc;
@@ -656,11 +647,11 @@ BackPlan back_plan(long M, int N, int K, int dtype) {
     return b;
 }
 template <typename T>
-int dz_t(const void* dy, long ldy, const void* z, int act, int M, int N, void* dz, long ldz, void* t, long ldt, float* sums, hipStream_t s) {
+int dz_t(const void* dy, long ldy, const float* z, int act, int M, int N, void* dz, long ldz, void* t, long ldt, float* sums, hipStream_t s) {
     const long rows = ldt > M ? ldt : M;
     const long cols = dz && ldz > N ? ldz : N;
     hipLaunchKernelGGL(dz_kernel<T>, dim3((unsigned)ceil_div(rows, 64), (unsigned)ceil_div(cols, 64)), dim3(256), 0, s,
-                       static_cast<const T*>(dy), ldy, static_cast<const T*>(z), act, M, N, static_cast<T*>(dz), ldz,
+                       static_cast<const T*>(dy), ldy, z, act, M, N, static_cast<T*>(dz), ldz,
                        static_cast<T*>(t), ldt, sums);
     return check_launch("dz_kernel");
 }
@@ -671,7 +662,7 @@ extern "C" size_t afd_linear_backward_workspace_bytes(long long M, int N, int K,
     return back_plan(M, N, K, dtype).total;
 }
 
-extern "C" int afd_linear_backward(const void* x, long long ldx, const void* w, long long ldw, const void* z, const void* dy,
+extern "C" int afd_linear_backward(const void* x, long long ldx, const void* w, long long ldw, const float* z, const void* dy,
                                    long long ldy, void* dx, void* dw, void* dbias, int bias_f32, long long M, int N, int K,
                                    int act, int dtype, void* ws, size_t ws_bytes, afd_stream_t stream) {
     if (!x || !w || !dy || (act != kNone && !z)) return fail(AFD_ERR_ARG, "linear backward: missing tensor");

@@ -658,18 +658,18 @@ int afd_state_scan_step(const void* x, const void* dt, const void* b, const void
                         const long long* strides, const float* a, const float* d, const float* dt_bias, const float* state,
                         void* y, float* state_out, int B, int D, int N, int softplus, int dtype, afd_stream_t stream);
 
-/* y [M][N] = act(x [M][K] . w [N][K]^T + bias [N]) + residual [M][N] on the matrix cores; x, w, residual, y, z of type dtype
+/* y [M][N] = act(x [M][K] . w [N][K]^T + bias [N]) + residual [M][N] on the matrix cores; x, w, residual, y of type dtype
  * (fp32: exact products; bf16 / fp16: fp32 sums), row strides ldx, ldw, ldr in elements, y and z dense.  bias fp32 when
  * bias_f32 != 0, else of type dtype; bias, residual, z may be NULL.  act: 0 none, 1 relu, 2 z sigmoid(z), 3 z Phi(z).  z
- * receives x . w^T + bias, rounded to dtype, for the backward (not needed for act 0).
+ * (fp32) receives x . w^T + bias for the backward (not needed for act 0).
  * Backward: from dy [M][N] (row stride ldy), dx = dz . w, dw = dz^T . x, dbias = sums of dz, with dz = dy act'(z) (rounded to
- * dtype in front of the two products); dx, dw, dbias may be NULL where not wanted.  The residual's gradient is dy. */
+ * dtype in front of the two products, not for dbias); dx, dw, dbias may be NULL where not wanted.  The residual's gradient is dy. */
 size_t afd_linear_workspace_bytes(long long M, int N, int K, int dtype);
 int afd_linear_forward(const void* x, long long ldx, const void* w, long long ldw, const void* bias, int bias_f32,
-                       const void* residual, long long ldr, void* y, void* z, long long M, int N, int K, int act, int dtype,
+                       const void* residual, long long ldr, void* y, float* z, long long M, int N, int K, int act, int dtype,
                        void* ws, size_t ws_bytes, afd_stream_t stream);
 size_t afd_linear_backward_workspace_bytes(long long M, int N, int K, int dtype);
-int afd_linear_backward(const void* x, long long ldx, const void* w, long long ldw, const void* z, const void* dy,
+int afd_linear_backward(const void* x, long long ldx, const void* w, long long ldw, const float* z, const void* dy,
                         long long ldy, void* dx, void* dw, void* dbias, int bias_f32, long long M, int N, int K, int act,
                         int dtype, void* ws, size_t ws_bytes, afd_stream_t stream);
 
