@@ -852,3 +852,147 @@ def test_linear_past_32_bits():
     y = ops.linear(x, w, None, "silu")
     assert torch.equal(y[-40000:], ops.linear(x[-40000:], w, None, "silu"))
     assert torch.equal(y[:40001], ops.linear(x[:40001], w, None, "silu"))
+
+
+def _silu64(v):
+    return v * torch.sigmoid(v)
+
+
+def _layer64(x, p, rank, n):
+    """The layer of the next test in float64 torch operations, for autograd on the CPU."""
+    b, l, _ = x.shape
+    d = p["conv"].shape[0]
+    z = x @ p["w_in"].t() + p["b_in"]
+    u, gate = z[..., :d], z[..., d:]
+    taps = p["conv"].shape[1]
+    full = torch.cat([torch.zeros(b, taps - 1, d, dtype=x.dtype), u], 1)
+    h = _silu64(sum(full[:, j:j + l] * p["conv"][:, j] for j in range(taps)) + p["conv_b"])
+    s = h @ p["w_x"].t()
+    dt, bb, cc = s[..., :rank] @ p["w_dt"].t(), s[..., rank:rank + n], s[..., rank + n:]
+    delta = torch.nn.functional.softplus(dt + p["dt_bias"])
+    state, rows = torch.zeros(b, d, n, dtype=x.dtype), []
+    for t in range(l):
+        state = torch.exp(delta[:, t, :, None] * p["a"]) * state + (delta[:, t] * h[:, t])[:, :, None] * bb[:, t, None, :]
+        rows.append((state * cc[:, t, None, :]).sum(-1))
+    y = (torch.stack(rows, 1) + p["d"] * h) * _silu64(gate)
+    return y @ p["w_out"].t() + p["b_out"] + x
+
+
+def test_a_whole_state_space_layer_trains():
+    """Projection in -> convolution -> projections to the scan's inputs -> scan with gate -> projection out onto the residual,
+    as views of each other's results, with its loss, all gradients, and the clipped step."""
+    b, l, k, d, n, rank = 3, 29, 24, 40, 16, 4
+    g = torch.Generator().manual_seed(90)
+    shapes = dict(w_in=(2 * d, k), b_in=(2 * d,), conv=(d, 4), conv_b=(d,), w_x=(rank + 2 * n, d), w_dt=(d, rank), a=(d, n),
+                  d=(d,), dt_bias=(d,), w_out=(k, d), b_out=(k,))
+    p = {name: torch.nn.Parameter(_rnd(g, *s, scale=0.3)) for name, s in shapes.items()}
+    with torch.no_grad():
+        p["a"].copy_(-torch.arange(1, n + 1, device="cuda").float().expand(d, n))
+        p["dt_bias"].sub_(2)
+    x = _rnd(g, b, l, k).requires_grad_(True)
+    wl, labels = _rnd(g, 2, k, scale=0.3), torch.tensor([0, 1, 1], device="cuda")
+    opt = ops.FusedAdam(p.values(), lr=1e-2)
+    opt.zero_grad()
+    z = ops.linear(x, p["w_in"], p["b_in"])
+    u, gate = z[..., :d], z[..., d:]
+    h = ops.causal_conv(u, p["conv"], p["conv_b"], "silu")
+    s = ops.linear(h, p["w_x"])
+    dt = ops.linear(s[..., :rank], p["w_dt"])
+    y = ops.state_scan(h, dt, p["a"], s[..., rank:rank + n], s[..., rank + n:], d=p["d"], gate=gate, dt_bias=p["dt_bias"],
+                       softplus=True)
+    out = ops.linear(y, p["w_out"], p["b_out"], residual=x)
+    loss = ops.CrossEntropyLoss()(ops.linear_mean(out, wl, torch.zeros(2, device="cuda")), labels)
+    loss.backward()
+    got = {name: q.grad.detach().clone() for name, q in p.items()}
+    got["x"] = x.grad.clone()
+    q = {name: v.detach().cpu().double().requires_grad_(True) for name, v in p.items()}
+    x64 = x.detach().cpu().double().requires_grad_(True)
+    out64 = _layer64(x64, q, rank, n)
+    loss64 = torch.nn.functional.cross_entropy((out64 @ wl.cpu().double().t()).mean(1), labels.cpu())
+    loss64.backward()
+    # a chain of half a dozen operators of at most a few hundred roundings each, forward and back: 4000 x 2^-24 of the
+    # largest value
+    tol = 4000 * 2.0 ** -24
+    assert float((out.detach().cpu().double() - out64.detach()).abs().max()) <= tol * float(out64.detach().abs().max())
+    for name, v in got.items():
+        want = (x64 if name == "x" else q[name]).grad
+        assert float((v.cpu().double() - want).abs().max()) <= tol * float(want.abs().max()), name
+    before = {name: v.detach().clone() for name, v in p.items()}
+    opt.step(max_grad_norm=0.05)
+    norm = float(torch.sqrt(sum(v.grad.square().sum() for v in q.values())))
+    assert abs(float(opt.last_grad_norm) - norm) <= tol * norm
+    assert all(not torch.equal(before[name], v) for name, v in p.items())
+
+
+def test_a_whole_layer_in_bf16_one_frame_at_a_time():
+    """The same layer's serving form: a prompt, then single frames through the step forms, against the whole sequence."""
+    b, l, k, d, n = 4, 20, 32, 64, 16
+    g = torch.Generator().manual_seed(91)
+    t = torch.bfloat16
+    w_in, w_x, w_out = _rnd(g, 2 * d, k, scale=0.2, dtype=t), _rnd(g, d + 2 * n, d, scale=0.2, dtype=t), _rnd(g, k, d, scale=0.2, dtype=t)
+    conv, conv_b = _rnd(g, d, 4, scale=0.4), _rnd(g, d, scale=0.1)
+    par = dict(a=-torch.rand(d, n, generator=g).cuda() * 4, d=_rnd(g, d), dt_bias=_rnd(g, d) - 2)
+    x = _rnd(g, b, l, k, dtype=t)
+
+    def layer(x, conv_f, scan_f):
+        z = ops.linear(x, w_in)
+        h = conv_f(z[..., :d])
+        s = ops.linear(h, w_x)
+        return ops.linear(scan_f(h, s, z[..., d:]), w_out, residual=x)
+
+    def scan_args(h, s, gate):
+        return dict(x=h, dt=s[..., :d], b=s[..., d:d + n], c=s[..., d + n:], gate=gate, softplus=True, **par)
+
+    with torch.no_grad():
+        whole = layer(x, lambda u: ops.causal_conv(u, conv, conv_b, "silu"), lambda *a: ops.state_scan(**scan_args(*a)))
+        states = {}
+
+        def conv_prompt(u):
+            y, states["c"] = ops.causal_conv(u, conv, conv_b, "silu", return_state=True)
+            return y
+
+        def scan_prompt(*a):
+            y, states["s"] = ops.state_scan(**scan_args(*a), return_state=True)
+            return y
+
+        layer(x[:, :11], conv_prompt, scan_prompt)
+        for i in range(11, l):
+            y = layer(x[:, i], lambda u: ops.causal_conv_step(u, states["c"], conv, conv_b, "silu"),
+                      lambda *a: ops.state_scan_step(state=states["s"], **scan_args(*a)))
+            # sums in other orders (the few rows' products split k): a bf16 step apart at most at each of four roundings
+            assert float((y.float() - whole[:, i].float()).abs().max()) <= 4 * 2.0 ** -7 * float(whole.float().abs().max())
+
+
+@pytest.mark.parametrize("kind", ["fused", "torch"])
+def test_trainer_clips_its_gradients(kind):
+    import os
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    import bench
+
+    torch.manual_seed(0)
+    args, trainer, _ = bench.build("sym5-l8", 4, False, torch.device("cuda", 0))
+    trainer.train_data_loader = None
+    params = [p for p in trainer.model.parameters() if p.requires_grad]
+    if kind == "torch":
+        trainer.optimizer = torch.optim.SGD(params, lr=1.0)
+    g = torch.Generator().manual_seed(4)
+    batch = {"audio": 0.1 * torch.randn(4, 1, 22050, generator=g), "label": torch.tensor([0, 1, 1, 0])}
+    trainer.model.train()
+    trainer._run_batch(0, batch)  # without the flag: no norm is taken
+    assert kind == "torch" or trainer.optimizer.last_grad_norm is None
+    args.clip_grad_norm = 1e-3
+    before = [p.detach().clone() for p in params]
+    trainer._run_batch(0, batch)
+    if kind == "fused":
+        # the arena holds the gradients as the backward left them
+        want = _norm64([trainer.optimizer.flat_grad])
+        assert abs(float(trainer.optimizer.last_grad_norm) - want) <= 2.0 ** -22 * want and want > 1e-3
+    else:
+        # plain descent at a rate of 1 moves by the clipped gradients; each parameter's difference is off by its rounding
+        moved = _norm64([b - p for b, p in zip(before, params)])
+        noise = 2.0 ** -23 * _norm64(before)
+        assert abs(moved - 1e-3) <= 1e-3 * 1e-3 + noise
