@@ -141,7 +141,7 @@ _SIGNATURES = {
                               c_sz, c_p]),
     "afd_multi_scale": (c_i, [ctypes.POINTER(c_p), ctypes.POINTER(c_p), ctypes.POINTER(c_l), ctypes.POINTER(c_i), c_i, c_p,
                               c_p]),
-    "afd_linear_workspace_bytes": (c_sz, [c_l, c_i, c_i, c_i]),
+    "afd_linear_workspace_bytes": (c_sz, [c_p, c_l, c_p, c_l, c_l, c_i, c_i, c_i]),
     "afd_linear_forward": (c_i, [c_p, c_l, c_p, c_l, c_p, c_i, c_p, c_l, c_p, c_p, c_l] + [c_i] * 4 + [c_p, c_sz, c_p]),
     "afd_linear_backward_workspace_bytes": (c_sz, [c_l, c_i, c_i, c_i]),
     "afd_linear_backward": (c_i, [c_p, c_l, c_p, c_l, c_p, c_p, c_l, c_p, c_p, c_p, c_i, c_l] + [c_i] * 4

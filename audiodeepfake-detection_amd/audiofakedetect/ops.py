@@ -1852,15 +1852,15 @@ def _linear_forward(x, w, b, residual, act, keep=False):
     y = torch.empty((m, n), dtype=x.dtype, device=x.device)
     z = torch.empty((m, n), dtype=torch.float32, device=x.device) if keep and act else None
     if m > 0:
-        dtype = _SEQ_DTYPES[x.dtype]
+        dtype, px, pw, ldx, ldw = _SEQ_DTYPES[x.dtype], x.data_ptr(), w.data_ptr(), x.stride(0), w.stride(0)
         with _OnDevice(x) as stream:
             lib = _lib()
-            nbytes = lib.afd_linear_workspace_bytes(m, n, k, dtype)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            nbytes = lib.afd_linear_workspace_bytes(px, ldx, pw, ldw, m, n, k, dtype)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
             _native.check(lib.afd_linear_forward(
-                x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), _at(b), int(b is not None and b.dtype is torch.float32),
-                _at(residual), residual.stride(0) if residual is not None else 0, y.data_ptr(), _at(z), m, n, k, act, dtype,
-                ws.data_ptr(), nbytes, stream), "afd_linear_forward")
+                px, ldx, pw, ldw, _at(b), int(b is not None and b.dtype is torch.float32), _at(residual),
+                residual.stride(0) if residual is not None else 0, y.data_ptr(), _at(z), m, n, k, act, dtype, _at(ws), nbytes,
+                stream), "afd_linear_forward")
     return y, z
 
 
@@ -1998,9 +1998,12 @@ def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
 
 def _check_disjoint(src, dst, sizes) -> None:
     """No element may be scaled twice, nor be read after it was written for another tensor (addresses and bytes)."""
-    spans = [(o, o + n, True) for o, n in zip(dst, sizes) if n]
-    spans += [(s, s + n, False) for s, o, n in zip(src, dst, sizes) if n and s != o]
-    spans.sort()
+    spans = sorted([(o, o + n, True) for o, n in zip(dst, sizes) if n])
+    if src is not dst and spans:
+        lo, hi = spans[0][0], spans[-1][1]
+        # (an arena of its own: no source lies among the destinations)
+        if any(s < hi and s + n > lo for s, n in zip(src, sizes)):
+            spans = sorted(spans + [(s, s + n, False) for s, o, n in zip(src, dst, sizes) if n and s != o])
     end_any = end_written = 0
     for lo, hi, written in spans:
         if lo < (end_any if written else end_written):
@@ -2033,9 +2036,11 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
         into = list(out)
         if len(into) != len(grads):
             raise ValueError(f"{what}: {len(into)} tensors in out for {len(grads)} gradients")
-        for i, o in enumerate(into):
-            t = dense[i]
-            _seq_check(what, "an entry of out", o, t.shape, t.dtype, t.device)
+        for i, (o, t) in enumerate(zip(into, dense)):
+            if not isinstance(o, torch.Tensor):
+                raise TypeError(f"{what}: out[{i}] is a {type(o).__name__}, not a tensor")
+            if o.shape != t.shape or o.dtype is not t.dtype or o.device != t.device:
+                _seq_check(what, f"out[{i}]", o, t.shape, t.dtype, t.device)
             if not (o.is_contiguous() and t.is_contiguous()) and o.stride() != t.stride():
                 if not o.is_contiguous():
                     raise ValueError(f"{what}: out[{i}] has to be contiguous, or strided as its gradient")

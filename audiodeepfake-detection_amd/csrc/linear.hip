@@ -587,12 +587,13 @@ struct Arena {
 
 }  // namespace
 
-extern "C" size_t afd_linear_workspace_bytes(long long M, int N, int K, int dtype) {
-    if (M < 1 || N < 1 || K < 1 || !dtype_ok(dtype)) return 0;
+extern "C" size_t afd_linear_workspace_bytes(const void* x, long long ldx, const void* w, long long ldw, long long M, int N, int K,
+                                             int dtype) {
+    if (M < 1 || M > 0x7fffff00L || N < 1 || K < 1 || !dtype_ok(dtype)) return 0;
     const size_t e = dtype_bytes(dtype);
     const long kp = pad_to(K, 16 / (long)e);
-    // (copies of operands that cannot be read as they are: counted always, one size for a shape)
-    return align256((size_t)M * kp * e) + align256((size_t)N * kp * e) + gemm_shape((int)M, N, K, dtype).part;
+    return (direct(x, ldx, K, dtype) ? 0 : align256((size_t)M * kp * e)) +
+           (direct(w, ldw, K, dtype) ? 0 : align256((size_t)N * kp * e)) + gemm_shape((int)M, N, (int)kp, dtype).part;
 }
 
 extern "C" int afd_linear_forward(const void* x, long long ldx, const void* w, long long ldw, const void* bias, int bias_f32,
@@ -603,8 +604,7 @@ extern "C" int afd_linear_forward(const void* x, long long ldx, const void* w, l
     const size_t e = dtype_bytes(dtype);
     const long kp = pad_to(K, 16 / (long)e);
     const bool dx = direct(x, ldx, K, dtype), dw = direct(w, ldw, K, dtype);
-    const size_t need = (dx ? 0 : align256((size_t)M * kp * e)) + (dw ? 0 : align256((size_t)N * kp * e)) +
-                        gemm_shape((int)M, N, (int)kp, dtype).part;
+    const size_t need = afd_linear_workspace_bytes(x, ldx, w, ldw, M, N, K, dtype);
     if (need > 0 && (!ws || ws_bytes < need)) return fail(AFD_ERR_WORKSPACE, "linear: workspace of %zu bytes, %zu needed", ws_bytes, need);
     hipStream_t s = static_cast<hipStream_t>(stream);
     ScopedTiming timing(AFD_K_SEQUENCE, 2.0 * (double)M * N * K, s);

@@ -664,7 +664,8 @@ int afd_state_scan_step(const void* x, const void* dt, const void* b, const void
  * (fp32) receives x . w^T + bias for the backward (not needed for act 0).
  * Backward: from dy [M][N] (row stride ldy), dx = dz . w, dw = dz^T . x, dbias = sums of dz, with dz = dy act'(z) (rounded to
  * dtype in front of the two products, not for dbias); dx, dw, dbias may be NULL where not wanted.  The residual's gradient is dy. */
-size_t afd_linear_workspace_bytes(long long M, int N, int K, int dtype);
+size_t afd_linear_workspace_bytes(const void* x, long long ldx, const void* w, long long ldw, long long M, int N, int K,
+                                  int dtype); /* (what the forward of these very operands needs; may be 0) */
 int afd_linear_forward(const void* x, long long ldx, const void* w, long long ldw, const void* bias, int bias_f32,
                        const void* residual, long long ldr, void* y, float* z, long long M, int N, int K, int act, int dtype,
                        void* ws, size_t ws_bytes, afd_stream_t stream);

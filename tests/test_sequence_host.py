@@ -275,7 +275,11 @@ def test_linear_c_entries_refuse():
 
     lib = _native.load()
     one = ctypes.c_void_p(16)
-    assert lib.afd_linear_workspace_bytes(0, 4, 4, 0) == 0 and lib.afd_linear_workspace_bytes(4, 4, 4, 9) == 0
+    size = lib.afd_linear_workspace_bytes
+    assert size(one, 4, one, 4, 0, 4, 4, 0) == 0 and size(one, 4, one, 4, 4, 4, 4, 9) == 0
+    assert size(one, 64, one, 64, 4096, 4096, 64, 0) == 0               # read as they are
+    assert size(one, 65, one, 64, 4096, 4096, 64, 0) == 4096 * 64 * 4   # x's rows leave the 16-byte grid: copied
+    assert size(one, 64, ctypes.c_void_p(20), 64, 4096, 4096, 64, 0) == 4096 * 64 * 4
     assert lib.afd_linear_forward(one, 4, one, 4, None, 0, None, 0, one, None, 4, 4, 4, 7, 0, None, 0, None) == -1
     assert lib.afd_linear_forward(one, 4, one, 4, None, 0, None, 0, one, None, 4, 1 << 20, 4, 0, 0, None, 0, None) == -3
     assert lib.afd_linear_forward(one, 3, one, 3, None, 0, None, 0, one, None, 4, 4, 3, 0, 0, None, 0, None) == -4
