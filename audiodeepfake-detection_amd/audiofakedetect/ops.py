@@ -14,6 +14,7 @@ from typing import Optional
 
 import torch
 import torch.distributed as dist
+from torch.autograd.graph import increment_version
 
 from . import _native
 
@@ -1546,6 +1547,12 @@ def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
+def _near_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """`_rows`, with the rows at most 2^24 elements apart (the scan's lanes reach 16 rows with 32-bit offsets)."""
+    t = _rows(t)
+    return t if t is None or t.stride(1) <= 1 << 24 else t.contiguous()
+
+
 def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or t.is_contiguous() else t.contiguous()
 
@@ -1573,13 +1580,15 @@ def _wants_grad(*tensors) -> bool:
 
 
 def _step_state(what: str, state, state_out, tensors) -> torch.Tensor:
-    """The tensor a step writes its state to: `state` itself, or `state_out`, which may not overlap it otherwise."""
+    """The tensor a step writes its state to: `state` itself, or `state_out`, which may not overlap it otherwise.  (Its version
+    is moved on, so that a backward pass that saved the old state refuses to run on the new one.)"""
     if _wants_grad(*tensors):
         raise RuntimeError(f"{what}: single steps have no backward pass: call it under torch.no_grad() (the whole-sequence "
                            "form is differentiable)")
     if not state.is_contiguous():
         raise ValueError(f"{what}: state has to be contiguous (it is updated in place)")
     if state_out is None:
+        increment_version(state)
         return state
     _seq_check(what, "state_out", state_out, state.shape, state.dtype, state.device)
     if not state_out.is_contiguous():
@@ -1587,6 +1596,7 @@ def _step_state(what: str, state, state_out, tensors) -> torch.Tensor:
     p, q, n = state.data_ptr(), state_out.data_ptr(), state.numel() * state.element_size()
     if p != q and p < q + n and q < p + n:
         raise ValueError(f"{what}: state_out overlaps state without being it")
+    increment_version(state_out)
     return state_out
 
 
@@ -1785,7 +1795,7 @@ class _StateScan(torch.autograd.Function):
                 grads[8].copy_(dstate_out)
             return (*grads, None, None, None)
         dx, ddt, da, db, dc, dd, dgate, dbias, dstate = grads
-        dy = _rows(dy) if dy is not None else torch.zeros_like(x)
+        dy = _near_rows(dy) if dy is not None else torch.zeros(x.shape, dtype=x.dtype, device=x.device)
         dstate_out = _dense(dstate_out)
         with _OnDevice(x) as stream:
             lib = _lib()
@@ -1811,11 +1821,11 @@ def state_scan(x, dt, a, b, c, d=None, gate=None, dt_bias=None, softplus: bool =
     a [D, N], 1 <= N <= 64, d [D], dt_bias [D] and `state` [B, D, N] float32.  gate, d, dt_bias and state may be absent.
     `lengths` and `return_state` as `causal_conv`'s; the state is float32.  Differentiable in every tensor but lengths; the
     recurrence and all sums in float32, results rounded once to the type of their tensor.  Gradients do not depend on the
-    order of execution.  Training keeps the state in front of every 16 tokens (float32)."""
+    order of execution.  Training keeps the state in front of every 8 tokens (float32)."""
     _scan_check("state_scan", x, dt, a, b, c, d, gate, dt_bias, state, 3)
     lengths = _seq_lengths("state_scan", lengths, x)
     _seq_gpu("state_scan", x)
-    x, dt, b, c, gate = _rows(x), _rows(dt), _rows(b), _rows(c), _rows(gate)
+    x, dt, b, c, gate = _near_rows(x), _near_rows(dt), _near_rows(b), _near_rows(c), _near_rows(gate)
     a, d, dt_bias, state = _dense(a), _dense(d), _dense(dt_bias), _dense(state)
     run = _StateScan.apply if _wants_grad(x, dt, a, b, c, d, gate, dt_bias, state) else _scan_forward
     y, state_out = run(x, dt, a, b, c, d, gate, dt_bias, state, lengths, int(bool(softplus)), bool(return_state))[:2]
@@ -1843,6 +1853,7 @@ def state_scan_step(x, state, dt, a, b, c, d=None, gate=None, dt_bias=None, soft
 
 
 _LINEAR_ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+_LINEAR_GRAD_ROWS = 8_000_000  # (turned operands: rows of this many elements, 255 of them within a 32-bit offset)
 
 
 def _linear_forward(x, w, b, residual, act, keep=False):
@@ -1904,8 +1915,8 @@ def linear(x, w, b=None, activation: str = "none", residual=None):
     """act(x @ w.T + b) + residual in one pass: x [..., K], w [N, K] and residual [..., N] of one type (float32 / bfloat16 /
     float16), b [N] float32 or of that type; `activation` "none", "relu", "silu" or "gelu" (with the error function).  float32
     products are exact, all sums are float32, the result is rounded once.  Differentiable in every tensor; the backward
-    keeps x @ w.T + b in float32 for the activation's slope, and rounds the gradient to the type of x in front of its two
-    products (not for b's)."""
+    keeps x @ w.T + b in float32 for the activation's slope, rounds the gradient to the type of x in front of its two
+    products (not for b's), and takes at most 8 million rows."""
     what = "linear"
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what}: x is a {type(x).__name__}, not a tensor")
@@ -1927,11 +1938,15 @@ def linear(x, w, b=None, activation: str = "none", residual=None):
     _seq_check(what, "residual", residual, (*x.shape[:-1], n), x.dtype, x.device)
     if activation not in _LINEAR_ACTIVATIONS:
         raise ValueError(f"{what}: activation {activation!r}; one of {sorted(_LINEAR_ACTIVATIONS)} expected")
+    rows = x.reshape(-1, k)
+    grad = _wants_grad(x, w, b, residual)
+    if grad and rows.shape[0] > _LINEAR_GRAD_ROWS:
+        raise ValueError(f"{what}: {rows.shape[0]} rows; at most {_LINEAR_GRAD_ROWS} where gradients are wanted")
     _seq_gpu(what, x)
-    rows = _rows(x.reshape(-1, k))
+    rows = _rows(rows)
     res = _rows(residual.reshape(-1, n)) if residual is not None else None
     w, b = _rows(w), _dense(b)
-    if _wants_grad(rows, w, b, res):
+    if grad:
         y = _Linear.apply(rows, w, b, res, _LINEAR_ACTIVATIONS[activation])
     else:
         y = _linear_forward(rows, w, b, res, _LINEAR_ACTIVATIONS[activation])[0]
@@ -2017,7 +2032,8 @@ def _check_disjoint(src, dst, sizes) -> None:
 def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """Scales `grads` by min(1, max_norm / (norm + 1e-6)), norm being their `global_norm`, in place or into the tensors of
     `out` (same shapes and types; in place where an entry is the gradient itself).  Returns the norm in front of the
-    scaling, a float32 scalar on the device; nothing waits for it on the host.  A norm of inf gives zeros, NaN gives NaN."""
+    scaling, a float32 scalar on the device; nothing waits for it on the host.  With a norm of inf the finite elements become
+    zero and the others NaN (as inf * 0 is); a norm of NaN makes all of them NaN."""
     what = "clip_gradients"
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
@@ -2052,6 +2068,7 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     arrays, src, sizes = _norm_arrays(dense)
     dst = src if out is None else [t.data_ptr() for t in into]
     _check_disjoint(src, dst, sizes)
+    increment_version(into)
     with _OnDevice(dense[0]) as stream:
         stats = _launch_norm(arrays, n, dense[0].device, norm_type, max_norm, 1.0, stream)
         _native.check(_lib().afd_multi_scale(arrays[0], (_native.c_p * n)(*dst), arrays[1], arrays[2], n, stats.data_ptr(),

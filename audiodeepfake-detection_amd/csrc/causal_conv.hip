@@ -340,7 +340,7 @@ int run(Kind kind, ConvArgs& p, int W, int dtype, hipStream_t s) {
         const int per = kT / p.gx;
         grid = (((size_t)p.B * p.ntiles + per - 1) / per) * p.gblocks;
     }
-    if (grid > 0x7fffffffu) return fail(AFD_ERR_UNSUPPORTED, "causal conv: %zu workgroups", grid);
+    if (grid > (size_t)kMaxGroups) return fail(AFD_ERR_UNSUPPORTED, "causal conv: %zu workgroups", grid);
     if (dtype == AFD_T_F32) {
         if (v > 1) launch_w<float, 4>(kind, W, p, (unsigned)grid, s);
         else launch_w<float, 1>(kind, W, p, (unsigned)grid, s);

@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(const Gemm g) {
     constexpr int EPC = 16 / (int)sizeof(T), KS = kSlab / (int)sizeof(T);  // elements per chunk and per slab
     constexpr int CA = TM * 8 / kThreads, CB = TN * 8 / kThreads;          // chunks a thread stages
     constexpr int kBuf = (TM + TN) * kSlab;
-    extern __shared__ char lds[];
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     int tm, tn;
     tile_of(g, blockIdx.x, tm, tn);
     const int m0 = tm * TM, n0 = tn * TN;
@@ -411,8 +411,8 @@ __global__ void __launch_bounds__(256) pad_kernel(const T* __restrict__ src, lon
     }
 }
 
-// dz = dy act'(z) as rows (ldz, zeros behind N; NULL: not wanted) and turned (ldt, zeros behind M), and its column sums over
-// the tile's rows.
+// dz = dy act'(z) as rows (ldz, zeros behind N) and turned (ldt, zeros behind M), and its column sums over the tile's rows;
+// NULL: not wanted.
 template <typename T>
 __global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ dy, long ldy, const float* __restrict__ z, int act, int M, int N,
                                                  T* __restrict__ dz, long ldz, T* __restrict__ turned, long ldt,
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ dy, long 
         float v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = t[x8 + k][i];
-        if (n0 + i < N) store8<T>(turned + (size_t)(n0 + i) * ldt + m0 + x8, (int)min(ldt - m0 - x8, 8L), v);
+        if (turned && n0 + i < N) store8<T>(turned + (size_t)(n0 + i) * ldt + m0 + x8, (int)min(ldt - m0 - x8, 8L), v);
     }
     if (!sums) return;
     __shared__ float red[4][64];
@@ -570,14 +570,14 @@ bool direct(const void* p, long ld, int K, int dtype) {
 int check(const char* what, long M, int N, int K, int act, int dtype) {
     if (M < 1 || N < 1 || K < 1 || act < 0 || act > 3 || !dtype_ok(dtype))
         return fail(AFD_ERR_ARG, "%s: M=%ld N=%d K=%d act=%d dtype=%d", what, M, N, K, act, dtype);
-    if (M > 0x7fffff00L || N > (1 << 20) - 64 || K > (1 << 20) - 64 || (long)ceil_div(M, 128) * ceil_div(N, 128) > 0x7fffffffL)
+    if (M > 0x7fffff00L || N > (1 << 20) - 64 || K > (1 << 20) - 64 || (long)ceil_div(M, 128) * ceil_div(N, 64) > kMaxGroups)
         return fail(AFD_ERR_UNSUPPORTED, "%s: M=%ld N=%d K=%d is too large", what, M, N, K);
     return AFD_OK;
 }
 
 struct Arena {
     char* base;
-    size_t at, size;
+    size_t at;
     void* take(size_t n) {
         void* p = base + at;
         at += align256(n);
@@ -608,7 +608,7 @@ extern "C" int afd_linear_forward(const void* x, long long ldx, const void* w, l
     if (need > 0 && (!ws || ws_bytes < need)) return fail(AFD_ERR_WORKSPACE, "linear: workspace of %zu bytes, %zu needed", ws_bytes, need);
     hipStream_t s = static_cast<hipStream_t>(stream);
     ScopedTiming timing(AFD_K_SEQUENCE, 2.0 * (double)M * N * K, s);
-    Arena ar{static_cast<char*>(ws), 0, ws_bytes};
+    Arena ar{static_cast<char*>(ws), 0};
     if (!dx) {
         void* c = ar.take((size_t)M * kp * e);
         if (int rc = pad(x, ldx, (int)M, K, c, kp, dtype, s)) return rc;
@@ -674,7 +674,7 @@ extern "C" int afd_linear_backward(const void* x, long long ldx, const void* w, 
         return fail(AFD_ERR_WORKSPACE, "linear backward: workspace of %zu bytes, %zu needed", ws_bytes, b.total);
     hipStream_t s = static_cast<hipStream_t>(stream);
     ScopedTiming timing(AFD_K_SEQUENCE, 2.0 * (double)M * N * K * ((dx != nullptr) + (dw != nullptr)), s);
-    Arena ar{static_cast<char*>(ws), 0, ws_bytes};
+    Arena ar{static_cast<char*>(ws), 0};
     void* dz = ar.take(b.dz);
     void* dzt = ar.take(b.dzt);
     void* xt = ar.take(b.xt);
@@ -684,10 +684,14 @@ extern "C" int afd_linear_backward(const void* x, long long ldx, const void* w, 
     // without an activation dy is dz, and can be read as it is where its rows allow
     const bool rows = act != kNone || !direct(dy, ldy, N, dtype);
     void* rz = dx && rows ? dz : nullptr;
-    int rc = dtype == AFD_T_F32 ? dz_t<float>(dy, ldy, z, act, (int)M, N, rz, b.np, dzt, b.mp, dbias ? sums : nullptr, s)
-             : dtype == AFD_T_BF16 ? dz_t<bf16_t>(dy, ldy, z, act, (int)M, N, rz, b.np, dzt, b.mp, dbias ? sums : nullptr, s)
-                                   : dz_t<f16_t>(dy, ldy, z, act, (int)M, N, rz, b.np, dzt, b.mp, dbias ? sums : nullptr, s);
-    if (rc) return rc;
+    void* rt = dw ? dzt : nullptr;
+    float* rs = dbias ? sums : nullptr;
+    if (rz || rt || rs) {
+        const int rc = dtype == AFD_T_F32 ? dz_t<float>(dy, ldy, z, act, (int)M, N, rz, b.np, rt, b.mp, rs, s)
+                       : dtype == AFD_T_BF16 ? dz_t<bf16_t>(dy, ldy, z, act, (int)M, N, rz, b.np, rt, b.mp, rs, s)
+                                             : dz_t<f16_t>(dy, ldy, z, act, (int)M, N, rz, b.np, rt, b.mp, rs, s);
+        if (rc) return rc;
+    }
     if (dbias) {
         ColumnOuts o{};
         o.n = 1;

@@ -1,4 +1,4 @@
-// Shared by the sequence-layer kernels (causal_conv.hip, state_scan*.hip, grad_clip.hip): element types, the
+// Shared by the sequence-layer kernels (causal_conv.hip, state_scan*.hip, linear.hip, grad_clip.hip): element types, the
 // non-linearities of the state-space layer and the column sums that end their parameter gradients.
 #pragma once
 
@@ -12,6 +12,8 @@ typedef _Float16 f16_t;
 
 template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }  // round to nearest even
+
+constexpr long kMaxGroups = 0xffffff;  // workgroups of 256 threads: a launch holds less than 2^32 threads
 
 inline size_t dtype_bytes(int dtype) { return dtype == AFD_T_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == AFD_T_F32 || dtype == AFD_T_BF16 || dtype == AFD_T_F16; }

@@ -120,7 +120,7 @@ template <typename T, int Q, int NS, bool LOCAL>
 __global__ void __launch_bounds__(kScanT, LOCAL ? 4 : kBwdWaves) scan_bwd_kernel(const ScanArgs p) {
     constexpr int NP = Q * NS, TB = kTokB, R = TB > Q ? TB / Q : 1;
     constexpr int TS = 2 * TB;  // tokens between barriers: b and c rows come, and sums over channels go, for TS at a time
-    __shared__ float lds[2][TS * 2 * NP];
+    __shared__ __attribute__((aligned(16))) float lds[2][TS * 2 * NP];
     __shared__ float red[LOCAL ? 1 : 2][LOCAL ? 1 : 4 * TS * 2 * NP];
     const ScanPlace w = scan_place<Q, NS>(p);
     const int wave = threadIdx.x >> 6;

@@ -11,7 +11,7 @@ using namespace afd;
 template <typename T, int Q, int NS, bool LOCAL>
 __global__ void __launch_bounds__(kScanT) scan_fwd_kernel(const ScanArgs p) {
     constexpr int NP = Q * NS, R = kTokF / Q;
-    __shared__ float lds[2][kTokF * 2 * NP];
+    __shared__ __attribute__((aligned(16))) float lds[2][kTokF * 2 * NP];
     const ScanPlace w = scan_place<Q, NS>(p);
     const int start = w.s * p.seg;
     const int end = min(start + p.seg, w.n);  // tokens [start, end) are this segment's
@@ -318,7 +318,7 @@ int check(const char* what, int B, int L, int D, int N, int dtype) {
     if (B < 1 || L < 1 || D < 1 || N < 1 || N > 64 || !dtype_ok(dtype))
         return fail(AFD_ERR_ARG, "%s: B=%d L=%d D=%d N=%d (1..64) dtype=%d", what, B, L, D, N, dtype);
     const ScanPlan q = scan_plan(B, L, D, N, false);
-    if ((long)B * q.S * q.nb > 0x7fffffffL || (long)D * (q.g.NP + 2) > 0x7fffffc0L || L > 0x7fff0000 ||
+    if ((long)B * q.S * q.nb > kMaxGroups || (long)D * (q.g.NP + 2) > 0x3fffffffL || L > 0x7fff0000 ||
         (long)D * kTokF * 4 > 0x7fffffffL)
         return fail(AFD_ERR_UNSUPPORTED, "%s: B=%d L=%d D=%d is too large", what, B, L, D);
     return AFD_OK;

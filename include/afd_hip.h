@@ -641,7 +641,7 @@ int afd_causal_conv_step(const void* x, long long xb, const void* w, const void*
  *   h[t] = exp(delta a) h[t-1] + delta b[t] x[t],   y = (sum_n c[t][n] h[t][n] + d x[t]) * silu(gate)
  * gate, d, dt_bias, state, state_out may be NULL.  strides (HOST): batch, row of x, dt, b, c, gate (10 values), then
  * of dy (backward: 12); the step form takes the batch strides alone (5).  checkpoints: NULL, or
- * afd_state_scan_checkpoint_floats floats that the backward reads (the state in front of every 16 tokens).
+ * afd_state_scan_checkpoint_floats floats that the backward reads (the state in front of every 8 tokens).
  * b, c [B][L][N]; db, dc likewise, dense.  dgate, dd, ddt_bias, dstate may be NULL where the input is. */
 size_t afd_state_scan_workspace_bytes(int B, int L, int D, int N, int backward);
 size_t afd_state_scan_checkpoint_floats(int B, int L, int D, int N);

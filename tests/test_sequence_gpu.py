@@ -309,6 +309,43 @@ def test_scan_strided_views_and_expanded_rows():
     assert torch.equal(dp, torch.cat([dx, dg], -1))
 
 
+def test_scan_rows_far_apart_in_memory():
+    """Rows farther apart than the lanes' 32-bit offsets reach."""
+    t = _scan_inputs(9, "bf16", 1, 40, 24, 4)
+    want = ops.state_scan(**t, softplus=True)
+    far = torch.empty(40 * ((1 << 24) + 8), dtype=torch.bfloat16, device="cuda")
+    x = far.as_strided((1, 40, 24), (0, (1 << 24) + 8, 1))
+    x.copy_(t["x"])
+    assert torch.equal(ops.state_scan(**dict(t, x=x), softplus=True), want)
+    near = far.as_strided((1, 40, 24), (0, 1 << 24, 1))
+    near.copy_(t["x"])
+    assert torch.equal(ops.state_scan(**dict(t, x=near), softplus=True), want)
+    # ... and a gradient like that
+    v = t["x"].requires_grad_(True)
+    (dx,) = torch.autograd.grad(ops.state_scan(**t, softplus=True), [v], torch.ones_like(want))
+    x.fill_(1.0)
+    (dx2,) = torch.autograd.grad(ops.state_scan(**t, softplus=True), [v], x)
+    assert torch.equal(dx, dx2)
+
+
+def test_a_state_that_a_backward_pass_needs_is_not_changed_unseen():
+    t = _scan_inputs(10, "fp32", 2, 5, 8, 4)
+    c = _conv_inputs(10, "fp32", 2, 5, 8, 4, True, True)
+    x = t["x"].detach().requires_grad_(True)
+    state, cstate = t["state"].clone(), c["state"].clone()
+    ys = ops.state_scan(**dict(t, x=x, state=state), softplus=True), ops.causal_conv(x, c["w"], c["b"], "silu", state=cstate)
+    with torch.no_grad():
+        ops.state_scan_step(t["x"][:, 0], state, t["dt"][:, 0], t["a"], t["b"][:, 0], t["c"][:, 0])
+        ops.causal_conv_step(t["x"][:, 0], torch.empty_like(cstate), c["w"], state_out=cstate)
+    for y in ys:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y.sum(), [x])
+    p = torch.ones(5, device="cuda")
+    before = p._version
+    ops.clip_gradients([p], 1.0)
+    assert p._version > before
+
+
 def test_gradients_flow_through_the_state_between_parts():
     """Two parts joined by their state have the gradients of the whole, for both operators."""
     t = _scan_inputs(13, "fp32", 2, 50, 21, 6)
@@ -783,6 +820,26 @@ def test_linear_views_leading_axes_and_unaligned_rows():
     y = ops.linear(empty, w, torch.zeros(5, device="cuda"), "silu")
     dx, dw = torch.autograd.grad(y.sum(), [empty, w])
     assert y.shape == (0, 5) and dx.shape == (0, 72) and not dw.any()
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_linear_gradients_wanted_one_by_one(act, dtype):
+    """A frozen weight, a first layer, a bias alone: the same gradients, without the others' work."""
+    g = torch.Generator().manual_seed(79)
+    for k in (64, 37):
+        v = dict(x=_rnd(g, 70, k, dtype=TYPES[dtype]), w=_rnd(g, 48, k, dtype=TYPES[dtype]), b=_rnd(g, 48),
+                 residual=_rnd(g, 70, 48, dtype=TYPES[dtype]))
+        dy = _rnd(g, 70, 48, dtype=TYPES[dtype])
+
+        def grads(names):
+            t = {key: x.detach().requires_grad_(key in names) for key, x in v.items()}
+            y = ops.linear(t["x"], t["w"], t["b"], act, residual=t["residual"])
+            return torch.autograd.grad(y, [t[key] for key in names], dy)
+
+        every = dict(zip(v, grads(list(v))))
+        for names in (["x"], ["w"], ["b"], ["residual"], ["x", "b"], ["w", "b"], ["x", "w"]):
+            assert all(torch.equal(got, every[key]) for key, got in zip(names, grads(names))), names
 
 
 def test_linear_rows_do_not_leak_into_each_other():

@@ -286,3 +286,29 @@ def test_linear_c_entries_refuse():
     assert lib.afd_linear_backward(one, 4, one, 4, None, one, 4, one, one, None, 0, 4, 4, 4, 2, 0, None, 0, None) == -1
     assert lib.afd_linear_backward(one, 4, one, 4, one, one, 4, one, one, None, 0, 4, 4, 4, 2, 0, None, 0, None) == -4
     assert lib.afd_linear_backward(one, 4, one, 4, None, one, 4, one, one, None, 0, 9000000, 4, 4, 0, 0, one, 0, None) == -3
+
+
+def test_linear_refuses_more_rows_than_its_backward_takes():
+    x = torch.zeros(1, 8).expand(8_000_001, 8)
+    w = torch.zeros(4, 8, requires_grad=True)
+    with pytest.raises(ValueError, match="8000001 rows"):
+        ops.linear(x, w)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+        ops.linear(x, w)
+
+
+def test_c_entries_refuse_more_workgroups_than_a_launch_holds():
+    import ctypes
+
+    lib = _native.load()
+    one = ctypes.c_void_p(16)
+    strides = (_native.c_l * 12)()
+    most = 0xffffff  # workgroups of 256 threads
+    assert lib.afd_state_scan_step(one, one, one, one, None, strides, one, None, None, one, one, one, most + 1, 64, 16, 1, 0,
+                                   None) == -3
+    assert lib.afd_state_scan_forward(one, one, one, one, None, strides, one, None, None, None, None, one, None, None,
+                                      most + 1, 2, 64, 16, 1, 0, None, 0, None) == -3
+    assert lib.afd_state_scan_step(one, one, one, one, None, strides, one, None, None, one, one, one, 1, 0x3fffffff // 66 + 1,
+                                   64, 1, 0, None) == -3
+    assert lib.afd_causal_conv_step(one, 1, one, None, 1, one, one, one, 0x7fffffff, 8, 4, 0, 0, None) == -3
+    assert lib.afd_linear_forward(one, 4, one, 4, None, 0, None, 0, one, None, 0x7fffff00, 80, 4, 0, 0, None, 0, None) == -3
