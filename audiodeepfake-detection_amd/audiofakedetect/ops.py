@@ -1959,32 +1959,40 @@ def _gapless(t: torch.Tensor) -> bool:
     return t.permute(sorted(range(t.dim()), key=lambda k: -t.stride(k))).is_contiguous()
 
 
-def _norm_tables(what: str, tensors, norm_type):
-    """The list as tensors in dense memory (the order of the elements is of no interest to a norm: a permuted but gapless
-    tensor is taken as it lies), ready for `afd_global_norm`."""
-    if norm_type not in (2, 2.0, float("inf")):
-        raise ValueError(f"{what}: norm_type {norm_type}; 2 or inf expected")
-    dense, device = [], None
-    for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{what}: entry {len(dense)} is a {type(t).__name__}, not a tensor")
-        if t.dtype not in _SEQ_DTYPES or t.layout is not torch.strided:
-            raise TypeError(f"{what}: entry {len(dense)} is {t.layout} {t.dtype}; dense float32, bfloat16 or float16 expected")
-        if t.device != device:
-            if device is not None:
-                raise ValueError(f"{what}: entry {len(dense)} is on {t.device}, entry 0 on {device}")
-            device = t.device
-        dense.append(t if t.is_contiguous() or _gapless(t) else t.detach().contiguous())
-    return dense
+# (Lists of gradients are small tensors in the main, and the host's time per tensor is then the call's: every attribute is
+# read once, into a list, and the lists are compared as a whole; what does not match is looked for afterwards.)
+class _NormTable:
+    """The tensors of one call in dense memory, and what `afd_global_norm` wants to know of them.  (The order of the elements
+    is of no interest to a norm: a permuted but gapless tensor is taken as it lies.)"""
 
+    __slots__ = ("dense", "plain", "dtypes", "ptrs", "counts", "codes", "arrays")
 
-def _norm_arrays(dense):
-    """(pointers, counts, types) of the tensors as host arrays, and the pointers and sizes in bytes as lists."""
-    n = len(dense)
-    ptrs, counts = [t.data_ptr() for t in dense], [t.numel() for t in dense]
-    types = [_SEQ_DTYPES[t.dtype] for t in dense]
-    return ((_native.c_p * n)(*ptrs), (_native.c_l * n)(*counts), (_native.c_i * n)(*types)), ptrs, \
-        [c * (2 if k else 4) for c, k in zip(counts, types)]
+    def __init__(self, what: str, tensors, norm_type):
+        if norm_type != 2 and norm_type != float("inf"):
+            raise ValueError(f"{what}: norm_type {norm_type}; 2 or inf expected")
+        for i, t in enumerate(tensors):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{what}: entry {i} is a {type(t).__name__}, not a tensor")
+        self.dtypes = [t.dtype for t in tensors]
+        if not (set(self.dtypes) <= _SEQ_DTYPES.keys() and {t.layout for t in tensors} <= {torch.strided}):
+            i, t = next((i, t) for i, t in enumerate(tensors) if t.dtype not in _SEQ_DTYPES or t.layout is not torch.strided)
+            raise TypeError(f"{what}: entry {i} is {t.layout} {t.dtype}; dense float32, bfloat16 or float16 expected")
+        if len({t.get_device() for t in tensors}) > 1:
+            i = next(i for i, t in enumerate(tensors) if t.device != tensors[0].device)
+            raise ValueError(f"{what}: entry {i} is on {tensors[i].device}, entry 0 on {tensors[0].device}")
+        self.plain = all([t.is_contiguous() for t in tensors])
+        self.dense = tensors if self.plain else [t if t.is_contiguous() or _gapless(t) else t.detach().contiguous()
+                                                 for t in tensors]
+
+    def lay_out(self):
+        n = len(self.dense)
+        self.ptrs, self.counts = [t.data_ptr() for t in self.dense], [t.numel() for t in self.dense]
+        self.codes = [_SEQ_DTYPES[k] for k in self.dtypes]
+        self.arrays = (_native.c_p * n)(*self.ptrs), (_native.c_l * n)(*self.counts), (_native.c_i * n)(*self.codes)
+        return self.arrays
+
+    def sizes(self):
+        return [c << 1 if k else c << 2 for c, k in zip(self.counts, self.codes)]
 
 
 def _launch_norm(arrays, n: int, device, norm_type, max_norm: float, scale: float, stream: int) -> torch.Tensor:
@@ -2003,12 +2011,13 @@ def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """Norm of all elements of all `tensors` (float32 / bfloat16 / float16, mixed as they come) as one float32 scalar on their
     device, without a host synchronisation: the root of the sum of squares, taken in float64, or the largest magnitude
     (norm_type inf).  NaN if an element is; zero for an empty list."""
-    dense = _norm_tables("global_norm", tensors, norm_type)
+    table = _NormTable("global_norm", list(tensors), norm_type)
+    dense = table.dense
     if not dense:
         return torch.zeros(())
     _seq_gpu("global_norm", dense[0])
     with _OnDevice(dense[0]) as stream:
-        return _launch_norm(_norm_arrays(dense)[0], len(dense), dense[0].device, norm_type, 1.0, 1.0, stream)[0]
+        return _launch_norm(table.lay_out(), len(dense), dense[0].device, norm_type, 1.0, 1.0, stream)[0]
 
 
 def _check_disjoint(src, dst, sizes) -> None:
@@ -2017,7 +2026,7 @@ def _check_disjoint(src, dst, sizes) -> None:
     if src is not dst and spans:
         lo, hi = spans[0][0], spans[-1][1]
         # (an arena of its own: no source lies among the destinations)
-        if any(s < hi and s + n > lo for s, n in zip(src, sizes)):
+        if any([s < hi and s + n > lo for s, n in zip(src, sizes)]):
             spans = sorted(spans + [(s, s + n, False) for s, o, n in zip(src, dst, sizes) if n and s != o])
     end_any = end_written = 0
     for lo, hi, written in spans:
@@ -2039,11 +2048,12 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     if not max_norm >= 0.0:
         raise ValueError(f"{what}: max_norm {max_norm} has to be a number from 0 on")
     grads = list(grads)
-    dense = _norm_tables(what, grads, norm_type)
+    table = _NormTable(what, grads, norm_type)
+    dense = table.dense
     back = []  # (gradient, dense copy) where the gradient's memory has gaps
     if out is None:
         into = dense
-        for g, t in zip(grads, dense):
+        for g, t in zip(grads, dense) if not table.plain else ():
             if t is not g:
                 if any(s == 0 and k > 1 for s, k in zip(g.stride(), g.shape)):
                     raise ValueError(f"{what}: a gradient with elements that share memory cannot be scaled in place")
@@ -2052,22 +2062,26 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
         into = list(out)
         if len(into) != len(grads):
             raise ValueError(f"{what}: {len(into)} tensors in out for {len(grads)} gradients")
-        for i, (o, t) in enumerate(zip(into, dense)):
+        for i, o in enumerate(into):
             if not isinstance(o, torch.Tensor):
                 raise TypeError(f"{what}: out[{i}] is a {type(o).__name__}, not a tensor")
-            if o.shape != t.shape or o.dtype is not t.dtype or o.device != t.device:
+        if not (table.plain and [o.dtype for o in into] == table.dtypes and [o.shape for o in into] == [g.shape for g in grads]
+                and all([o.is_contiguous() for o in into]) and len({o.get_device() for o in (*into, *grads[:1])}) <= 1):
+            dense = list(dense)
+            for i, (o, t) in enumerate(zip(into, dense)):
                 _seq_check(what, f"out[{i}]", o, t.shape, t.dtype, t.device)
-            if not (o.is_contiguous() and t.is_contiguous()) and o.stride() != t.stride():
-                if not o.is_contiguous():
-                    raise ValueError(f"{what}: out[{i}] has to be contiguous, or strided as its gradient")
-                dense[i] = t.detach().contiguous()
+                if not (o.is_contiguous() and t.is_contiguous()) and o.stride() != t.stride():
+                    if not o.is_contiguous():
+                        raise ValueError(f"{what}: out[{i}] has to be contiguous, or strided as its gradient")
+                    dense[i] = t.detach().contiguous()
+            table.dense = dense
     if not dense:
         return torch.zeros(())
     _seq_gpu(what, dense[0])
     n = len(dense)
-    arrays, src, sizes = _norm_arrays(dense)
-    dst = src if out is None else [t.data_ptr() for t in into]
-    _check_disjoint(src, dst, sizes)
+    arrays = table.lay_out()
+    dst = table.ptrs if out is None else [t.data_ptr() for t in into]
+    _check_disjoint(table.ptrs, dst, table.sizes())
     increment_version(into)
     with _OnDevice(dense[0]) as stream:
         stats = _launch_norm(arrays, n, dense[0].device, norm_type, max_norm, 1.0, stream)
@@ -2176,8 +2190,8 @@ class FusedAdam(torch.optim.Optimizer):
         self.gather_grads()
         if max_grad_norm is not None:
             with _OnDevice(self.flat) as stream:
-                stats = _launch_norm(_norm_arrays([self._flat_grad])[0], 1, self.flat.device, 2.0, float(max_grad_norm),
-                                     float(grad_scale), stream)
+                stats = _launch_norm(_NormTable("FusedAdam.step", [self._flat_grad], 2.0).lay_out(), 1, self.flat.device, 2.0,
+                                     float(max_grad_norm), float(grad_scale), stream)
                 _native.check(_lib().afd_adam_step_clipped(
                     _native.ptr(self.flat), _native.ptr(self._flat_grad), _native.ptr(self.m), _native.ptr(self.v),
                     self.flat.numel(), g["lr"], g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"], self.step_count,
