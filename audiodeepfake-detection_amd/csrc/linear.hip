@@ -77,6 +77,14 @@ struct Gemm {
     int tm, tn;     // tiles
 };
 
+// One element.
+template <typename T> __device__ __forceinline__ void finish_one(const Epi& e, int m, int n, int N, float z) {
+    if (e.z) e.z[(size_t)m * N + n] = z;
+    float o = activate<T>(z, e.act);
+    if (e.residual) o += to_f32(static_cast<const T*>(e.residual)[(size_t)m * e.ldr + n]);
+    static_cast<T*>(e.out)[(size_t)m * e.ldo + n] = from_f32<T>(o);
+}
+
 // V consecutive columns n .. n + V of row m.  The pre-activation is kept in fp32 whatever the tensors' type: the bias gradient
 // is a sum of dy times its slope and an fp32 parameter's; at a z rounded to bf16 it was off by 2e-3.
 template <typename T, int V>
@@ -103,12 +111,7 @@ __device__ __forceinline__ void finish(const Epi& e, int m, int n, int N, float 
             for (int g = 0; g < V; g += 4) store_row<float, 4>(zp + g, *reinterpret_cast<float(*)[4]>(&v[g]));
         }
     } else {
-        for (int i = 0; i < V && n + i < N; ++i) {
-            const float z = v[i] + bias[i];
-            if (zp) zp[i] = z;
-            const float o = activate<T>(z, e.act);
-            out[i] = from_f32<T>(res ? o + to_f32(res[i]) : o);
-        }
+        for (int i = 0; i < V && n + i < N; ++i) finish_one<T>(e, m, n + i, N, v[i] + bias[i]);
     }
 }
 
@@ -194,11 +197,15 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(const Gemm g) {
             for (int e = 0; e < CA; ++e) ra[e] = at(pa, oa[e]);
 #pragma unroll
             for (int e = 0; e < CB; ++e) rb[e] = at(pb, ob[e]);
-        } else {  // (kend is a multiple of a chunk)
+        } else {  // (kend is a multiple of a chunk; for chunks behind it the row's first, then zeros: one wait for all)
 #pragma unroll
-            for (int e = 0; e < CA; ++e) ra[e] = k + chunk[e] * EPC < kend ? at(pa, oa[e]) : u32x4{0, 0, 0, 0};
+            for (int e = 0; e < CA; ++e) ra[e] = at(pa, k + chunk[e] * EPC < kend ? oa[e] : oa[e] - chunk[e] * 16);
 #pragma unroll
-            for (int e = 0; e < CB; ++e) rb[e] = k + chunk[e] * EPC < kend ? at(pb, ob[e]) : u32x4{0, 0, 0, 0};
+            for (int e = 0; e < CB; ++e) rb[e] = at(pb, k + chunk[e] * EPC < kend ? ob[e] : ob[e] - chunk[e] * 16);
+#pragma unroll
+            for (int e = 0; e < CA; ++e) ra[e] = k + chunk[e] * EPC < kend ? ra[e] : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < CB; ++e) rb[e] = k + chunk[e] * EPC < kend ? rb[e] : u32x4{0, 0, 0, 0};
         }
     };
     auto put = [&](int buf) {
@@ -327,6 +334,93 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(const Gemm g) {
             }
         }
         __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Up to 16 MT rows: B's rows (the weights) are what is read, each once, straight into the operand registers of 16-column
+// products, and x comes out of the L2.  A workgroup owns 16 columns and its 8 waves take every eighth slab of 128 bytes
+// of k, four at a time, so K = 2048 in bf16 is one batch of loads per wave; the waves meet in LDS, in a fixed order.
+constexpr int kFewWaves = 8, kFewBatch = 4;
+template <typename T> __device__ __forceinline__ void mma16(const u32x4& a, const u32x4& b, f32x4& c) {
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
+    } else if constexpr (__is_same(T, bf16_t)) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+}
+template <typename T, int MT, int NT> __global__ void __launch_bounds__(64 * kFewWaves, 2) few_rows_kernel(const Gemm g) {
+    constexpr int EPC = 16 / (int)sizeof(T), KS = kSlab / (int)sizeof(T), kStep = kFewWaves * KS, U = kFewBatch;
+    constexpr int kCols = NT * 16, kPitch = kCols + 4;  // (rows 0, 4, 8 and 12 of a tile on different banks)
+    __shared__ float red[kFewWaves][MT * 16][kPitch];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, quad = lane >> 4;
+    const int n0 = blockIdx.x * kCols;
+    const int kbeg = blockIdx.y * g.ksplit * KS, kend = min(kbeg + g.ksplit * KS, g.K);
+    const T *ap[MT], *bp[NT];
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        ap[t] = static_cast<const T*>(g.a) + (size_t)min(t * 16 + l15, g.M - 1) * g.lda;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) bp[j] = static_cast<const T*>(g.b) + (size_t)min(n0 + j * 16 + l15, g.N - 1) * g.ldb;
+    const u32x4 zero{0, 0, 0, 0};
+    for (int k0 = kbeg + wave * KS; k0 < kend; k0 += U * kStep) {
+        u32x4 ra[U][MT][2], rb[U][NT][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int ku = k0 + u * kStep;
+            const bool whole = ku + KS <= kend;  // (the same for the wave)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int k = ku + (s * 4 + quad) * EPC;
+                if (whole) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) rb[u][j][s] = *reinterpret_cast<const u32x4*>(bp[j] + k);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) ra[u][t][s] = *reinterpret_cast<const u32x4*>(ap[t] + k);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) rb[u][j][s] = k < kend ? *reinterpret_cast<const u32x4*>(bp[j] + k) : zero;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) ra[u][t][s] = k < kend ? *reinterpret_cast<const u32x4*>(ap[t] + k) : zero;
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) mma16<T>(ra[u][t][s], rb[u][j][s], acc[t][j]);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) red[wave][t * 16 + quad * 4 + r][j * 16 + l15] = acc[t][j][r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * 16 * kCols; i += 64 * kFewWaves) {
+        const int m = i / kCols, c = i % kCols, n = n0 + c;
+        if (m >= g.M || n >= g.N) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kFewWaves; ++w) v += red[w][m][c];
+        if (g.S > 1) {
+            g.part[((size_t)blockIdx.y * g.M + m) * g.ldp + n] = v;
+        } else {
+            float bias[1];
+            load_bias<T, 1>(g.e, n, g.N, bias);
+            finish_one<T>(g.e, m, n, g.N, v + bias[0]);
+        }
     }
 }
 
@@ -462,19 +556,31 @@ long pad_to(long n, long k) { return (n + k - 1) / k * k; }
 //   fp32 12928 x 512 x 1024: 128 x 128 166 / 152 / 129, 64 x 64 148 / 150 / 138, 128 x 64 144 / 139 / 132 (three workgroups
 //   per CU, and 1616 tiles where 808 leave a fifth of the card idle at the end; matrix instructions are busy 60 % of it);
 //   bf16 16384 x 2048 x 2048: 256 x 256 220 / 171 / 162, 128 x 128 263 / 211 / 186 (half the operand traffic per product).
-// Up to 32 rows there is one tile row of 32 and the weights are what is read.
+// Up to 32 rows the weights are what is read (us here, and with one 32 x 128 tile row split along k and joined):
+//   bf16 1 / 16 / 32 x 2048 x 2048: 4.9 / 6.2 / 8.1, 8.9 / 10.3 / 10.8; 32 x 8192 x 2048 (K): 12.9 with 32 columns per workgroup,
+//   15.8 with 16, 13.8; fp32 1 / 16 x 2048 x 2048: 7.9 / 11.1, 12.5 / 13.8; 4 x 10000 x 1024: 11.7 with 16 columns, 16.8 with
+//   32, 17.0; but 32 rows of fp32 re-read x too often for large weights: 29 against 21.6 at 8192 x 2048, 13.8 against 16.2 at
+//   2048 x 2048.
 struct Shape {
     int kind;
     int tm, tn, S, ksplit;
     size_t part;
 };
-enum { kTile32x128, kTile128x64, kTile128, kTile256 };
+enum { kFew16, kFew32, kTile32x128, kTile128x64, kTile128, kTile256 };
+constexpr int kFewLoad = kFewWaves * kFewBatch;  // slabs of one batch of a workgroup's loads
 Shape gemm_shape(int M, int N, int K, int dtype) {
     Shape s;
     const int slabs = ceil_div(K, kSlab / (int)dtype_bytes(dtype));
     int rows = 128, cols = 128, fill = 512;  // fill: workgroups that keep the card busy
     s.kind = kTile128;
-    if (M <= 32) {
+    if (M <= 16 || (M <= 32 && (dtype != AFD_T_F32 || (long)N * K <= 1 << 22))) {
+        const long loads = slabs / kFewLoad > 1 ? slabs / kFewLoad : 1;
+        const bool wide = M > 16 && ceil_div(N, 32) * loads >= 256;
+        s.kind = wide ? kFew32 : kFew16;
+        rows = 32;
+        cols = wide ? 32 : 16;
+        fill = 256;
+    } else if (M <= 32) {
         s.kind = kTile32x128;
         rows = 32;
     } else if (dtype == AFD_T_F32) {
@@ -491,7 +597,7 @@ Shape gemm_shape(int M, int N, int K, int dtype) {
     int want = 1;
     if (tiles < fill) {
         want = (int)((fill + tiles - 1) / tiles);
-        const int most = slabs / (s.kind == kTile32x128 ? 2 : 4);
+        const int most = slabs / (s.kind <= kFew32 ? kFewLoad : s.kind == kTile32x128 ? 2 : 4);
         if (want > most) want = most;
         if (want < 1) want = 1;
     }
@@ -517,10 +623,16 @@ template <typename T, int TM, int TN, int WM, int WN> int launch_tile(const Gemm
     return AFD_OK;
 }
 
+template <typename T, int MT, int NT> int launch_few(const Gemm& g, hipStream_t s) {
+    hipLaunchKernelGGL((few_rows_kernel<T, MT, NT>), dim3((unsigned)g.tn, (unsigned)g.S), dim3(64 * kFewWaves), 0, s, g);
+    return AFD_OK;
+}
+
 template <typename T> int gemm_t(const Gemm& g, int kind, hipStream_t s) {
     int rc;
-    if (kind == kTile32x128) rc = launch_tile<T, 32, 128, 1, 4>(g, s);
-    else if constexpr (sizeof(T) == 4) rc = launch_tile<T, 128, 64, 2, 2>(g, s);
+    if (kind == kFew32) rc = launch_few<T, 2, 2>(g, s);
+    else if (kind == kFew16) rc = g.M <= 16 ? launch_few<T, 1, 1>(g, s) : launch_few<T, 2, 1>(g, s);
+    else if constexpr (sizeof(T) == 4) rc = kind == kTile32x128 ? launch_tile<T, 32, 128, 1, 4>(g, s) : launch_tile<T, 128, 64, 2, 2>(g, s);
     else if (kind == kTile256) rc = launch_tile<T, 256, 256, 2, 4>(g, s);
     else rc = launch_tile<T, 128, 128, 2, 2>(g, s);
     if (rc) return rc;

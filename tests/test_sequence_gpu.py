@@ -755,6 +755,13 @@ LINEAR = [
     ("bf16", 2050, 1024, 1030, "silu", "fp32", True),  # 256 x 256 tiles, ragged in both directions
     ("fp16", 4100, 520, 2056, "gelu", "fp32", False),
     ("fp32", 2000, 260, 130, "gelu", "fp32", True),
+    ("bf16", 1, 2048, 2048, "silu", "fp32", True),     # few rows: whole slabs, tails inside a slab and inside a batch, splits
+    ("bf16", 16, 1000, 515, "gelu", "same", False),
+    ("fp16", 17, 264, 33, "none", None, True),
+    ("bf16", 32, 4104, 8200, "relu", "fp32", False),   # ... 32 columns at a time
+    ("fp32", 5, 36, 1, "silu", "fp32", False),
+    ("fp32", 16, 9000, 40, "none", "fp32", False),
+    ("fp32", 31, 2052, 2100, "gelu", None, True),      # ... 32 x 128 tiles
 ]
 
 
