@@ -4,12 +4,18 @@
 // One kernel computes C[m][n] = sum_k A[m][k] B[n][k] for operands whose rows are contiguous along k: the forward as it
 // stands, dx with w transposed, dw with dz and x transposed (small passes of this file, which also take operands whose
 // rows do not start on 16-byte boundaries or do not end on them).  A workgroup owns a TM x TN tile; 128 bytes of k per row
-// are staged in LDS, double buffered: the next slab's global loads are issued before the current slab's products and
-// written to LDS behind them, one barrier per slab.  Both operands of a lane are 16-byte reads: lane l holds row l % 32 and the
-// (2 s + l / 32)-th 16 bytes of its slab, which are 8 bf16 (one 32x32x16 product) or 4 fp32 (four 32x32x2 products, whose k
-// order does not matter as long as both operands agree).  Chunks are XORed with the row, so 8 rows' reads of one chunk
-// number spread over all banks.
+// are staged in LDS, double buffered, one barrier per slab, and a slab's global loads are under way for the whole slab in
+// front of it.  Both operands of a lane are 16-byte reads: lane l holds row l % 32 and the (2 s + l / 32)-th 16 bytes of its
+// slab, which are 8 bf16 (one 32x32x16 product) or 4 fp32 (four 32x32x2 products, whose k order does not matter as long as
+// both operands agree).  Chunks are XORed with the row, so 8 rows' reads of one chunk number spread over all banks.
 // Few tiles: the k axis is split over workgroups, which leave fp32 partial tiles for a second kernel with the same epilogue.
+//
+// Bound by the matrix instructions and what keeps them waiting.  Measured, with the library's product of the same sizes in
+// brackets: bf16 8192 x 8192 x 8192 1172 (1502) TFLOP/s, 16384 x 2048 x 2048 1062 (1384), where the matrix units are busy
+// half of the time (128 KB of LDS leave one workgroup per CU, and two waves per SIMD do not cover each other's barriers);
+// fp32 16384 x 2048 x 2048 135 (147), 12928 x 1024 x 512 111 (108).  Staging 2 or 3 slabs ahead, one wave per SIMD with 128 x 128
+// each, or two workgroups of 128 x 256 per CU were not faster (1113, 958 and 937 at 4096 to 8192 cubed).  The epilogue's own
+// traffic (fp32 z out, residual in) adds 78 us to the 138 of a 16384 x 2048 x 2048 product at 4.9 TB/s and is not hidden.
 #include "seq_common.h"
 
 namespace {
@@ -85,33 +91,67 @@ template <typename T> __device__ __forceinline__ void finish_one(const Epi& e, i
     static_cast<T*>(e.out)[(size_t)m * e.ldo + n] = from_f32<T>(o);
 }
 
-// V consecutive columns n .. n + V of row m.  The pre-activation is kept in fp32 whatever the tensors' type: the bias gradient
-// is a sum of dy times its slope and an fp32 parameter's; at a z rounded to bf16 it was off by 2e-3.
-template <typename T, int V>
-__device__ __forceinline__ void finish(const Epi& e, int m, int n, int N, float (&v)[V], const float (&bias)[V]) {
+// (Compact on purpose: every workgroup walks through its epilogue once, and with the activation chosen element by element
+// and all passes unrolled it was 90 KB of code that missed the instruction cache: 9 us for a product of a single slab.)
+template <typename T> __device__ __forceinline__ void activate8(float (&v)[8], int act) {
+    if (act == kRelu) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = activate<T>(v[i], kRelu);
+    } else if (act == kSilu) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = activate<T>(v[i], kSilu);
+    } else if (act == kGelu) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = activate<T>(v[i], kGelu);
+    }
+}
+
+// Eight columns n .. n + 8 of a residual's row, asked for ahead (zeros where there is none or the row ends inside).
+template <typename T> struct Ahead { u32x4 v[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ Ahead<T> ask_residual(const Epi& e, int m, int n, int M, int N) {
+    Ahead<T> r{};
+    if (e.residual && m < M && n + 8 <= N) {
+        const T* p = static_cast<const T*>(e.residual) + (size_t)m * e.ldr + n;
+#pragma unroll
+        for (int g = 0; g < (int)sizeof(T) / 2; ++g) r.v[g] = *reinterpret_cast<const u32x4_any*>(p + g * (16 / (int)sizeof(T)));
+    }
+    return r;
+}
+
+// Eight columns of row m.  The pre-activation is kept in fp32 whatever the tensors' type: the bias gradient is a sum of dy
+// times its slope and an fp32 parameter's; at a z rounded to bf16 it was off by 2e-3.
+template <typename T>
+__device__ __forceinline__ void finish(const Epi& e, int m, int n, int N, float (&v)[8], const float (&bias)[8], const Ahead<T>& r) {
     T* out = static_cast<T*>(e.out) + (size_t)m * e.ldo + n;
-    const T* res = e.residual ? static_cast<const T*>(e.residual) + (size_t)m * e.ldr + n : nullptr;
-    float* zp = e.z ? e.z + (size_t)m * N + n : nullptr;
     constexpr int W = 16 / (int)sizeof(T);
-    if (n + V <= N) {
+    const bool whole = n + 8 <= N;
 #pragma unroll
-        for (int g = 0; g < V; g += W) {
-            float r[W], o[W];
-            if (res) load_row<T, W>(res + g, r);
+    for (int i = 0; i < 8; ++i) v[i] += bias[i];
+    if (e.z) {
+        float* z = e.z + (size_t)m * N + n;
+        if (whole) {
+            store_row<float, 4>(z, *reinterpret_cast<float(*)[4]>(&v[0]));
+            store_row<float, 4>(z + 4, *reinterpret_cast<float(*)[4]>(&v[4]));
+        } else {
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-                v[g + i] += bias[g + i];
-                o[i] = activate<T>(v[g + i], e.act);
-                if (res) o[i] += r[i];
-            }
-            store_row<T, W>(out + g, o);
+            for (int i = 0; i < 8; ++i)
+                if (n + i < N) z[i] = v[i];
         }
-        if (zp) {
+    }
+    activate8<T>(v, e.act);
+    if (whole) {
+        if (e.residual) {
+            const Pack<T, 8> k = __builtin_bit_cast(Pack<T, 8>, r);
 #pragma unroll
-            for (int g = 0; g < V; g += 4) store_row<float, 4>(zp + g, *reinterpret_cast<float(*)[4]>(&v[g]));
+            for (int i = 0; i < 8; ++i) v[i] += to_f32(k.v[i]);
         }
+#pragma unroll
+        for (int g = 0; g < 8; g += W) store_row<T, W>(out + g, *reinterpret_cast<float(*)[W]>(&v[g]));
     } else {
-        for (int i = 0; i < V && n + i < N; ++i) finish_one<T>(e, m, n + i, N, v[i] + bias[i]);
+        const T* res = static_cast<const T*>(e.residual) + (size_t)m * e.ldr + n;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (n + i < N) out[i] = from_f32<T>(e.residual ? v[i] + to_f32(res[i]) : v[i]);
     }
 }
 
@@ -355,7 +395,12 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(const Gemm g) {
     constexpr int LPR = WC / 8, RPP = 64 / LPR;  // lanes per row, rows per pass
     const int col = (lane % LPR) * 8, n = n0 + wn * WC + col;
     float bias[8];
-    if (g.S == 1) load_bias<T, 8>(g.e, n, g.N, bias);
+    auto row_of = [&](int i, int r) { return m0 + wm * (TM / WM) + i * 32 + r; };
+    Ahead<T> next{};
+    if (g.S == 1) {
+        load_bias<T, 8>(g.e, n, g.N, bias);
+        next = ask_residual<T>(g.e, row_of(0, lane / LPR), n, g.M, g.N);
+    }
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
 #pragma unroll
@@ -363,25 +408,31 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(const Gemm g) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) tile[((r & 3) + 8 * (r >> 2) + 4 * half) * kPitch + j * 32 + l31] = acc[i][j][r];
         __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int p = 0; p < 32; p += RPP) {
-            const int row = p + lane / LPR, m = m0 + wm * (TM / WM) + i * 32 + row;
-            float v[8];
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + row * kPitch + col);
-            const f32x4 hi = *reinterpret_cast<const f32x4*>(tile + row * kPitch + col + 4);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                v[c] = lo[c];
-                v[4 + c] = hi[c];
+        if (g.S > 1) {  // 16 bytes per lane, in the order of memory (ldp is a multiple of 8)
+            constexpr int L4 = WC / 4;
+            const int c4 = (lane % L4) * 4, n4 = n0 + wn * WC + c4;
+            float* dst = g.part + ((size_t)blockIdx.y * g.M + row_of(i, lane / L4)) * g.ldp + n4;
+#pragma unroll 4
+            for (int p = lane / L4; p < 32; p += 64 / L4) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(tile + p * kPitch + c4);
+                if (row_of(i, p) < g.M && n4 < g.N) *reinterpret_cast<f32x4*>(dst) = v;
+                dst += (64 / L4) * g.ldp;
             }
-            if (m < g.M && n < g.N) {
-                if (g.S > 1) {  // (ldp is a multiple of 8)
-                    float* dst = g.part + ((size_t)blockIdx.y * g.M + m) * g.ldp + n;
-                    *reinterpret_cast<f32x4*>(dst) = lo;
-                    *reinterpret_cast<f32x4*>(dst + 4) = hi;
-                } else {
-                    finish<T, 8>(g.e, m, n, g.N, v, bias);
+        } else {
+#pragma unroll 1
+            for (int p = lane / LPR; p < 32; p += RPP) {
+                const int m = row_of(i, p);
+                float v[8];
+                const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + p * kPitch + col);
+                const f32x4 hi = *reinterpret_cast<const f32x4*>(tile + p * kPitch + col + 4);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    v[c] = lo[c];
+                    v[4 + c] = hi[c];
                 }
+                const Ahead<T> res = next;
+                next = ask_residual<T>(g.e, p + RPP < 32 ? m + RPP : row_of(i + 1, lane / LPR), n, g.M, g.N);
+                if (m < g.M && n < g.N) finish<T>(g.e, m, n, g.N, v, bias, res);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -495,7 +546,7 @@ template <typename T> __global__ void __launch_bounds__(256) join_kernel(const G
                 v[4 + c] += hi[c];
             }
         }
-        finish<T, 8>(g.e, m, n, g.N, v, bias);
+        finish<T>(g.e, m, n, g.N, v, bias, ask_residual<T>(g.e, m, n, g.M, g.N));
     }
 }
 
@@ -546,13 +597,25 @@ __global__ void __launch_bounds__(256) turn_kernel(const T* __restrict__ src, lo
     }
 }
 
-// dst[r][0 .. ldd) = src[r][0 .. C), zeros behind it
-template <typename T>
-__global__ void __launch_bounds__(256) pad_kernel(const T* __restrict__ src, long lds_, int R, int C, T* __restrict__ dst, long ldd) {
-    const long all = (long)R * ldd;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
-        const long r = i / ldd, c = i - r * ldd;
-        dst[i] = c < C ? src[(size_t)r * lds_ + c] : (T)0.f;
+// Rows of C elements copied to rows of ldd (whole 16-byte chunks, zeros behind C): one or two matrices in one launch, a wave
+// per row.
+struct PadJob {
+    const void* src;
+    void* dst;
+    long ld;
+    int rows;
+};
+template <typename T> __global__ void __launch_bounds__(256) pad_kernel(const PadJob a, const PadJob b, int C, int ldd) {
+    const PadJob j = blockIdx.y ? b : a;
+    const int lane8 = (threadIdx.x & 63) * 8;
+    for (long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6); r < j.rows; r += (long)gridDim.x * 4) {
+        const T* src = static_cast<const T*>(j.src) + (size_t)r * j.ld;
+        T* dst = static_cast<T*>(j.dst) + (size_t)r * ldd;
+        for (int c = lane8; c < ldd; c += 512) {
+            float v[8];
+            load8<T>(src + c, C - c, v);
+            store8<T>(dst + c, ldd - c, v);
+        }
     }
 }
 
@@ -603,12 +666,18 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ dy, long 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 long pad_to(long n, long k) { return (n + k - 1) / k * k; }
 
-// Tiles by what they took (us) for the three products of a training step, forward / dx / dw:
-//   fp32 12928 x 512 x 1024: 128 x 128 166 / 152 / 129, 64 x 64 148 / 150 / 138, 128 x 64 144 / 139 / 132 (three workgroups
-//   per CU, and 1616 tiles where 808 leave a fifth of the card idle at the end; matrix instructions are busy 60 % of it);
-//   bf16 16384 x 2048 x 2048: 256 x 256 220 / 171 / 162, 128 x 128 263 / 211 / 186 (half the operand traffic per product).
+// Tiles by what they took, us (M x N x K; `/` separates the tiles or splits compared).
+//   256 x 256, 16-bit, from 16 slabs of work per CU on: bf16 16384 x 2048 x 2048 and its two gradients 220 171 162, with
+//   128 x 128 263 211 186 (half the operand traffic per product).
+//   Below, the largest tile that leaves 1.5 workgroups per CU (of 128 x 128, 128 x 64, 64 x 64), splits of a long k counted:
+//   bf16 12928 x 512 x 1024 23 / 27 / 28, 2048 x 2048 x 2048 34 / 27 / 31, 4096 x 512 x 512 10.3 / 7.9 / 7.4, 1000 x 1000 x
+//   1000 13.6 / 10.4 / 8.0; fp32 (no 128 x 128: a fifth of the card idles at the end) 2048 x 2048 x 2048 - / 136 / 159,
+//   300 x 300 x 300 - / 15.2 / 9.6.
+//   k is split until every CU has a workgroup, into 4 slabs at least: the partial tiles cost their traffic and a second
+//   launch, and splitting on for two workgroups per CU took 14.2 against 8.3 at 1000 x 1000 x 1000 and 39 against 24 at
+//   12928 x 512 x 1024; but splits of 32 slabs and more are worth it, 33 against 46 at 1024 x 512 x 12928.
 // Up to 32 rows the weights are what is read (us here, and with one 32 x 128 tile row split along k and joined):
-//   bf16 1 / 16 / 32 x 2048 x 2048: 4.9 / 6.2 / 8.1, 8.9 / 10.3 / 10.8; 32 x 8192 x 2048 (K): 12.9 with 32 columns per workgroup,
+//   bf16 1 / 16 / 32 x 2048 x 2048: 4.9 / 6.2 / 8.1, 8.9 / 10.3 / 10.8; 32 x 8192 x 2048: 12.9 with 32 columns per workgroup,
 //   15.8 with 16, 13.8; fp32 1 / 16 x 2048 x 2048: 7.9 / 11.1, 12.5 / 13.8; 4 x 10000 x 1024: 11.7 with 16 columns, 16.8 with
 //   32, 17.0; but 32 rows of fp32 re-read x too often for large weights: 29 against 21.6 at 8192 x 2048, 13.8 against 16.2 at
 //   2048 x 2048.
@@ -617,41 +686,51 @@ struct Shape {
     int tm, tn, S, ksplit;
     size_t part;
 };
-enum { kFew16, kFew32, kTile32x128, kTile128x64, kTile128, kTile256 };
+enum { kFew16, kFew32, kTile32x128, kTile64, kTile128x64, kTile128, kTile256 };
+constexpr int kLong = 32;                         // slabs of a split that its workgroup's prologue and the joining are small against
 constexpr int kFewLoad = kFewWaves * kFewBatch;  // slabs of one batch of a workgroup's loads
 Shape gemm_shape(int M, int N, int K, int dtype) {
     Shape s;
     const int slabs = ceil_div(K, kSlab / (int)dtype_bytes(dtype));
-    int rows = 128, cols = 128, fill = 512;  // fill: workgroups that keep the card busy
-    s.kind = kTile128;
+    int rows = 64, cols = 64, least = 4, fill = 1024;  // slabs of a split at least; workgroups that a long k is split into
+    const int longs = slabs / kLong > 1 ? slabs / kLong : 1;
+    s.kind = kTile64;
+    auto tiles = [&](int r, int c) { return (long)ceil_div(M, r) * ceil_div(N, c); };
     if (M <= 16 || (M <= 32 && (dtype != AFD_T_F32 || (long)N * K <= 1 << 22))) {
         const long loads = slabs / kFewLoad > 1 ? slabs / kFewLoad : 1;
         const bool wide = M > 16 && ceil_div(N, 32) * loads >= 256;
         s.kind = wide ? kFew32 : kFew16;
         rows = 32;
         cols = wide ? 32 : 16;
-        fill = 256;
+        least = kFewLoad;
     } else if (M <= 32) {
         s.kind = kTile32x128;
         rows = 32;
-    } else if (dtype == AFD_T_F32) {
-        s.kind = kTile128x64;
-        cols = 64;
-        fill = 768;
-    } else if ((long)ceil_div(M, 256) * ceil_div(N, 256) * slabs >= 256 * 16) {  // 16 slabs for every CU
+        cols = 128;
+        least = 2;
+    } else if (dtype != AFD_T_F32 && tiles(256, 256) * slabs >= 256 * 16) {  // 16 slabs for every CU
         s.kind = kTile256;
         rows = cols = fill = 256;
+    } else if (dtype != AFD_T_F32 && M > 64 && N > 64 && tiles(128, 128) * longs >= 400) {
+        s.kind = kTile128;
+        rows = cols = 128;
+        fill = 512;
+    } else if (M > 64 && tiles(128, 64) * longs >= 400) {
+        s.kind = kTile128x64;
+        rows = 128;
+        fill = 768;
     }
     s.tm = ceil_div(M, rows);
     s.tn = ceil_div(N, cols);
-    const long tiles = (long)s.tm * s.tn;
-    int want = 1;
-    if (tiles < fill) {
-        want = (int)((fill + tiles - 1) / tiles);
-        const int most = slabs / (s.kind <= kFew32 ? kFewLoad : s.kind == kTile32x128 ? 2 : 4);
-        if (want > most) want = most;
-        if (want < 1) want = 1;
-    }
+    // k is split for a workgroup on every CU, and for all that fit where the splits stay long
+    const long all = (long)s.tm * s.tn;
+    auto split = [&](long to, int slabs_each) {
+        const long want = (to + all - 1) / all, most = slabs / slabs_each;
+        return (int)(want < most ? want : most);
+    };
+    int want = split(256, least);
+    if (want < split(fill, kLong)) want = split(fill, kLong);
+    if (want < 1) want = 1;
     s.ksplit = ceil_div(slabs, want);
     s.S = ceil_div(slabs, s.ksplit);
     s.part = s.S > 1 ? align256((size_t)s.S * M * pad_to(N, 8) * 4) : 0;
@@ -683,7 +762,9 @@ template <typename T> int gemm_t(const Gemm& g, int kind, hipStream_t s) {
     int rc;
     if (kind == kFew32) rc = launch_few<T, 2, 2>(g, s);
     else if (kind == kFew16) rc = g.M <= 16 ? launch_few<T, 1, 1>(g, s) : launch_few<T, 2, 1>(g, s);
-    else if constexpr (sizeof(T) == 4) rc = kind == kTile32x128 ? launch_tile<T, 32, 128, 1, 4>(g, s) : launch_tile<T, 128, 64, 2, 2>(g, s);
+    else if (kind == kTile64) rc = launch_tile<T, 64, 64, 2, 2>(g, s);
+    else if (kind == kTile128x64) rc = launch_tile<T, 128, 64, 2, 2>(g, s);
+    else if constexpr (sizeof(T) == 4) rc = launch_tile<T, 32, 128, 1, 4>(g, s);
     else if (kind == kTile256) rc = launch_tile<T, 256, 256, 2, 4>(g, s);
     else rc = launch_tile<T, 128, 128, 2, 2>(g, s);
     if (rc) return rc;
@@ -714,13 +795,13 @@ template <typename T> int turn_t(const void* src, long ld, int R, int C, void* d
 int turn(const void* src, long ld, int R, int C, void* dst, long ldd, int dtype, hipStream_t s) {
     return dtype == AFD_T_F32 ? turn_t<float>(src, ld, R, C, dst, ldd, s) : turn_t<bf16_t>(src, ld, R, C, dst, ldd, s);
 }
-int pad(const void* src, long ld, int R, int C, void* dst, long ldd, int dtype, hipStream_t s) {
-    const long grid = ((long)R * ldd + 255) / 256;
-    const dim3 d((unsigned)(grid < 65536 ? grid : 65536));
-    if (dtype == AFD_T_F32)
-        hipLaunchKernelGGL(pad_kernel<float>, d, dim3(256), 0, s, static_cast<const float*>(src), ld, R, C, static_cast<float*>(dst), ldd);
-    else
-        hipLaunchKernelGGL(pad_kernel<bf16_t>, d, dim3(256), 0, s, static_cast<const bf16_t*>(src), ld, R, C, static_cast<bf16_t*>(dst), ldd);
+int pad(const PadJob* jobs, int n, int C, long ldd, int dtype, hipStream_t s) {
+    const PadJob &a = jobs[0], &b = jobs[n - 1];
+    const long most = a.rows > b.rows ? a.rows : b.rows, grid = (most + 3) / 4;
+    const dim3 d((unsigned)(grid < 65536 ? grid : 65536), (unsigned)n);
+    if (dtype == AFD_T_F32) hipLaunchKernelGGL(pad_kernel<float>, d, dim3(256), 0, s, a, b, C, (int)ldd);
+    else if (dtype == AFD_T_BF16) hipLaunchKernelGGL(pad_kernel<bf16_t>, d, dim3(256), 0, s, a, b, C, (int)ldd);
+    else hipLaunchKernelGGL(pad_kernel<f16_t>, d, dim3(256), 0, s, a, b, C, (int)ldd);
     return check_launch("pad_kernel");
 }
 
@@ -772,18 +853,20 @@ extern "C" int afd_linear_forward(const void* x, long long ldx, const void* w, l
     hipStream_t s = static_cast<hipStream_t>(stream);
     ScopedTiming timing(AFD_K_SEQUENCE, 2.0 * (double)M * N * K, s);
     Arena ar{static_cast<char*>(ws), 0};
+    PadJob jobs[2];
+    int n = 0;
     if (!dx) {
-        void* c = ar.take((size_t)M * kp * e);
-        if (int rc = pad(x, ldx, (int)M, K, c, kp, dtype, s)) return rc;
-        x = c;
+        jobs[n++] = {x, ar.take((size_t)M * kp * e), (long)ldx, (int)M};
+        x = jobs[n - 1].dst;
         ldx = kp;
     }
     if (!dw) {
-        void* c = ar.take((size_t)N * kp * e);
-        if (int rc = pad(w, ldw, N, K, c, kp, dtype, s)) return rc;
-        w = c;
+        jobs[n++] = {w, ar.take((size_t)N * kp * e), (long)ldw, N};
+        w = jobs[n - 1].dst;
         ldw = kp;
     }
+    if (n > 0)
+        if (int rc = pad(jobs, n, K, kp, dtype, s)) return rc;
     Epi ep{bias, bias_f32, residual, ldr, y, N, z, act};
     return gemm(x, ldx, w, ldw, (int)M, N, (int)kp, ep, dtype, reinterpret_cast<float*>(ar.base + ar.at), s);
 }

@@ -762,6 +762,11 @@ LINEAR = [
     ("fp32", 5, 36, 1, "silu", "fp32", False),
     ("fp32", 16, 9000, 40, "none", "fp32", False),
     ("fp32", 31, 2052, 2100, "gelu", None, True),      # ... 32 x 128 tiles
+    ("bf16", 3330, 130, 2050, "silu", "same", True),   # 128 x 128 tiles, the gradients' k long enough to be split
+    ("fp16", 1700, 1024, 2000, "gelu", "fp32", False), # 128 x 64
+    ("fp32", 1700, 96, 2000, "silu", "fp32", True),
+    ("bf16", 40, 36, 700, "none", "fp32", True),       # 64 x 64
+    ("bf16", 33, 9001, 65, "silu", "fp32", True),      # ... split, rows copied
 ]
 
 
