@@ -574,16 +574,22 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int left, con
     }
 }
 
-// dst[c][r] = src[r][c] for R x C elements, rows of dst padded with zeros to ldd (a multiple of 16 bytes).
-template <typename T>
-__global__ void __launch_bounds__(256) turn_kernel(const T* __restrict__ src, long ld, int R, int C, T* __restrict__ dst, long ldd) {
-    __shared__ float t[64][65];
-    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+// dst[c][r] = src[r][c] for R x C elements, rows of dst padded with zeros to ldd (a multiple of 16 bytes); `tiles` along r.
+struct TurnJob {
+    const void* src;
+    void* dst;
+    long ld, ldd;
+    int R, C, tiles, groups;  // groups: workgroups, 0: nothing to turn
+};
+template <typename T> __device__ __forceinline__ void turn_tile(const TurnJob& j, int id, float (&t)[64][65]) {
+    const int r0 = id % j.tiles * 64, c0 = id / j.tiles * 64;
     const int x8 = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
+    const T* src = static_cast<const T*>(j.src);
+    T* dst = static_cast<T*>(j.dst);
 #pragma unroll
     for (int i = y; i < 64; i += 32) {
         float v[8];
-        load8<T>(src + (size_t)min(r0 + i, R - 1) * ld + c0 + x8, r0 + i < R ? C - c0 - x8 : 0, v);
+        load8<T>(src + (size_t)min(r0 + i, j.R - 1) * j.ld + c0 + x8, r0 + i < j.R ? j.C - c0 - x8 : 0, v);
 #pragma unroll
         for (int k = 0; k < 8; ++k) t[i][x8 + k] = v[k];
     }
@@ -593,7 +599,7 @@ __global__ void __launch_bounds__(256) turn_kernel(const T* __restrict__ src, lo
         float v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = t[x8 + k][i];
-        if (c0 + i < C) store8<T>(dst + (size_t)(c0 + i) * ldd + r0 + x8, (int)min(ldd - r0 - x8, 8L), v);
+        if (c0 + i < j.C) store8<T>(dst + (size_t)(c0 + i) * j.ldd + r0 + x8, (int)min(j.ldd - r0 - x8, 8L), v);
     }
 }
 
@@ -621,45 +627,62 @@ template <typename T> __global__ void __launch_bounds__(256) pad_kernel(const Pa
 
 // dz = dy act'(z) as rows (ldz, zeros behind N) and turned (ldt, zeros behind M), and its column sums over the tile's rows;
 // NULL: not wanted.
-template <typename T>
-__global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ dy, long ldy, const float* __restrict__ z, int act, int M, int N,
-                                                 T* __restrict__ dz, long ldz, T* __restrict__ turned, long ldt,
-                                                 float* __restrict__ sums) {
-    __shared__ float t[64][65];
-    const int m0 = blockIdx.x * 64, n0 = blockIdx.y * 64;
+struct DzJob {
+    const void* dy;
+    const float* z;
+    void *dz, *turned;
+    float* sums;
+    long ldy, ldz, ldt;
+    int act, M, N, tiles, groups;
+};
+template <typename T> __device__ __forceinline__ void dz_tile(const DzJob& j, int id, float (&t)[64][65], float (&red)[4][64]) {
+    const int m0 = id % j.tiles * 64, n0 = id / j.tiles * 64;
     const int x8 = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
+    const T* dy = static_cast<const T*>(j.dy);
+    T *dz = static_cast<T*>(j.dz), *turned = static_cast<T*>(j.turned);
 #pragma unroll
     for (int i = y; i < 64; i += 32) {
-        const int m = m0 + i, n = n0 + x8, left = m < M ? N - n : 0;
+        const int m = m0 + i, n = n0 + x8, left = m < j.M ? j.N - n : 0;
         float v[8], zv[8];
-        load8<T>(dy + (size_t)min(m, M - 1) * ldy + n, left, v);
-        if (act != kNone) {
-            load8<float>(z + (size_t)min(m, M - 1) * N + n, left, zv);
+        load8<T>(dy + (size_t)min(m, j.M - 1) * j.ldy + n, left, v);
+        if (j.act != kNone) {
+            load8<float>(j.z + (size_t)min(m, j.M - 1) * j.N + n, left, zv);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = k < left ? v[k] * activate_slope<T>(zv[k], act) : 0.f;
+            for (int k = 0; k < 8; ++k) v[k] = k < left ? v[k] * activate_slope<T>(zv[k], j.act) : 0.f;
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) t[i][x8 + k] = v[k];
-        if (dz && m < M) store8<T>(dz + (size_t)m * ldz + n, (int)min(ldz - n, 8L), v);
+        if (dz && m < j.M) store8<T>(dz + (size_t)m * j.ldz + n, (int)min(j.ldz - n, 8L), v);
     }
     __syncthreads();
+    if (turned) {
 #pragma unroll
-    for (int i = y; i < 64; i += 32) {
-        float v[8];
+        for (int i = y; i < 64; i += 32) {
+            float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = t[x8 + k][i];
-        if (turned && n0 + i < N) store8<T>(turned + (size_t)(n0 + i) * ldt + m0 + x8, (int)min(ldt - m0 - x8, 8L), v);
+            for (int k = 0; k < 8; ++k) v[k] = t[x8 + k][i];
+            if (n0 + i < j.N) store8<T>(turned + (size_t)(n0 + i) * j.ldt + m0 + x8, (int)min(j.ldt - m0 - x8, 8L), v);
+        }
     }
-    if (!sums) return;
-    __shared__ float red[4][64];
+    if (!j.sums) return;
     const int col = threadIdx.x & 63, part = threadIdx.x >> 6;
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s += t[part * 16 + i][col];
     red[part][col] = s;
     __syncthreads();
-    if (part == 0 && n0 + col < N)
-        sums[(size_t)blockIdx.x * N + n0 + col] = (red[0][col] + red[1][col]) + (red[2][col] + red[3][col]);
+    if (part == 0 && n0 + col < j.N)
+        j.sums[(size_t)(id % j.tiles) * j.N + n0 + col] = (red[0][col] + red[1][col]) + (red[2][col] + red[3][col]);
+}
+
+// What the two products of a backward pass read, in one launch: the workgroups share themselves out over the three jobs.
+template <typename T> __global__ void __launch_bounds__(256) prepare_kernel(const DzJob d, const TurnJob w, const TurnJob x) {
+    __shared__ float t[64][65];
+    __shared__ float red[4][64];
+    const int id = blockIdx.x;
+    if (id < d.groups) dz_tile<T>(d, id, t, red);
+    else if (id < d.groups + w.groups) turn_tile<T>(w, id - d.groups, t);
+    else turn_tile<T>(x, id - d.groups - w.groups, t);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
@@ -786,14 +809,9 @@ int gemm(const void* a, long lda, const void* b, long ldb, int M, int N, int K, 
     return gemm_t<f16_t>(g, q.kind, s);
 }
 
-template <typename T> int turn_t(const void* src, long ld, int R, int C, void* dst, long ldd, hipStream_t s) {
-    hipLaunchKernelGGL(turn_kernel<T>, dim3((unsigned)ceil_div(ldd, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, s,
-                       static_cast<const T*>(src), ld, R, C, static_cast<T*>(dst), ldd);
-    return check_launch("turn_kernel");
-}
-// (types of one size move alike)
-int turn(const void* src, long ld, int R, int C, void* dst, long ldd, int dtype, hipStream_t s) {
-    return dtype == AFD_T_F32 ? turn_t<float>(src, ld, R, C, dst, ldd, s) : turn_t<bf16_t>(src, ld, R, C, dst, ldd, s);
+TurnJob turn_job(const void* src, long ld, int R, int C, void* dst, long ldd) {
+    const int tiles = ceil_div(ldd, 64);
+    return {src, dst, ld, ldd, R, C, tiles, tiles * ceil_div(C, 64)};
 }
 int pad(const PadJob* jobs, int n, int C, long ldd, int dtype, hipStream_t s) {
     const PadJob &a = jobs[0], &b = jobs[n - 1];
@@ -892,15 +910,6 @@ BackPlan back_plan(long M, int N, int K, int dtype) {
     b.total = b.dz + b.dzt + b.xt + b.wt + b.sums + b.part;
     return b;
 }
-template <typename T>
-int dz_t(const void* dy, long ldy, const float* z, int act, int M, int N, void* dz, long ldz, void* t, long ldt, float* sums, hipStream_t s) {
-    const long rows = ldt > M ? ldt : M;
-    const long cols = dz && ldz > N ? ldz : N;
-    hipLaunchKernelGGL(dz_kernel<T>, dim3((unsigned)ceil_div(rows, 64), (unsigned)ceil_div(cols, 64)), dim3(256), 0, s,
-                       static_cast<const T*>(dy), ldy, z, act, M, N, static_cast<T*>(dz), ldz,
-                       static_cast<T*>(t), ldt, sums);
-    return check_launch("dz_kernel");
-}
 }  // namespace
 
 extern "C" size_t afd_linear_backward_workspace_bytes(long long M, int N, int K, int dtype) {
@@ -915,6 +924,8 @@ extern "C" int afd_linear_backward(const void* x, long long ldx, const void* w, 
     if (int rc = check("linear backward", M, N, K, act, dtype)) return rc;
     // (a tile's rows of the turned operands have to be within a 32-bit offset of each other)
     if (M > 8000000) return fail(AFD_ERR_UNSUPPORTED, "linear backward: M=%lld, at most 8000000 rows", M);
+    const long mt = ceil_div(M + 8, 64), nt = ceil_div(N + 8, 64), kt = ceil_div(K, 64);
+    if (mt * nt + mt * kt + nt * kt > kMaxGroups) return fail(AFD_ERR_UNSUPPORTED, "linear backward: M=%lld N=%d K=%d", M, N, K);
     const BackPlan b = back_plan(M, N, K, dtype);
     if (!ws || ws_bytes < b.total)
         return fail(AFD_ERR_WORKSPACE, "linear backward: workspace of %zu bytes, %zu needed", ws_bytes, b.total);
@@ -929,15 +940,18 @@ extern "C" int afd_linear_backward(const void* x, long long ldx, const void* w, 
     float* part = reinterpret_cast<float*>(ar.base + ar.at);
     // without an activation dy is dz, and can be read as it is where its rows allow
     const bool rows = act != kNone || !direct(dy, ldy, N, dtype);
-    void* rz = dx && rows ? dz : nullptr;
-    void* rt = dw ? dzt : nullptr;
-    float* rs = dbias ? sums : nullptr;
-    if (rz || rt || rs) {
-        const int rc = dtype == AFD_T_F32 ? dz_t<float>(dy, ldy, z, act, (int)M, N, rz, b.np, rt, b.mp, rs, s)
-                       : dtype == AFD_T_BF16 ? dz_t<bf16_t>(dy, ldy, z, act, (int)M, N, rz, b.np, rt, b.mp, rs, s)
-                                             : dz_t<f16_t>(dy, ldy, z, act, (int)M, N, rz, b.np, rt, b.mp, rs, s);
-        if (rc) return rc;
+    DzJob jd{dy, z, dx && rows ? dz : nullptr, dw ? dzt : nullptr, dbias ? sums : nullptr, ldy, b.np, b.mp, act, (int)M, N, 0, 0};
+    if (jd.dz || jd.turned || jd.sums) {
+        jd.tiles = ceil_div(b.mp, 64);
+        jd.groups = jd.tiles * ceil_div(b.np, 64);
     }
+    const TurnJob jw = dx ? turn_job(w, ldw, N, K, wt, b.np) : TurnJob{}, jx = dw ? turn_job(x, ldx, (int)M, K, xt, b.mp) : TurnJob{};
+    const dim3 grid((unsigned)(jd.groups + jw.groups + jx.groups));
+    if (grid.x == 0) return AFD_OK;
+    if (dtype == AFD_T_F32) hipLaunchKernelGGL(prepare_kernel<float>, grid, dim3(256), 0, s, jd, jw, jx);
+    else if (dtype == AFD_T_BF16) hipLaunchKernelGGL(prepare_kernel<bf16_t>, grid, dim3(256), 0, s, jd, jw, jx);
+    else hipLaunchKernelGGL(prepare_kernel<f16_t>, grid, dim3(256), 0, s, jd, jw, jx);
+    if (int rc = check_launch("prepare_kernel")) return rc;
     if (dbias) {
         ColumnOuts o{};
         o.n = 1;
@@ -945,12 +959,10 @@ extern "C" int afd_linear_backward(const void* x, long long ldx, const void* w, 
         if (int r = launch_column_sums(sums, ceil_div(b.mp, 64), N, o, s)) return r;
     }
     if (dx) {
-        if (int r = turn(w, ldw, N, K, wt, b.np, dtype, s)) return r;
         Epi e{nullptr, 0, nullptr, 0, dx, K, nullptr, kNone};
         if (int r = gemm(rows ? dz : dy, rows ? b.np : ldy, wt, b.np, (int)M, K, (int)b.np, e, dtype, part, s)) return r;
     }
     if (dw) {
-        if (int r = turn(x, ldx, (int)M, K, xt, b.mp, dtype, s)) return r;
         Epi e{nullptr, 0, nullptr, 0, dw, K, nullptr, kNone};
         if (int r = gemm(dzt, b.mp, xt, b.mp, N, K, (int)b.mp, e, dtype, part, s)) return r;
     }
