@@ -2,8 +2,8 @@
 // bf16 and fp16 (32x32x16, sums in fp32).
 //
 // One kernel computes C[m][n] = sum_k A[m][k] B[n][k] for operands whose rows are contiguous along k: the forward as it
-// stands, dx with w transposed, dw with dz and x transposed (small passes of this file, which also take operands whose
-// rows do not start on 16-byte boundaries or do not end on them).  A workgroup owns a TM x TN tile; 128 bytes of k per row
+// stands, dx with w transposed, dw with dz and x transposed (prepare_kernel; operands of the forward whose rows do not start
+// or end on 16-byte boundaries are copied by pad_kernel).  A workgroup owns a TM x TN tile; 128 bytes of k per row
 // are staged in LDS, double buffered, one barrier per slab, and a slab's global loads are under way for the whole slab in
 // front of it.  Both operands of a lane are 16-byte reads: lane l holds row l % 32 and the (2 s + l / 32)-th 16 bytes of its
 // slab, which are 8 bf16 (one 32x32x16 product) or 4 fp32 (four 32x32x2 products, whose k order does not matter as long as
@@ -676,6 +676,7 @@ template <typename T> __device__ __forceinline__ void dz_tile(const DzJob& j, in
 }
 
 // What the two products of a backward pass read, in one launch: the workgroups share themselves out over the three jobs.
+// Bound by memory: 485 MB in 93 us (5.2 TB/s) at 16384 x 2048 x 2048 bf16 with an activation; three launches took 102.
 template <typename T> __global__ void __launch_bounds__(256) prepare_kernel(const DzJob d, const TurnJob w, const TurnJob x) {
     __shared__ float t[64][65];
     __shared__ float red[4][64];
