@@ -14,8 +14,9 @@
 // brackets: bf16 8192 x 8192 x 8192 1172 (1502) TFLOP/s, 16384 x 2048 x 2048 1062 (1384), where the matrix units are busy
 // half of the time (128 KB of LDS leave one workgroup per CU, and two waves per SIMD do not cover each other's barriers);
 // fp32 16384 x 2048 x 2048 135 (147), 12928 x 1024 x 512 111 (108).  Staging 2 or 3 slabs ahead, one wave per SIMD with 128 x 128
-// each, or two workgroups of 128 x 256 per CU were not faster (1113, 958 and 937 at 4096 to 8192 cubed).  The epilogue's own
-// traffic (fp32 z out, residual in) adds 78 us to the 138 of a 16384 x 2048 x 2048 product at 4.9 TB/s and is not hidden.
+// each, or two workgroups of 128 x 256 per CU were not faster (1113, 958 and 937 at 4096 to 8192 cubed).  A forward with
+// GELU, residual and the fp32 z takes 216 us at 16384 x 2048 x 2048, its input gradient 155: 201 MB more to move and 24 us of
+// arithmetic, which no other workgroup of the CU covers.
 #include "seq_common.h"
 
 namespace {
