@@ -658,6 +658,53 @@ def test_two_training_passes_and_a_clip_in_graphs():
             assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
 
 
+def test_prompts_in_a_graph_with_changing_lengths():
+    """Ragged prompts whose time axis is split, and projections of a few and of many rows: every replay is the eager result."""
+    t = _scan_inputs(43, "bf16", 3, 700, 40, 16)
+    c = _conv_inputs(43, "bf16", 3, 700, 40, 4, True, True)
+    g = torch.Generator().manual_seed(43)
+    w, b = _rnd(g, 40, 40, scale=0.2, dtype=torch.bfloat16), _rnd(g, 40)
+    lengths = torch.tensor([700, 1, 0], device="cuda")
+
+    def run():
+        h, cs = ops.causal_conv(ops.linear(c["x"], w, b), c["w"], c["b"], "silu", state=c["state"], lengths=lengths,
+                                return_state=True)
+        y, ss = ops.state_scan(**dict(t, x=h), softplus=True, lengths=lengths, return_state=True)
+        return [y, cs, ss, ops.linear(y[:, 0], w, b, "gelu")]
+
+    graph, outs = _capture(run)
+    for turn in range(4):
+        lengths.copy_(torch.tensor([[700, 1, 0], [0, 699, 128], [16, 700, 700], [5, 129, 640]][turn]))
+        c["x"].mul_(1.25)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        assert all(torch.equal(a, e) for a, e in zip(got, run())), turn
+        torch.cuda.synchronize()
+
+
+def test_projections_on_two_streams_at_once():
+    g = torch.Generator().manual_seed(44)
+    sets = [[_rnd(g, m, 264, dtype=torch.bfloat16).requires_grad_(True), _rnd(g, 130, 264, dtype=torch.bfloat16).requires_grad_(True),
+             _rnd(g, 130).requires_grad_(True)] for m in (9, 2000)]
+
+    def both(v):
+        y = ops.linear(*v, "silu")
+        return [y, *torch.autograd.grad(y, v, torch.ones_like(y))]
+
+    want = [both(v) for v in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = both(sets[i])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 # ---- the operators together --------------------------------------------------------------------------------------------
 def _layer(t, c, x, lengths=None, states=(None, None)):
     h, cs = ops.causal_conv(x, c["w"], c["b"], "silu", state=states[0], lengths=lengths, return_state=True)
