@@ -1547,10 +1547,35 @@ def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _near_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """`_rows`, with the rows at most 2^24 elements apart (the scan's lanes reach 16 rows with 32-bit offsets)."""
-    t = _rows(t)
-    return t if t is None or t.stride(1) <= 1 << 24 else t.contiguous()
+def _token_rows(tensors):
+    """[B, L, D] tensors as the scan's lanes reach them -- a contiguous last axis, rows at most 2^24 elements apart (16 rows
+    are within 32-bit offsets) -- and their (batch, row) strides."""
+    out, strides = [], []
+    for t in tensors:
+        if t is None:
+            strides += (0, 0)
+        else:
+            s = t.stride()
+            if (s[2] != 1 and t.shape[2] > 1) or s[1] > 1 << 24:
+                t = t.contiguous()
+                s = t.stride()
+            strides += s[:2]
+        out.append(t)
+    return out, strides
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _first_order(backward):
+    """`once_differentiable`, whose two mode switches cost as much as a launch, where a second derivative may be asked for."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -1621,7 +1646,7 @@ def _conv_check(what: str, x, w, b, activation, ndim: int):
 def _conv_forward(x, w, b, state, lengths, act, return_state):
     bsz, steps, d = x.shape
     taps = w.shape[1]
-    y = torch.empty((bsz, steps, d), dtype=x.dtype, device=x.device)
+    y = _like(x)
     state_out = torch.empty((bsz, taps - 1, d), dtype=x.dtype, device=x.device) if return_state else None
     if y.numel() > 0:
         with _OnDevice(x) as stream:
@@ -1643,7 +1668,7 @@ class _CausalConv(torch.autograd.Function):
         return _conv_forward(x, w, b, state, lengths, act, return_state)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dy, dstate_out):
         x, w, b, state, lengths = ctx.saved_tensors
         bsz, steps, d = x.shape
@@ -1657,10 +1682,9 @@ class _CausalConv(torch.autograd.Function):
                     None, None, None)
         dy = _rows(dy) if dy is not None else torch.zeros_like(x)
         dstate_out = _dense(dstate_out)
-        dx = torch.empty((bsz, steps, d), dtype=x.dtype, device=x.device)
-        dw = torch.empty_like(w)
-        db = torch.empty_like(b) if b is not None else None
-        dstate = torch.empty_like(state) if need[3] else None
+        dx, dw = _like(x), _like(w)
+        db = _like(b) if b is not None else None
+        dstate = _like(state) if need[3] else None
         with _OnDevice(x) as stream:
             lib = _lib()
             nbytes = lib.afd_causal_conv_backward_workspace_bytes(bsz, steps, d, taps)
@@ -1734,17 +1758,15 @@ def _scan_check(what: str, x, dt, a, b, c, d, gate, dt_bias, state, ndim: int) -
     _seq_check(what, "state", state, (x.shape[0], chans, n), torch.float32, device)
 
 
-def _scan_strides(tensors, axes):
-    out = [t.stride(i) if t is not None else 0 for t in tensors for i in axes]
-    return (_native.c_l * len(out))(*out)
+_Strides5, _Strides10, _Strides12 = (_native.c_l * n for n in (5, 10, 12))
 
 
-def _scan_forward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, softplus, return_state, keep=False):
+def _scan_forward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, strides, softplus, return_state, keep=False):
     """(y, state behind the last token or None, checkpoints for the backward or None)"""
     bsz, steps, chans = x.shape
     n = a.shape[1]
     device = x.device
-    y = torch.empty((bsz, steps, chans), dtype=x.dtype, device=device)
+    y = _like(x)
     state_out = torch.empty((bsz, chans, n), dtype=torch.float32, device=device) if return_state else None
     ckpt = ws = None
     if y.numel() > 0:
@@ -1757,10 +1779,9 @@ def _scan_forward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, softplus, re
             if nbytes:
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
             _native.check(lib.afd_state_scan_forward(
-                x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _at(gate),
-                _scan_strides((x, dt, b, c, gate), (0, 1)), a.data_ptr(), _at(d), _at(dt_bias), _at(state), _at(lengths),
-                y.data_ptr(), _at(state_out), _at(ckpt), bsz, steps, chans, n, softplus, _SEQ_DTYPES[x.dtype], _at(ws),
-                nbytes, stream), "afd_state_scan_forward")
+                x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _at(gate), _Strides10(*strides), a.data_ptr(), _at(d),
+                _at(dt_bias), _at(state), _at(lengths), y.data_ptr(), _at(state_out), _at(ckpt), bsz, steps, chans, n,
+                softplus, _SEQ_DTYPES[x.dtype], _at(ws), nbytes, stream), "afd_state_scan_forward")
     elif state_out is not None:
         state_out.copy_(state) if state is not None else state_out.zero_()
     return y, state_out, ckpt
@@ -1768,34 +1789,33 @@ def _scan_forward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, softplus, re
 
 class _StateScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, dt, a, b, c, d, gate, dt_bias, state, lengths, softplus, return_state):
+    def forward(ctx, x, dt, a, b, c, d, gate, dt_bias, state, lengths, strides, softplus, return_state):
         ctx.set_materialize_grads(False)
-        y, state_out, ckpt = _scan_forward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, softplus, return_state, True)
+        y, state_out, ckpt = _scan_forward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, strides, softplus, return_state,
+                                           True)
         ctx.save_for_backward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, ckpt)
-        ctx.softplus = softplus
+        ctx.softplus, ctx.strides = softplus, strides
         return y, state_out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dy, dstate_out):
         x, dt, a, b, c, d, gate, dt_bias, state, lengths, ckpt = ctx.saved_tensors
         bsz, steps, chans = x.shape
         n = a.shape[1]
         need = ctx.needs_input_grad
 
-        def like(t, want=True):
-            return torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and want else None
-
-        grads = [like(t) for t in (x, dt, a, b, c, d, gate, dt_bias)] + [like(state, need[8])]
+        grads = [_like(t) if t is not None else None for t in (x, dt, a, b, c, d, gate, dt_bias)]
+        grads.append(_like(state) if need[8] else None)
         if x.numel() == 0:
             for g in grads:
                 if g is not None:
                     g.zero_()
             if grads[8] is not None and dstate_out is not None:
                 grads[8].copy_(dstate_out)
-            return (*grads, None, None, None)
+            return (*grads, None, None, None, None)
         dx, ddt, da, db, dc, dd, dgate, dbias, dstate = grads
-        dy = _near_rows(dy) if dy is not None else torch.zeros(x.shape, dtype=x.dtype, device=x.device)
+        (dy,), far = _token_rows([dy if dy is not None else torch.zeros(x.shape, dtype=x.dtype, device=x.device)])
         dstate_out = _dense(dstate_out)
         with _OnDevice(x) as stream:
             lib = _lib()
@@ -1803,11 +1823,11 @@ class _StateScan(torch.autograd.Function):
             ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
             _native.check(lib.afd_state_scan_backward(
                 x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _at(gate), dy.data_ptr(),
-                _scan_strides((x, dt, b, c, gate, dy), (0, 1)), a.data_ptr(), _at(d), _at(dt_bias), _at(lengths),
+                _Strides12(*ctx.strides, *far), a.data_ptr(), _at(d), _at(dt_bias), _at(lengths),
                 ckpt.data_ptr(), _at(dstate_out), dx.data_ptr(), ddt.data_ptr(), db.data_ptr(), dc.data_ptr(), _at(dgate),
                 da.data_ptr(), _at(dd), _at(dbias), _at(dstate), bsz, steps, chans, n, ctx.softplus, _SEQ_DTYPES[x.dtype],
                 ws.data_ptr(), nbytes, stream), "afd_state_scan_backward")
-        return (*grads, None, None, None)
+        return (*grads, None, None, None, None)
 
 
 def state_scan(x, dt, a, b, c, d=None, gate=None, dt_bias=None, softplus: bool = False, state=None, lengths=None,
@@ -1825,10 +1845,10 @@ def state_scan(x, dt, a, b, c, d=None, gate=None, dt_bias=None, softplus: bool =
     _scan_check("state_scan", x, dt, a, b, c, d, gate, dt_bias, state, 3)
     lengths = _seq_lengths("state_scan", lengths, x)
     _seq_gpu("state_scan", x)
-    x, dt, b, c, gate = _near_rows(x), _near_rows(dt), _near_rows(b), _near_rows(c), _near_rows(gate)
+    (x, dt, b, c, gate), strides = _token_rows((x, dt, b, c, gate))
     a, d, dt_bias, state = _dense(a), _dense(d), _dense(dt_bias), _dense(state)
     run = _StateScan.apply if _wants_grad(x, dt, a, b, c, d, gate, dt_bias, state) else _scan_forward
-    y, state_out = run(x, dt, a, b, c, d, gate, dt_bias, state, lengths, int(bool(softplus)), bool(return_state))[:2]
+    y, state_out = run(x, dt, a, b, c, d, gate, dt_bias, state, lengths, strides, int(bool(softplus)), bool(return_state))[:2]
     return (y, state_out) if return_state else y
 
 
@@ -1846,7 +1866,8 @@ def state_scan_step(x, state, dt, a, b, c, d=None, gate=None, dt_bias=None, soft
     if y.numel() > 0:
         with _OnDevice(x) as stream:
             _native.check(_lib().afd_state_scan_step(
-                x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _at(gate), _scan_strides((x, dt, b, c, gate), (0,)),
+                x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _at(gate),
+                _Strides5(x.stride(0), dt.stride(0), b.stride(0), c.stride(0), gate.stride(0) if gate is not None else 0),
                 a.data_ptr(), _at(d), _at(dt_bias), state.data_ptr(), y.data_ptr(), into.data_ptr(), x.shape[0], x.shape[1],
                 a.shape[1], int(bool(softplus)), _SEQ_DTYPES[x.dtype], stream), "afd_state_scan_step")
     return y
@@ -1885,15 +1906,15 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, w, b, z = ctx.saved_tensors
         need = ctx.needs_input_grad
         m, k = x.shape
         n = w.shape[0]
-        dx = torch.empty((m, k), dtype=x.dtype, device=x.device) if need[0] else None
-        dw = torch.empty((n, k), dtype=w.dtype, device=x.device) if need[1] else None
-        db = torch.empty_like(b) if need[2] else None
+        dx = _like(x) if need[0] else None
+        dw = _like(w) if need[1] else None
+        db = _like(b) if need[2] else None
         if m == 0:
             for t in (dw, db):
                 if t is not None:
@@ -1938,13 +1959,13 @@ def linear(x, w, b=None, activation: str = "none", residual=None):
     _seq_check(what, "residual", residual, (*x.shape[:-1], n), x.dtype, x.device)
     if activation not in _LINEAR_ACTIVATIONS:
         raise ValueError(f"{what}: activation {activation!r}; one of {sorted(_LINEAR_ACTIVATIONS)} expected")
-    rows = x.reshape(-1, k)
+    rows = x if x.dim() == 2 else x.reshape(-1, k)
     grad = _wants_grad(x, w, b, residual)
     if grad and rows.shape[0] > _LINEAR_GRAD_ROWS:
         raise ValueError(f"{what}: {rows.shape[0]} rows; at most {_LINEAR_GRAD_ROWS} where gradients are wanted")
     _seq_gpu(what, x)
     rows = _rows(rows)
-    res = _rows(residual.reshape(-1, n)) if residual is not None else None
+    res = _rows(residual if x.dim() == 2 else residual.reshape(-1, n)) if residual is not None else None
     w, b = _rows(w), _dense(b)
     if grad:
         y = _Linear.apply(rows, w, b, res, _LINEAR_ACTIVATIONS[activation])

@@ -328,6 +328,19 @@ def test_scan_rows_far_apart_in_memory():
     assert torch.equal(dx, dx2)
 
 
+def test_second_derivatives_are_refused():
+    t = _scan_inputs(11, "fp32", 1, 4, 6, 4)
+    c = _conv_inputs(11, "fp32", 1, 4, 6, 3)
+    x = t["x"].detach().requires_grad_(True)
+    for y in (ops.state_scan(**dict(t, x=x), softplus=True), ops.causal_conv(x, c["w"], c["b"], "silu"),
+              ops.linear(x, torch.ones(5, 6, device="cuda"), activation="silu")):
+        dy = torch.ones_like(y, requires_grad=True)
+        (dx,) = torch.autograd.grad(y, [x], dy, create_graph=True)
+        assert torch.equal(dx, torch.autograd.grad(y, [x], dy)[0])
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            dx.sum().backward()
+
+
 def test_a_state_that_a_backward_pass_needs_is_not_changed_unseen():
     t = _scan_inputs(10, "fp32", 2, 5, 8, 4)
     c = _conv_inputs(10, "fp32", 2, 5, 8, 4, True, True)
