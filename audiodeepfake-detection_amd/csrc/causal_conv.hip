@@ -5,11 +5,11 @@
 //
 // Rows before the first are the `state` (the last W - 1 rows of an earlier part, oldest first) or zero.  Bound by memory:
 // 2 W + 6 flops against one element read and one written, so every element is loaded once: a thread owns V neighbouring
-// channels (16 bytes) and walks over consecutive rows with the W taps' window in registers; rows are loaded several at a
-// time ahead of the window.  The taps come through LDS: 16-byte reads of [channel][tap] rows, one per lane, touched a cache
-// line per lane and made up half of the line traffic.
+// channels (16 bytes; 4 in the backward) and walks over consecutive rows with the W taps' window in registers; rows are
+// loaded several at a time ahead of the window.  The taps come through LDS: 16-byte reads of [channel][tap] rows, one per
+// lane, touched a cache line per lane and made up half of the line traffic.
 // Measured at 4 x 4096 x 2048 bf16, 4 taps: forward 32 us (4.2 TB/s of what it has to move; a large copy runs at 4.9), backward
-// 63 us (3.2 TB/s: taps, two windows and the sums take 198 registers, which leaves two waves per SIMD).
+// 56 us (3.6 TB/s: every 32 rows the W - 1 behind them are walked again).
 #include "seq_common.h"
 
 namespace {
@@ -308,9 +308,13 @@ enum Kind { kFwd, kBwd, kStep };
 
 template <typename T, int W, int V> void launch_t(Kind kind, const ConvArgs& p, unsigned grid, hipStream_t s) {
     const unsigned lds = (unsigned)(p.gx * V * (W + 1) * sizeof(float));
-    if (kind == kFwd) hipLaunchKernelGGL((conv_fwd_kernel<T, W, V>), dim3(grid), dim3(kT), lds, s, p);
-    else if (kind == kBwd) hipLaunchKernelGGL((conv_bwd_kernel<T, W, V>), dim3(grid), dim3(kT), lds, s, p);
-    else hipLaunchKernelGGL((conv_step_kernel<T, W, V>), dim3(grid), dim3(kT), 0, s, p);
+    constexpr bool kWide = V == 1 || V * sizeof(T) == 16;
+    if constexpr (V <= 4)
+        if (kind == kBwd) hipLaunchKernelGGL((conv_bwd_kernel<T, W, V>), dim3(grid), dim3(kT), lds, s, p);
+    if constexpr (kWide) {
+        if (kind == kFwd) hipLaunchKernelGGL((conv_fwd_kernel<T, W, V>), dim3(grid), dim3(kT), lds, s, p);
+        if (kind == kStep) hipLaunchKernelGGL((conv_step_kernel<T, W, V>), dim3(grid), dim3(kT), 0, s, p);
+    }
 }
 
 template <typename T, int V> void launch_w(Kind kind, int W, const ConvArgs& p, unsigned grid, hipStream_t s) {
@@ -326,9 +330,10 @@ template <typename T, int V> void launch_w(Kind kind, int W, const ConvArgs& p, 
 }
 
 int run(Kind kind, ConvArgs& p, int W, int dtype, hipStream_t s) {
-    // Whole sequences take 16 bytes of channels per thread from the width of one such group on.  The step form writes its
-    // state in place, so no channel may be computed twice there: single channels where V does not divide D.
-    int v = (int)(16 / dtype_bytes(dtype));
+    // Whole sequences take 16 bytes of channels per thread from the width of one such group on; backward four channels (with
+    // eight of a 16-bit type its registers leave two waves per SIMD: 63 us against 56 at 4 x 4096 x 2048 bf16).  The step form
+    // writes its state in place, so no channel may be computed twice there: single channels where V does not divide D.
+    int v = kind == kBwd ? 4 : (int)(16 / dtype_bytes(dtype));
     if (kind == kStep ? p.D % v != 0 : p.D < v) v = 1;
     p.groups = (p.D + v - 1) / v;
     size_t grid;
@@ -347,10 +352,12 @@ int run(Kind kind, ConvArgs& p, int W, int dtype, hipStream_t s) {
         if (v > 1) launch_w<float, 4>(kind, W, p, (unsigned)grid, s);
         else launch_w<float, 1>(kind, W, p, (unsigned)grid, s);
     } else if (dtype == AFD_T_BF16) {
-        if (v > 1) launch_w<bf16_t, 8>(kind, W, p, (unsigned)grid, s);
+        if (v == 8) launch_w<bf16_t, 8>(kind, W, p, (unsigned)grid, s);
+        else if (v == 4) launch_w<bf16_t, 4>(kind, W, p, (unsigned)grid, s);
         else launch_w<bf16_t, 1>(kind, W, p, (unsigned)grid, s);
     } else {
-        if (v > 1) launch_w<f16_t, 8>(kind, W, p, (unsigned)grid, s);
+        if (v == 8) launch_w<f16_t, 8>(kind, W, p, (unsigned)grid, s);
+        else if (v == 4) launch_w<f16_t, 4>(kind, W, p, (unsigned)grid, s);
         else launch_w<f16_t, 1>(kind, W, p, (unsigned)grid, s);
     }
     return check_launch("causal_conv kernel");
@@ -358,8 +365,8 @@ int run(Kind kind, ConvArgs& p, int W, int dtype, hipStream_t s) {
 
 // Rows per thread: long tiles repeat fewer rows at their ends (W - 1, both ends backward) and load fewer taps, short ones
 // make more waves.  The longest up to 32 that leaves two waves per SIMD, counted at 8 channels per thread.  4 x 4096 x 2048
-// bf16: backward and the sums behind it 77 + 8 / 63 + 5 us with 16 / 32 rows, forward 33 / 32; 16 x 777 x 1024: forward
-// 17.1 / 19.2 us with 8 / 16 rows.
+// bf16: backward and the sums behind it 56 + 5 / 66 + 5 / 73 + 4 us with 32 / 48 / 64 rows, forward 33 / 32 us with 16 / 32;
+// 16 x 777 x 1024: forward 17.1 / 19.2 us with 8 / 16 rows.
 int tile_rows(int B, int L, int D, int shortest) {
     const double waves = (double)B * L * D / (8 * 64);
     int tile = 32;
