@@ -11,11 +11,11 @@
 // Few tiles: the k axis is split over workgroups, which leave fp32 partial tiles for a second kernel with the same epilogue.
 //
 // Bound by the matrix instructions and what keeps them waiting.  Measured, with the library's product of the same sizes in
-// brackets: bf16 8192 x 8192 x 8192 1172 (1502) TFLOP/s, 16384 x 2048 x 2048 1062 (1384), where the matrix units are busy
-// half of the time (128 KB of LDS leave one workgroup per CU, and two waves per SIMD do not cover each other's barriers);
-// fp32 16384 x 2048 x 2048 135 (147), 12928 x 1024 x 512 111 (108).  Staging 2 or 3 slabs ahead, one wave per SIMD with 128 x 128
-// each, or two workgroups of 128 x 256 per CU were not faster (1113, 958 and 937 at 4096 to 8192 cubed).  A forward with
-// GELU, residual and the fp32 z takes 216 us at 16384 x 2048 x 2048, its input gradient 155: 201 MB more to move and 24 us of
+// brackets: bf16 8192 x 8192 x 8192 1255 (1555) TFLOP/s, 16384 x 2048 x 2048 1124 (1402), where the matrix units are busy
+// three fifths of the time (128 KB of LDS leave one workgroup per CU, and two waves per SIMD do not cover each other's barriers);
+// fp32 16384 x 2048 x 2048 135 (147), 12928 x 1024 x 512 111 (108).  Before the waves' priorities, at 1172:
+// staging 2 or 3 slabs ahead 1164, one wave per SIMD with 128 x 128 each 958, two workgroups of 128 x 256 per CU 958.  A forward with
+// GELU, residual and the fp32 z takes 208 us at 16384 x 2048 x 2048, its input gradient 146: 201 MB more to move and 24 us of
 // arithmetic, which no other workgroup of the CU covers.
 #include "seq_common.h"
 
@@ -267,8 +267,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(const Gemm g) {
     const int arow = wm * (TM / WM) + l31, brow = wn * (TN / WN) + l31;
     // One slab: four steps of 32 bytes of k.  A step's fragments are read while the step before it is multiplied.  The next
     // slab's registers go to LDS between the first three steps' products, each loaded anew at once, so every load has a whole
-    // slab's time to arrive (written in the third step and loaded behind it: 981 TFLOP/s at 16384 x 2048 x 2048 bf16, 1037 like
-    // this); the barrier is passed in front of the last step, whose products cover the next slab's first reads.
+    // slab's time to arrive (written in the third step and loaded behind it: 981 TFLOP/s at 16384 x 2048 x 2048 bf16 where this had
+    // 1037); the barrier is passed in front of the last step, whose products cover the next slab's first reads.
     u32x4 fa[2][MI], fb[2][NI];
     auto read = [&](int buf, int st, int to) {
         const char* base = lds + buf * kBuf;
@@ -278,11 +278,17 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(const Gemm g) {
 #pragma unroll
         for (int j = 0; j < NI; ++j) fb[to][j] = *reinterpret_cast<const u32x4*>(base + TM * kSlab + (brow + j * 32) * kSlab + c);
     };
+    // 16-bit: the products go first at the SIMD while they last, so that two waves take turns instead of waiting for the same
+    // thing (1061 to 1124 TFLOP/s at 16384 x 2048 x 2048); the four times longer fp32 products only get in each other's way (135
+    // to 121).
+    constexpr bool kFirst = sizeof(T) == 2;
     auto multiply = [&](int from) {
+        if constexpr (kFirst) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
             for (int j = 0; j < NI; ++j) mma<T>(fa[from][i], fb[from][j], acc[i][j]);
+        if constexpr (kFirst) __builtin_amdgcn_s_setprio(0);
     };
     // reads, writes and products of a step take turns
     constexpr int kMma = MI * NI * (sizeof(T) == 4 ? 4 : 1);
