@@ -8,7 +8,7 @@
 // of an fp32 or bf16 gradient can leave the range of 32 bits either way.  Every piece has a slot of its own for its sum and
 // one workgroup adds the slots in order: the same bits every time.
 // Measured on 200 bf16 tensors of 300 M elements together: norm 132 us in two launches (4.5 TB/s), scaling 215 us in three
-// (5.6 TB/s).  On 48 small tensors the kernels take 14 us of a call's 69, the rest is the host's.
+// (5.6 TB/s).  On 48 small tensors the kernels take 14 us of a call's 70, the rest is the host's.
 // The scaling pass walks the tensors from the last piece to the first, so it starts on what the norm pass read last, which
 // the 256 MB memory-side cache still holds.
 #include "seq_common.h"

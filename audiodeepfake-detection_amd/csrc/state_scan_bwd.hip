@@ -16,8 +16,8 @@
 // values per lane over 16 channels take 17 instructions instead of 32; the 4 waves meet in LDS, the workgroups in a second
 // small kernel.
 // Bound by vector instruction issue: 25 instructions per token, channel and state, 16 of them the formulas above, the rest
-// broadcasts and sums over lanes.  Measured, 16 states: 128 x 101 x 1024 fp32 240 us (issue 75 % of the time); 4 x 4096 x 2048
-// bf16 in 8 time segments 136 + 528 us (92 and 79 %) + 13 for the workgroups' db and dc + 5 for the parameters' sums.
+// broadcasts and sums over lanes.  Measured, 16 states: 128 x 101 x 1024 fp32 227 us (issue 81 % of the time); 4 x 4096 x 2048
+// bf16 in 8 time segments 136 + 490 us (95 and 89 %) + 13 for the workgroups' db and dc + 5 for the parameters' sums.
 #include "state_scan.h"
 
 namespace {
@@ -246,6 +246,7 @@ __global__ void __launch_bounds__(kScanT, LOCAL ? 4 : kBwdWaves) scan_bwd_kernel
         }
         if (t0 > start) fetch(t0 - TB);
         if constexpr (LOCAL) {
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int j = TB - 1; j >= 0; --j) {
                 const int i = j / Q, ql = j % Q;
@@ -255,7 +256,12 @@ __global__ void __launch_bounds__(kScanT, LOCAL ? 4 : kBwdWaves) scan_bwd_kernel
 #pragma unroll
                 for (int k = 0; k < NS; ++k) X[k] = __builtin_amdgcn_exp2f(de * a2[k]) * fmaf(cv[k], gj, X[k]);
             }
+            __builtin_amdgcn_s_setprio(0);
         } else {
+            // The steps go first at the SIMD, in front of what other waves do between their blocks, and the steps back in front of
+            // those forward: waves take turns instead of moving in step.  545 to 490 us at 4 x 4096 x 2048 bf16; steps back alone
+            // 494, all alike 515.
+            __builtin_amdgcn_s_setprio(1);
             float e[TB][NS], hs[TB][NS], part1[Q], part2[Q];
             float nb[NS], nc[NS];  // the next token's rows, asked for one token ahead
             load_vec<NS>(row, nb);
@@ -286,6 +292,7 @@ __global__ void __launch_bounds__(kScanT, LOCAL ? 4 : kBwdWaves) scan_bwd_kernel
                     own_sum<Q>(y, ql, part1, yv[i]);
                 }
             }
+            __builtin_amdgcn_s_setprio(2);
 #pragma unroll
             for (int j = TB - 1; j >= 0; --j) {
                 const int i = j / Q, ql = j % Q;
@@ -316,6 +323,7 @@ __global__ void __launch_bounds__(kScanT, LOCAL ? 4 : kBwdWaves) scan_bwd_kernel
                 own_sum_down<Q>(s2, ql, part2, s2v[i]);
                 channel_sums<Q, NS>(v, &red[turn][(wave * TS + half + j) * 2 * NP], w.q);
             }
+            __builtin_amdgcn_s_setprio(0);
             loads_arrived();
             T odx[R], odt[R], odg[R];
 #pragma unroll

@@ -1,7 +1,7 @@
 // Forward of the selective state-space scan (see state_scan.h for the formulas and the lane layout).
 // Bound by vector instruction issue: per token, channel and state one exponential (two issue slots), two products and two
-// multiply-adds, 6 slots, against 8 bytes per token and channel.  Measured, 16 states: 128 x 101 x 1024 fp32 84 us, vector
-// issue 89 % of the time; 4 x 4096 x 2048 bf16 in 8 time segments 122 + 184 us, 90 and 85 %; 1 x 16384 x 1024 64 + 96 us.
+// multiply-adds, 6 slots, against 8 bytes per token and channel.  Measured, 16 states: 128 x 101 x 1024 fp32 82 us, vector
+// issue 93 % of the time; 4 x 4096 x 2048 bf16 in 8 time segments 120 + 180 us, 96 and 93 %; 1 x 16384 x 1024 62 + 90 us.
 #include "state_scan.h"
 
 namespace {
@@ -101,6 +101,9 @@ __global__ void __launch_bounds__(kScanT) scan_fwd_kernel(const ScanArgs p) {
             for (int i = 0; i < R; ++i) sum_delta += dl[i];
         }
         if (t0 + kTokF < end) fetch(t0 + kTokF);
+        // The steps go first at the SIMD, in front of what other waves do between their blocks: waves then take turns instead of
+        // moving in step (190 to 182 us at 4 x 4096 x 2048 bf16, 54 to 49 at 16 x 777 x 771 fp16).
+        __builtin_amdgcn_s_setprio(1);
         float part[Q], nb[NS], nc[NS];  // nb, nc: the next token's rows, asked for one token ahead
         load_vec<NS>(row, nb);
         if (!LOCAL) load_vec<NS>(row + NP, nc);
@@ -132,6 +135,7 @@ __global__ void __launch_bounds__(kScanT) scan_fwd_kernel(const ScanArgs p) {
                 if (ql == Q - 1) yv[i] = scatter_lanes<Q>(part);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         if (!LOCAL) {
             loads_arrived();
             T out[R];
@@ -287,8 +291,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 // Time segments: batch and channels give `have` workgroups.  From one per CU on the axis is walked in one piece; below that
 // it is split into about 4 workgroups per CU, in segments of at least 128 tokens, which costs a second, lighter walk.
-// 4 x 4096 x 2048 bf16, 128 workgroups, forward (both walks) / backward (both): 424 / 1018 us in 2 segments, 339 / 688 in 4,
-// 305 / 659 in 8, 305 / 667 in 16; one walk alone at 256 workgroups takes 125 ns a token (backward 385) whatever the split
+// 4 x 4096 x 2048 bf16, 128 workgroups, forward (both walks) / backward (both): 422 / 1011 us in 2 segments, 328 / 629 in 4,
+// 299 / 619 in 8, 297 / 637 in 16; one walk alone at 256 workgroups takes 125 ns a token (backward 385) whatever the split
 // would make of it: 512 us for 4096 tokens against 610 in 4 segments.
 int segments(int B, int nb, int nblk) {
     const long have = (long)B * nb;
