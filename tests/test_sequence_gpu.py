@@ -53,6 +53,9 @@ CONV = [
     ("bf16", 2, 65, 264, 7, "silu", True, True, None, None),
     ("bf16", 1, 5, 16, 8, "silu", True, True, None, None),  # fewer rows than taps
     ("bf16", 2, 64, 513, 4, "silu", True, False, None, None),
+    ("bf16", 3, 41, 5, 4, "silu", True, True, torch.int32, None),  # narrower than 16 bytes of channels
+    ("fp16", 2, 33, 7, 3, "none", True, False, None, "same"),
+    ("bf16", 2, 50, 4, 2, "silu", False, True, None, None),
 ]
 
 
