@@ -1568,6 +1568,8 @@ def _like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+# (Saved tensors are laid out anew in a backward pass: a saved-tensor hook, `save_on_cpu` for one, may give the same values
+# back with other strides.)
 def _first_order(backward):
     """`once_differentiable`, whose two mode switches cost as much as a launch, where a second derivative may be asked for."""
     guarded = torch.autograd.function.once_differentiable(backward)
@@ -1671,6 +1673,7 @@ class _CausalConv(torch.autograd.Function):
     @_first_order
     def backward(ctx, dy, dstate_out):
         x, w, b, state, lengths = ctx.saved_tensors
+        x, w, b, state, lengths = _rows(x), _dense(w), _dense(b), _dense(state), _dense(lengths)
         bsz, steps, d = x.shape
         taps = w.shape[1]
         need = ctx.needs_input_grad
@@ -1794,13 +1797,15 @@ class _StateScan(torch.autograd.Function):
         y, state_out, ckpt = _scan_forward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, strides, softplus, return_state,
                                            True)
         ctx.save_for_backward(x, dt, a, b, c, d, gate, dt_bias, state, lengths, ckpt)
-        ctx.softplus, ctx.strides = softplus, strides
+        ctx.softplus = softplus
         return y, state_out
 
     @staticmethod
     @_first_order
     def backward(ctx, dy, dstate_out):
         x, dt, a, b, c, d, gate, dt_bias, state, lengths, ckpt = ctx.saved_tensors
+        (x, dt, b, c, gate), strides = _token_rows((x, dt, b, c, gate))
+        a, d, dt_bias, lengths, ckpt = _dense(a), _dense(d), _dense(dt_bias), _dense(lengths), _dense(ckpt)
         bsz, steps, chans = x.shape
         n = a.shape[1]
         need = ctx.needs_input_grad
@@ -1823,7 +1828,7 @@ class _StateScan(torch.autograd.Function):
             ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
             _native.check(lib.afd_state_scan_backward(
                 x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), _at(gate), dy.data_ptr(),
-                _Strides12(*ctx.strides, *far), a.data_ptr(), _at(d), _at(dt_bias), _at(lengths),
+                _Strides12(*strides, *far), a.data_ptr(), _at(d), _at(dt_bias), _at(lengths),
                 ckpt.data_ptr(), _at(dstate_out), dx.data_ptr(), ddt.data_ptr(), db.data_ptr(), dc.data_ptr(), _at(dgate),
                 da.data_ptr(), _at(dd), _at(dbias), _at(dstate), bsz, steps, chans, n, ctx.softplus, _SEQ_DTYPES[x.dtype],
                 ws.data_ptr(), nbytes, stream), "afd_state_scan_backward")
@@ -1909,6 +1914,7 @@ class _Linear(torch.autograd.Function):
     @_first_order
     def backward(ctx, dy):
         x, w, b, z = ctx.saved_tensors
+        x, w, z = _rows(x), _rows(w), _dense(z)
         need = ctx.needs_input_grad
         m, k = x.shape
         n = w.shape[0]

@@ -1128,3 +1128,37 @@ def test_trainer_clips_its_gradients(kind):
         moved = _norm64([b - p for b, p in zip(before, params)])
         noise = 2.0 ** -23 * _norm64(before)
         assert abs(moved - 1e-3) <= 1e-3 * 1e-3 + noise
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_gradients_of_views_under_saved_tensor_hooks(dtype):
+    """x | gate and dt | b | c as views of two projections: the gradients are the same bits whether the saved tensors stay
+    where they are, go to the host and back, or come back in another layout."""
+    g = torch.Generator().manual_seed(80)
+    t = TYPES[dtype]
+    d, n, l = 40, 16, 35
+    xz, dbc = _rnd(g, 2, l, 2 * d, dtype=t).requires_grad_(True), _rnd(g, 2, l, d + 2 * n, dtype=t).requires_grad_(True)
+    a, skip, bias = -_rnd(g, d, n).abs(), _rnd(g, d), _rnd(g, d)
+    taps, wide = _rnd(g, d, 4, scale=0.5), _rnd(g, 24, 2 * d, dtype=t)
+    leaves = [xz, dbc, *(p.requires_grad_(True) for p in (a, skip, bias, taps, wide))]
+    dys = [_rnd(g, 2, l, k, dtype=t) for k in (d, d, 24)]
+
+    def run():
+        x, gate = xz.chunk(2, -1)
+        dt, b, c = dbc.split([d, n, n], -1)
+        ys = (ops.state_scan(x, dt, a, b, c, d=skip, gate=gate, dt_bias=bias, softplus=True),
+              ops.causal_conv(x, taps, None, "silu"), ops.linear(gate, wide[:, 8:8 + d], None, "gelu"))
+        return lambda: torch.autograd.grad(ys, leaves, dys)
+
+    want = run()()
+
+    def turned(v):
+        return v.transpose(-1, -2).contiguous().transpose(-1, -2) if v.dim() > 1 else v.clone()
+
+    for hooks in (torch.autograd.graph.save_on_cpu(pin_memory=True),
+                  torch.autograd.graph.saved_tensors_hooks(lambda v: v.clone(memory_format=torch.contiguous_format), lambda v: v),
+                  torch.autograd.graph.saved_tensors_hooks(turned, lambda v: v)):
+        with hooks:
+            backward = run()
+        got = backward()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), hooks

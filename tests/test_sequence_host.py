@@ -312,3 +312,94 @@ def test_c_entries_refuse_more_workgroups_than_a_launch_holds():
                                    64, 1, 0, None) == -3
     assert lib.afd_causal_conv_step(one, 1, one, None, 1, one, one, one, 0x7fffffff, 8, 4, 0, 0, None) == -3
     assert lib.afd_linear_forward(one, 4, one, 4, None, 0, None, 0, one, None, 0x7fffff00, 80, 4, 0, 0, None, 0, None) == -3
+
+
+# ---- what the entry points hand to the library, with the launches stubbed out -------------------------------------------
+class _Launches:
+    """The library with its sizes answered and its launches noted down: (entry, arguments)."""
+
+    def __init__(self, lib):
+        self.lib, self.calls = lib, []
+
+    def __getattr__(self, name):
+        if name.endswith(("_bytes", "_floats")):
+            return getattr(self.lib, name)
+
+        def note(*args):
+            self.calls.append((name, args))
+            return 0
+
+        return note
+
+
+class _NoDevice:
+    def __init__(self, t):
+        pass
+
+    def __enter__(self):
+        return 0
+
+    def __exit__(self, *exc):
+        pass
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    stub = _Launches(_native.load())
+    monkeypatch.setattr(ops, "_lib", lambda: stub)
+    monkeypatch.setattr(ops, "_OnDevice", _NoDevice)
+    monkeypatch.setattr(ops, "_seq_gpu", lambda what, x: None)
+    return stub
+
+
+def _turned(t):
+    """The same values with the last two axes the other way round in memory."""
+    return t.transpose(-1, -2).contiguous().transpose(-1, -2) if t.dim() > 1 else t.clone()
+
+
+@pytest.mark.parametrize("store", [lambda t: t.contiguous() if not t.is_contiguous() else t.clone(), _turned])
+def test_backward_takes_the_layout_of_what_saved_tensor_hooks_give_back(launches, store):
+    """A hook that stores the saved tensors elsewhere may give them back in another layout: the pointers and the strides of a
+    launch have to belong together."""
+    given = {}
+
+    def unpack(t):
+        given[t.data_ptr()] = t
+        return t
+
+    xz = torch.randn(2, 5, 16, requires_grad=True)
+    bcd = torch.randn(2, 5, 14, requires_grad=True)
+    x, gate = xz.chunk(2, -1)
+    dt, b, c = bcd.split([8, 3, 3], -1)
+    wide = torch.randn(6, 16)
+    with torch.autograd.graph.saved_tensors_hooks(store, unpack):
+        scanned = ops.state_scan(x, dt, torch.zeros(8, 3), b, c, gate=gate)
+        conved = ops.causal_conv(x, torch.zeros(8, 4), torch.zeros(8), "silu", state=torch.zeros(2, 3, 8))
+        linear = ops.linear(x, wide[:, 4:12], None, "silu")
+
+    def rows(ptr, shape, strides, name):
+        """Whatever lies at `ptr` with these strides is one of the tensors given back, or a copy of its rows."""
+        t = given.get(ptr)
+        assert t is None or (t.stride(-1) == 1 and t.stride()[:len(strides)] == tuple(strides)), (name, t.stride(), strides)
+        if t is None:  # a copy: rows one behind the other
+            assert strides[-1] == shape[-1], (name, strides)
+
+    keep = []  # (copies made for a launch stay alive through their gradients; addresses are looked at right behind it)
+    launches.calls.clear()
+    keep.append(torch.autograd.grad(scanned.sum(), [xz, bcd], retain_graph=True))
+    (name, args), = [k for k in launches.calls if k[0] == "afd_state_scan_backward"]
+    strides = list(args[6])
+    for i, (what, shape) in enumerate((("x", x.shape), ("dt", dt.shape), ("b", b.shape), ("c", c.shape), ("gate", gate.shape))):
+        rows(args[i], shape, strides[2 * i:2 * i + 2], what)
+    assert args[7] not in given or given[args[7]].is_contiguous()
+    launches.calls.clear()
+    keep.append(torch.autograd.grad(conved.sum(), [xz], retain_graph=True))
+    (name, args), = [k for k in launches.calls if k[0] == "afd_causal_conv_backward"]
+    rows(args[0], x.shape, args[1:3], "x")
+    for i in (3, 6):
+        assert args[i] not in given or given[args[i]].is_contiguous(), i
+    launches.calls.clear()
+    keep.append(torch.autograd.grad(linear.sum(), [xz]))
+    (name, args), = [k for k in launches.calls if k[0] == "afd_linear_backward"]
+    rows(args[0], (10, 8), [args[1]], "x")
+    rows(args[2], (6, 8), [args[3]], "w")
