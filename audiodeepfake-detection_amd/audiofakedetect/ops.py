@@ -14,6 +14,7 @@ from typing import Optional
 
 import torch
 import torch.distributed as dist
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _native
@@ -1519,6 +1520,15 @@ def _seq_gpu(what: str, x) -> None:
         raise RuntimeError(f"{what}: tensors on {x.device}; there is no CPU path")
 
 
+def _no_tangents(what: str, *tensors) -> None:
+    """The kernels have no forward-mode derivative, and an entry point that goes past autograd would drop a tangent."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: an argument carries a forward-mode tangent; there is no forward-mode derivative")
+
+
 class _OnDevice:
     """Launches go to the device of the tensors, whatever the current one is; `with` gives that device's current stream."""
 
@@ -1712,6 +1722,7 @@ def causal_conv(x, w, b=None, activation: str = "none", state=None, lengths=None
     act = _conv_check("causal_conv", x, w, b, activation, 3)
     _seq_check("causal_conv", "state", state, (x.shape[0], w.shape[1] - 1, x.shape[2]), x.dtype, x.device)
     lengths = _seq_lengths("causal_conv", lengths, x)
+    _no_tangents("causal_conv", x, w, b, state)
     _seq_gpu("causal_conv", x)
     x, w, b, state = _rows(x), _dense(w), _dense(b), _dense(state)
     run = _CausalConv.apply if _wants_grad(x, w, b, state) else _conv_forward
@@ -1726,6 +1737,7 @@ def causal_conv_step(x, state, w, b=None, activation: str = "none", state_out=No
     if state is None:
         raise TypeError("causal_conv_step: state has to be a tensor")
     _seq_check("causal_conv_step", "state", state, (x.shape[0], w.shape[1] - 1, x.shape[1]), x.dtype, x.device)
+    _no_tangents("causal_conv_step", x, w, b, state, state_out)
     into = _step_state("causal_conv_step", state, state_out, (x, w, b, state))
     _seq_gpu("causal_conv_step", x)
     x, w, b = _rows(x), _dense(w), _dense(b)
@@ -1849,6 +1861,7 @@ def state_scan(x, dt, a, b, c, d=None, gate=None, dt_bias=None, softplus: bool =
     order of execution.  Training keeps the state in front of every 8 tokens (float32)."""
     _scan_check("state_scan", x, dt, a, b, c, d, gate, dt_bias, state, 3)
     lengths = _seq_lengths("state_scan", lengths, x)
+    _no_tangents("state_scan", x, dt, a, b, c, d, gate, dt_bias, state)
     _seq_gpu("state_scan", x)
     (x, dt, b, c, gate), strides = _token_rows((x, dt, b, c, gate))
     a, d, dt_bias, state = _dense(a), _dense(d), _dense(dt_bias), _dense(state)
@@ -1863,6 +1876,7 @@ def state_scan_step(x, state, dt, a, b, c, d=None, gate=None, dt_bias=None, soft
     if state is None:
         raise TypeError("state_scan_step: state has to be a tensor")
     _scan_check("state_scan_step", x, dt, a, b, c, d, gate, dt_bias, state, 2)
+    _no_tangents("state_scan_step", x, state, dt, a, b, c, d, gate, dt_bias, state_out)
     into = _step_state("state_scan_step", state, state_out, (x, state, dt, a, b, c, d, gate, dt_bias))
     _seq_gpu("state_scan_step", x)
     x, dt, b, c, gate = _rows(x), _rows(dt), _rows(b), _rows(c), _rows(gate)
@@ -1965,6 +1979,7 @@ def linear(x, w, b=None, activation: str = "none", residual=None):
     _seq_check(what, "residual", residual, (*x.shape[:-1], n), x.dtype, x.device)
     if activation not in _LINEAR_ACTIVATIONS:
         raise ValueError(f"{what}: activation {activation!r}; one of {sorted(_LINEAR_ACTIVATIONS)} expected")
+    _no_tangents(what, x, w, b, residual)
     rows = x if x.dim() == 2 else x.reshape(-1, k)
     grad = _wants_grad(x, w, b, residual)
     if grad and rows.shape[0] > _LINEAR_GRAD_ROWS:
@@ -2038,10 +2053,12 @@ def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """Norm of all elements of all `tensors` (float32 / bfloat16 / float16, mixed as they come) as one float32 scalar on their
     device, without a host synchronisation: the root of the sum of squares, taken in float64, or the largest magnitude
     (norm_type inf).  NaN if an element is; zero for an empty list."""
-    table = _NormTable("global_norm", list(tensors), norm_type)
+    tensors = list(tensors)
+    table = _NormTable("global_norm", tensors, norm_type)
     dense = table.dense
     if not dense:
         return torch.zeros(())
+    _no_tangents("global_norm", *tensors)
     _seq_gpu("global_norm", dense[0])
     with _OnDevice(dense[0]) as stream:
         return _launch_norm(table.lay_out(), len(dense), dense[0].device, norm_type, 1.0, 1.0, stream)[0]
@@ -2104,6 +2121,7 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
             table.dense = dense
     if not dense:
         return torch.zeros(())
+    _no_tangents(what, *grads, *into)
     _seq_gpu(what, dense[0])
     n = len(dense)
     arrays = table.lay_out()

@@ -403,3 +403,34 @@ def test_backward_takes_the_layout_of_what_saved_tensor_hooks_give_back(launches
     (name, args), = [k for k in launches.calls if k[0] == "afd_linear_backward"]
     rows(args[0], (10, 8), [args[1]], "x")
     rows(args[2], (6, 8), [args[3]], "w")
+
+
+def _calls_of_every_entry():
+    """name -> (call, tensors): the tensor arguments of each entry point by name, all fit for it."""
+    z = torch.zeros
+    seq = dict(x=z(2, 5, 6), dt=z(2, 5, 6), a=z(6, 4), b=z(2, 5, 4), c=z(2, 5, 4), d=z(6), gate=z(2, 5, 6), dt_bias=z(6),
+               state=z(2, 6, 4))
+    one = {k: t[:, 0] if t.dim() == 3 and k != "state" else t for k, t in seq.items()}
+    return {
+        "causal_conv": (ops.causal_conv, dict(x=z(2, 5, 6), w=z(6, 4), b=z(6), state=z(2, 3, 6))),
+        "causal_conv_step": (ops.causal_conv_step, dict(x=z(2, 6), state=z(2, 3, 6), w=z(6, 4), b=z(6), state_out=z(2, 3, 6))),
+        "state_scan": (ops.state_scan, seq),
+        "state_scan_step": (ops.state_scan_step, dict(one, state_out=z(2, 6, 4))),
+        "linear": (ops.linear, dict(x=z(2, 3, 4), w=z(6, 4), b=z(6), residual=z(2, 3, 6))),
+        "global_norm": (lambda **t: ops.global_norm(list(t.values())), dict(p=z(3), q=z(2, 8)[:, ::2])),
+        "clip_gradients": (lambda p, q, o: ops.clip_gradients([p, q], 1.0, out=[p, o]), dict(p=z(3), q=z(4), o=z(4))),
+    }
+
+
+@pytest.mark.parametrize("entry", sorted(_calls_of_every_entry()))
+def test_forward_mode_tangents_are_refused(launches, entry):
+    """No entry point has a forward-mode derivative: a tangent is refused by name, not dropped."""
+    from torch.autograd import forward_ad
+
+    call, tensors = _calls_of_every_entry()[entry]
+    with forward_ad.dual_level():
+        call(**tensors)  # nothing carries a tangent: an ordinary call
+        for name, t in tensors.items():
+            with pytest.raises(NotImplementedError, match="forward"):
+                call(**dict(tensors, **{name: forward_ad.make_dual(t, torch.ones_like(t))}))
+    call(**tensors)
