@@ -2052,13 +2052,15 @@ def _launch_norm(arrays, n: int, device, norm_type, max_norm: float, scale: floa
 def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """Norm of all elements of all `tensors` (float32 / bfloat16 / float16, mixed as they come) as one float32 scalar on their
     device, without a host synchronisation: the root of the sum of squares, taken in float64, or the largest magnitude
-    (norm_type inf).  NaN if an element is; zero for an empty list."""
+    (norm_type inf).  NaN if an element is; zero for an empty list.  No backward pass."""
     tensors = list(tensors)
     table = _NormTable("global_norm", tensors, norm_type)
     dense = table.dense
     if not dense:
         return torch.zeros(())
     _no_tangents("global_norm", *tensors)
+    if _wants_grad(*tensors):
+        raise RuntimeError("global_norm: the norm has no backward pass: call it under torch.no_grad(), or of detached tensors")
     _seq_gpu("global_norm", dense[0])
     with _OnDevice(dense[0]) as stream:
         return _launch_norm(table.lay_out(), len(dense), dense[0].device, norm_type, 1.0, 1.0, stream)[0]
@@ -2086,7 +2088,8 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     """Scales `grads` by min(1, max_norm / (norm + 1e-6)), norm being their `global_norm`, in place or into the tensors of
     `out` (same shapes and types; in place where an entry is the gradient itself).  Returns the norm in front of the
     scaling, a float32 scalar on the device; nothing waits for it on the host.  With a norm of inf the finite elements become
-    zero and the others NaN (as inf * 0 is); a norm of NaN makes all of them NaN."""
+    zero and the others NaN (as inf * 0 is); a norm of NaN makes all of them NaN.  Autograd records nothing of it, as of an
+    optimizer's step."""
     what = "clip_gradients"
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

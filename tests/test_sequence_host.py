@@ -434,3 +434,14 @@ def test_forward_mode_tangents_are_refused(launches, entry):
             with pytest.raises(NotImplementedError, match="forward"):
                 call(**dict(tensors, **{name: forward_ad.make_dual(t, torch.ones_like(t))}))
     call(**tensors)
+
+
+def test_global_norm_refuses_to_leave_the_graph_unseen(launches):
+    """The norm has no backward pass: of tensors that require grad it is taken under no_grad, or not at all."""
+    p = torch.ones(4, requires_grad=True)
+    for tensors in ([p], [torch.zeros(3), p * 2]):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            ops.global_norm(tensors)
+        with torch.no_grad():
+            assert not ops.global_norm(tensors).requires_grad
+    ops.global_norm([p.detach()])
