@@ -1559,7 +1559,7 @@ def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 def _token_rows(tensors):
     """[B, L, D] tensors as the scan's lanes reach them -- a contiguous last axis, rows at most 2^24 elements apart (16 rows
-    are within 32-bit offsets) -- and their (batch, row) strides."""
+    are within 32-bit offsets; the stride of a single row is never used) -- and their (batch, row) strides."""
     out, strides = [], []
     for t in tensors:
         if t is None:
@@ -1567,8 +1567,12 @@ def _token_rows(tensors):
         else:
             s = t.stride()
             if (s[2] != 1 and t.shape[2] > 1) or s[1] > 1 << 24:
-                t = t.contiguous()
-                s = t.stride()
+                if t.shape[1] == 1:  # (contiguous() may leave this stride alone)
+                    t = _rows(t)
+                    s = (t.stride(0), 0)
+                else:
+                    t = t.contiguous()
+                    s = t.stride()
             strides += s[:2]
         out.append(t)
     return out, strides

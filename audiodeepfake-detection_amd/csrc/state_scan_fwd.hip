@@ -332,10 +332,10 @@ int check(const char* what, int B, int L, int D, int N, int dtype) {
     return AFD_OK;
 }
 
-// the lanes' offsets inside a block of tokens are 32-bit
+// the lanes' offsets inside a block of tokens are 32-bit: 2^24 elements of 4 bytes between rows at most
 int check_rows(const char* what, const long long* st, int n, int dtype) {
     for (int i = 1; i < n; i += 2)
-        if (st[i] < 0 || st[i] * kTokF * (long long)dtype_bytes(dtype) > 0x3fffffffLL)
+        if (st[i] < 0 || st[i] * kTokF * (long long)dtype_bytes(dtype) > 0x40000000LL)
             return fail(AFD_ERR_UNSUPPORTED, "%s: row stride %lld", what, st[i]);
     return AFD_OK;
 }

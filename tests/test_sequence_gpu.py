@@ -1162,3 +1162,30 @@ def test_gradients_of_views_under_saved_tensor_hooks(dtype):
             backward = run()
         got = backward()
         assert all(torch.equal(p, q) for p, q in zip(got, want)), hooks
+
+
+def test_scan_rows_at_the_edge_of_the_lanes_offsets():
+    """fp32 rows exactly 2^24 elements apart, where 16 rows fill the 32-bit offsets, as inputs and as a gradient; and a single
+    frame whose row stride is beyond them and never used."""
+    t = _scan_inputs(81, "fp32", 1, 40, 24, 4)
+    v = t["x"].detach().requires_grad_(True)
+    want = ops.state_scan(**dict(t, x=v), softplus=True)
+    (dx,) = torch.autograd.grad(want, [v], torch.ones_like(want))
+    edge = torch.empty(40 << 24, device="cuda").as_strided((1, 40, 24), (0, 1 << 24, 1))
+    edge.copy_(t["x"])
+    x = edge.detach().requires_grad_(True)
+    y = ops.state_scan(**dict(t, x=x), softplus=True)
+    assert torch.equal(y, want)
+    ones = torch.empty(40 << 24, device="cuda").as_strided((1, 40, 24), (0, 1 << 24, 1)).fill_(1.0)
+    (dx2,) = torch.autograd.grad(y, [x], ones)
+    assert torch.equal(dx, dx2)
+    first = {k: u[:, :1] if u.dim() == 3 and k != "state" else u for k, u in t.items()}
+    far = torch.empty((1 << 25) + 24, device="cuda").as_strided((1, 1, 24), (24, 1 << 25, 1))
+    far.copy_(first["x"])
+    x = far.detach().requires_grad_(True)
+    y = ops.state_scan(**dict(first, x=x), softplus=True)
+    assert torch.equal(y, want[:, :1])
+    (dx2,) = torch.autograd.grad(y, [x], torch.ones_like(far))
+    u = first["x"].detach().clone().requires_grad_(True)
+    (dx,) = torch.autograd.grad(ops.state_scan(**dict(first, x=u), softplus=True), [u], torch.ones_like(y))
+    assert torch.equal(dx, dx2)

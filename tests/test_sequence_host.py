@@ -445,3 +445,32 @@ def test_global_norm_refuses_to_leave_the_graph_unseen(launches):
         with torch.no_grad():
             assert not ops.global_norm(tensors).requires_grad
     ops.global_norm([p.detach()])
+
+
+def test_scan_rows_at_the_edge_of_the_lanes_offsets(launches):
+    """Rows 2^24 elements apart are read as they are, farther ones are copied, and a single row's stride does not count."""
+    lib, t = _native.load(), torch.zeros
+    small = dict(dt=t(1, 2, 8), a=t(8, 3), b=t(1, 2, 3), c=t(1, 2, 3))
+    for far, seen in ((1 << 24, 1 << 24), ((1 << 24) + 1, 8)):
+        x = torch.empty(far + 8).as_strided((1, 2, 8), (0, far, 1))
+        launches.calls.clear()
+        ops.state_scan(x, **small)
+        (name, args), = launches.calls
+        assert args[5][1] == seen and (args[0] == x.data_ptr()) == (seen == far)
+    one = {k: v[:, :1] if v.dim() == 3 else v for k, v in small.items()}
+    x = torch.empty((1 << 25) + 8).as_strided((1, 1, 8), (8, 1 << 25, 1))  # one frame of a time-major batch
+    launches.calls.clear()
+    ops.state_scan(x, **one)
+    (name, args), = launches.calls
+    assert args[0] == x.data_ptr() and args[5][1] <= 1 << 24
+    # the library draws the line where the binding does, for every type (-4: the next check, a missing workspace)
+    import ctypes
+
+    p = ctypes.c_void_p(16)
+    for dtype, size in ((0, 4), (1, 2), (2, 2)):
+        for stride, rc in ((1 << 24, -4), ((1 << 24) * 4 // size + 1, -3)):
+            st = (_native.c_l * 12)(*([0, stride] * 6))
+            assert lib.afd_state_scan_forward(p, p, p, p, None, st, p, None, None, None, None, p, None, None, 1, 16384, 64, 16,
+                                              1, dtype, None, 0, None) == rc, (dtype, stride)
+            assert lib.afd_state_scan_backward(p, p, p, p, None, p, st, p, None, None, None, p, None, p, p, p, p, None, p, None,
+                                               None, None, 1, 16384, 64, 16, 1, dtype, None, 0, None) == rc, (dtype, stride)
