@@ -164,6 +164,17 @@ template <int NS> __device__ __forceinline__ void store_states(float* p, int n0,
         if (live && n0 + k < N) p[n0 + k] = r[k];
 }
 
+// The carry over a time segment: v exp(a sum delta) + e, a2 = a log2 e.  A whole segment's decay leaves the range of fp32 where
+// the value that it multiplies does not (growing decays over a stretch of zeros, a large state that fades): half of it is
+// applied at a time, and no half is infinite, so that zero stays zero as it does token by token.
+template <int NS> __device__ __forceinline__ void carry(const float (&a2)[NS], float sum_delta, const float (&e)[NS], float (&v)[NS]) {
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {
+        const float f = __builtin_amdgcn_exp2f(fminf(0.5f * a2[k] * sum_delta, 127.f));  // (NaN comes in through e)
+        v[k] = fmaf(f, f * v[k], e[k]);
+    }
+}
+
 __device__ __forceinline__ int scan_rows(const int* lengths, int b, int L) {
     if (!lengths) return L;
     const int n = lengths[b];

@@ -147,9 +147,7 @@ __global__ void __launch_bounds__(kScanT, LOCAL ? 4 : kBwdWaves) scan_bwd_kernel
             const size_t at = ((size_t)w.b * p.S + s) * p.D + w.cl;
             float e[NS];
             load_vec<NS>(p.seg_h + at * NP + w.n0, e);
-            const float sd = p.seg_d[at];
-#pragma unroll
-            for (int k = 0; k < NS; ++k) X[k] = fmaf(__builtin_amdgcn_exp2f(a2[k] * sd), X[k], e[k]);
+            carry<NS>(a2, p.seg_d[at], e, X);
         }
         if (!w.live) {  // lanes behind the last channel add nothing to db and dc
 #pragma unroll

@@ -35,9 +35,7 @@ __global__ void __launch_bounds__(kScanT) scan_fwd_kernel(const ScanArgs p) {
                 const size_t at = ((size_t)w.b * p.S + s) * p.D + w.cl;
                 float e[NS];
                 load_vec<NS>(p.seg_h + at * NP + w.n0, e);
-                const float sd = p.seg_d[at];
-#pragma unroll
-                for (int k = 0; k < NS; ++k) h[k] = fmaf(__builtin_amdgcn_exp2f(a2[k] * sd), h[k], e[k]);
+                carry<NS>(a2, p.seg_d[at], e, h);
             }
         }
     }

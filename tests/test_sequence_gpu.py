@@ -1189,3 +1189,39 @@ def test_scan_rows_at_the_edge_of_the_lanes_offsets():
     u = first["x"].detach().clone().requires_grad_(True)
     (dx,) = torch.autograd.grad(ops.state_scan(**dict(first, x=u), softplus=True), [u], torch.ones_like(y))
     assert torch.equal(dx, dx2)
+
+
+@pytest.mark.parametrize("batch", [1, 256])  # the time axis in four segments, and in one piece
+def test_scan_decays_that_leave_the_range_over_a_segment(batch):
+    """Over 128 tokens a decay leaves float32's range in both directions while the states stay inside it: zeros that would
+    grow by 2^184 stay zeros, a state of 1e30 that fades by 2^-160 is still there.  The count of the roundings is that of any
+    scan of this length."""
+    l, d, n = 512, 8, 4
+    g = torch.Generator().manual_seed(82)
+    t = dict(x=torch.zeros(1, l, d), dt=torch.ones(1, l, d), a=torch.ones(d, n), b=torch.rand(1, l, n, generator=g) + 0.5,
+             c=torch.rand(1, l, n, generator=g) + 0.5)
+    t["x"][:, 500:] = torch.randn(1, 12, d, generator=g)
+    dy = torch.zeros(1, l, d)
+    dy[:, :12] = torch.randn(1, 12, d, generator=g)
+
+    def check(t, dy, names, **kw):
+        v = {k: (u.expand(batch, *u.shape[1:]) if u.dim() == 3 else u).cuda().requires_grad_(True) for k, u in t.items()}
+        y = ops.state_scan(**v, **kw)
+        got = dict(zip(names, torch.autograd.grad(y, [v[k] for k in names], dy.expand(batch, l, d).cuda())))
+        want, bound = ref.scan(**t, dy=dy, **kw), ref.scan(**t, dy=dy, absolute=True, **kw)
+        for i in {0, batch - 1}:
+            ref.close(y[i:i + 1], want["y"], bound["y"], 64 + 5 * l, "y")
+            for k in names:
+                ref.close(got[k][i:i + 1], want["d" + k], bound["d" + k], 160 + 12 * l + 1, "d" + k)
+        return y
+
+    check(t, dy, ["x", "dt", "b", "c"])
+    fade = dict(t, x=torch.zeros(1, l, d), dt=torch.full((1, l, d), 0.87), a=-torch.ones(d, n),
+                state=1e30 * (1 + torch.rand(1, d, n, generator=g)))
+    dy = torch.zeros(1, l, d)
+    dy[:, 140] = 1e20
+    y = check(fade, dy, ["c", "state"])
+    assert 1e-25 < float(y[0, 140].min()) and float(y[0, 140].max()) < 1e-15
+    late = torch.zeros(1, l, d)
+    late[:, 300] = 1e30  # 2^100, 2^-117 by the time it has crossed the segment in front of its own
+    check(fade, late, ["x"])
