@@ -2088,9 +2088,19 @@ def _check_disjoint(src, dst, sizes) -> None:
             end_written = hi
 
 
+def _check_behind(back, src, dst, sizes) -> None:
+    """What is copied back into gradients with gaps goes over no other tensor's result (by the gradients' first and last
+    elements: a result inside a gap counts as an overlap)."""
+    for g, t in back:
+        lo = g.data_ptr()
+        hi = lo + (sum((k - 1) * s for k, s in zip(g.shape, g.stride())) + 1) * g.element_size() if g.numel() else lo
+        if any(s != o and n and o < hi and o + n > lo for s, o, n in zip(src, dst, sizes)):
+            raise ValueError("clip_gradients: tensors to be scaled overlap in memory")
+
+
 def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """Scales `grads` by min(1, max_norm / (norm + 1e-6)), norm being their `global_norm`, in place or into the tensors of
-    `out` (same shapes and types; in place where an entry is the gradient itself).  Returns the norm in front of the
+    `out` (same shapes and types; contiguous, or strided as a gradient without gaps, or the gradient itself).  Returns the norm in front of the
     scaling, a float32 scalar on the device; nothing waits for it on the host.  With a norm of inf the finite elements become
     zero and the others NaN (as inf * 0 is); a norm of NaN makes all of them NaN.  Autograd records nothing of it, as of an
     optimizer's step."""
@@ -2102,13 +2112,17 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     table = _NormTable(what, grads, norm_type)
     dense = table.dense
     back = []  # (gradient, dense copy) where the gradient's memory has gaps
+
+    def through_a_copy(g, t):
+        if any(s == 0 and k > 1 for s, k in zip(g.stride(), g.shape)):
+            raise ValueError(f"{what}: a gradient with elements that share memory cannot be scaled in place")
+        back.append((g, t))
+
     if out is None:
         into = dense
         for g, t in zip(grads, dense) if not table.plain else ():
             if t is not g:
-                if any(s == 0 and k > 1 for s, k in zip(g.stride(), g.shape)):
-                    raise ValueError(f"{what}: a gradient with elements that share memory cannot be scaled in place")
-                back.append((g, t))
+                through_a_copy(g, t)
     else:
         into = list(out)
         if len(into) != len(grads):
@@ -2119,11 +2133,14 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
         if not (table.plain and [o.dtype for o in into] == table.dtypes and [o.shape for o in into] == [g.shape for g in grads]
                 and all([o.is_contiguous() for o in into]) and len({o.get_device() for o in (*into, *grads[:1])}) <= 1):
             dense = list(dense)
-            for i, (o, t) in enumerate(zip(into, dense)):
+            for i, (o, t, g) in enumerate(zip(into, dense, grads)):
                 _seq_check(what, f"out[{i}]", o, t.shape, t.dtype, t.device)
-                if not (o.is_contiguous() and t.is_contiguous()) and o.stride() != t.stride():
+                if t is not g and o.data_ptr() == g.data_ptr() and o.stride() == g.stride():
+                    through_a_copy(o, t)
+                    into[i] = t
+                elif not (o.is_contiguous() and t.is_contiguous()) and o.stride() != t.stride():
                     if not o.is_contiguous():
-                        raise ValueError(f"{what}: out[{i}] has to be contiguous, or strided as its gradient")
+                        raise ValueError(f"{what}: out[{i}] has to be contiguous, strided as its gradient without gaps, or it")
                     dense[i] = t.detach().contiguous()
             table.dense = dense
     if not dense:
@@ -2134,6 +2151,8 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     arrays = table.lay_out()
     dst = table.ptrs if out is None else [t.data_ptr() for t in into]
     _check_disjoint(table.ptrs, dst, table.sizes())
+    if out is not None and back:
+        _check_behind(back, table.ptrs, dst, table.sizes())
     increment_version(into)
     with _OnDevice(dense[0]) as stream:
         stats = _launch_norm(arrays, n, dense[0].device, norm_type, max_norm, 1.0, stream)

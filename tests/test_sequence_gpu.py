@@ -1225,3 +1225,19 @@ def test_scan_decays_that_leave_the_range_over_a_segment(batch):
     late = torch.zeros(1, l, d)
     late[:, 300] = 1e30  # 2^100, 2^-117 by the time it has crossed the segment in front of its own
     check(fade, late, ["x"])
+
+
+def test_clip_gradients_out_may_be_a_gradient_with_gaps():
+    """`out` in place where an entry is the gradient itself, gaps or not, beside entries that are not."""
+    base = torch.randn(50, 7, generator=torch.Generator().manual_seed(3)).cuda()
+    for view in (lambda t: t[:, :3], lambda t: t[::2], lambda t: t.t()[1:4], lambda t: t):
+        t, other = base.clone(), torch.randn(33, generator=torch.Generator().manual_seed(4)).cuda()
+        kept, far = other.clone(), torch.zeros(33, device="cuda")
+        g = view(t)
+        want = t.clone()
+        version = g._version
+        norm = ops.clip_gradients([view(want), kept.clone()], 0.5)
+        got = ops.clip_gradients([g, other], 0.5, out=[g, far])
+        assert torch.equal(got, norm) and torch.equal(t, want) and torch.equal(other, kept) and g._version > version
+        factor = 0.5 / (float(norm) + 1e-6)
+        ref.close(far, kept.cpu().double() * factor, kept.cpu().double(), 4, "beside it")

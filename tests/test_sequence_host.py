@@ -474,3 +474,22 @@ def test_scan_rows_at_the_edge_of_the_lanes_offsets(launches):
                                               1, dtype, None, 0, None) == rc, (dtype, stride)
             assert lib.afd_state_scan_backward(p, p, p, p, None, p, st, p, None, None, None, p, None, p, p, p, p, None, p, None,
                                                None, None, 1, 16384, 64, 16, 1, dtype, None, 0, None) == rc, (dtype, stride)
+
+
+def test_clip_out_in_place_with_gaps(launches):
+    base = torch.arange(24.0).view(4, 6)
+    g = base[:, :3]
+    ops.clip_gradients([g], 1.0, out=[g])  # (the launches are noted, not run: a factor of one)
+    assert [name for name, _ in launches.calls] == ["afd_global_norm", "afd_multi_scale"]
+    assert torch.equal(base, torch.arange(24.0).view(4, 6))
+    ops.clip_gradients([g, torch.zeros(4, 3)], 1.0, out=[base[:, :3], torch.zeros(4, 3)])  # another view of the same elements
+    with pytest.raises(ValueError, match="share memory"):
+        wide = torch.zeros(4, 1).expand(4, 3)
+        ops.clip_gradients([wide], 1.0, out=[wide])
+    with pytest.raises(ValueError, match="overlap"):  # the other gradient would be written over with what is copied back
+        ops.clip_gradients([g, torch.zeros(6)], 1.0, out=[g, base[1]])
+    for other in (base[:, 3:], torch.zeros(4, 6)[:, 3:]):
+        with pytest.raises(ValueError, match="gaps"):
+            ops.clip_gradients([g], 1.0, out=[other])
+    with pytest.raises(ValueError, match="gaps"):
+        ops.clip_gradients([torch.zeros(4, 3)], 1.0, out=[base[:, 3:]])
