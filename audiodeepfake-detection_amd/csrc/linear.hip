@@ -716,6 +716,7 @@ struct Shape {
     int kind;
     int tm, tn, S, ksplit;
     size_t part;
+    double issued;  // flops with the tiles' padding
 };
 enum { kFew16, kFew32, kTile32x128, kTile64, kTile128x64, kTile128, kTile256 };
 constexpr int kLong = 32;                         // slabs of a split that its workgroup's prologue and the joining are small against
@@ -765,6 +766,7 @@ Shape gemm_shape(int M, int N, int K, int dtype) {
     s.ksplit = ceil_div(slabs, want);
     s.S = ceil_div(slabs, s.ksplit);
     s.part = s.S > 1 ? align256((size_t)s.S * M * pad_to(N, 8) * 4) : 0;
+    s.issued = 2.0 * s.tm * (s.kind == kFew16 && M <= 16 ? 16 : rows) * s.tn * cols * slabs * (kSlab / (int)dtype_bytes(dtype));
     return s;
 }
 
@@ -877,7 +879,9 @@ extern "C" int afd_linear_forward(const void* x, long long ldx, const void* w, l
     const size_t need = afd_linear_workspace_bytes(x, ldx, w, ldw, M, N, K, dtype);
     if (need > 0 && (!ws || ws_bytes < need)) return fail(AFD_ERR_WORKSPACE, "linear: workspace of %zu bytes, %zu needed", ws_bytes, need);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    ScopedTiming timing(AFD_K_SEQUENCE, 2.0 * (double)M * N * K, s);
+    ScopedTiming timing(AFD_K_LINEAR, 2.0 * (double)M * N * K, s);
+    timing.issued(gemm_shape((int)M, N, (int)kp, dtype).issued);
+    timing.bytes((double)e * ((double)M * K + (double)N * K + (double)M * N * (residual ? 2 : 1)) + (z ? 4.0 * M * N : 0.0));
     Arena ar{static_cast<char*>(ws), 0};
     PadJob jobs[2];
     int n = 0;
@@ -938,7 +942,10 @@ extern "C" int afd_linear_backward(const void* x, long long ldx, const void* w, 
     if (!ws || ws_bytes < b.total)
         return fail(AFD_ERR_WORKSPACE, "linear backward: workspace of %zu bytes, %zu needed", ws_bytes, b.total);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    ScopedTiming timing(AFD_K_SEQUENCE, 2.0 * (double)M * N * K * ((dx != nullptr) + (dw != nullptr)), s);
+    ScopedTiming timing(AFD_K_LINEAR, 2.0 * (double)M * N * K * ((dx != nullptr) + (dw != nullptr)), s);
+    timing.issued((dx ? gemm_shape((int)M, K, (int)b.np, dtype).issued : 0.0) + (dw ? gemm_shape(N, K, (int)b.mp, dtype).issued : 0.0));
+    timing.bytes((double)dtype_bytes(dtype) * ((double)M * N + (dx ? (double)N * K + (double)M * K : 0.0) +
+                                               (dw ? (double)M * K + (double)N * K : 0.0)) + (act != kNone ? 4.0 * M * N : 0.0));
     Arena ar{static_cast<char*>(ws), 0};
     void* dz = ar.take(b.dz);
     void* dzt = ar.take(b.dzt);

@@ -58,7 +58,8 @@ int afd_version(void);
 #define AFD_K_CONV1X1 11    /* 1x1 convolutions forward / backward-data: GEMMs at 16 flop per byte, HBM-leaning;
                                work = direct-form flops, issued = the same with tile padding, bytes = tensors once */
 #define AFD_K_SEQUENCE 12   /* causal convolution, state-space scan, global norm / gradient scaling: work = bytes */
-#define AFD_K_COUNT 13
+#define AFD_K_LINEAR 13     /* afd_linear_*: work = flops, issued = the same with tile padding, bytes = tensors once */
+#define AFD_K_COUNT 14
 
 /* Element types of the entry points that take more than fp32 */
 #define AFD_T_F32 0

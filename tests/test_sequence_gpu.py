@@ -1241,3 +1241,32 @@ def test_clip_gradients_out_may_be_a_gradient_with_gaps():
         assert torch.equal(got, norm) and torch.equal(t, want) and torch.equal(other, kept) and g._version > version
         factor = 0.5 / (float(norm) + 1e-6)
         ref.close(far, kept.cpu().double() * factor, kept.cpu().double(), 4, "beside it")
+
+
+def test_timing_classes_add_like_to_like():
+    """"sequence" sums bytes, "linear" flops (issued: with the tiles' padding) and the bytes of its tensors."""
+    from audiofakedetect import _native
+
+    x = torch.ones(1, 70, 40, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    w, taps = torch.ones(30, 40, device="cuda", dtype=torch.bfloat16).requires_grad_(True), torch.ones(40, 4, device="cuda")
+    few = torch.ones(9, 40, device="cuda", dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    _native.timing_reset()
+    _native.timing_enable(True)
+    try:
+        with torch.no_grad():
+            ops.causal_conv(x, taps)
+            ops.linear(few, w)
+        y = ops.linear(x, w, None, "silu")
+        torch.autograd.grad(y, [x, w], torch.ones_like(y))
+        torch.cuda.synchronize()
+        seq, lin = _native.timing_collect("sequence"), _native.timing_collect("linear")
+    finally:
+        _native.timing_enable(False)
+        _native.timing_reset()
+    assert seq["launches"] == 1 and seq["work"] == seq["bytes"] == 2 * 2 * 70 * 40 and seq["issued"] == 0
+    assert lin["launches"] == 3 and lin["work"] == 2.0 * 30 * 40 * (9 + 3 * 70)
+    # 16 x 32 x 64 for the few rows; 64 x 64 tiles forward and for dx, 128 x 64 x 64; dw has few rows again, 32 x 48 x 128
+    assert lin["issued"] == 2.0 * (16 * 32 * 64 + 2 * 128 * 64 * 64 + 32 * 48 * 128)
+    xs, ws, ys = 70 * 40, 30 * 40, 70 * 30
+    assert lin["bytes"] == 2.0 * (9 * 40 + ws + 9 * 30) + 2.0 * (xs + ws + ys) + 4.0 * ys + 2.0 * (ys + 2 * (xs + ws)) + 4.0 * ys
