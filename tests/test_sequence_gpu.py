@@ -1270,3 +1270,27 @@ def test_timing_classes_add_like_to_like():
     assert lin["issued"] == 2.0 * (16 * 32 * 64 + 2 * 128 * 64 * 64 + 32 * 48 * 128)
     xs, ws, ys = 70 * 40, 30 * 40, 70 * 30
     assert lin["bytes"] == 2.0 * (9 * 40 + ws + 9 * 30) + 2.0 * (xs + ws + ys) + 4.0 * ys + 2.0 * (ys + 2 * (xs + ws)) + 4.0 * ys
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_linear_gelu_tails_are_right_to_the_types_last_bit(dtype):
+    """GELU of a negative z is z times a tail that falls to 1e-32 over the range: relative to that value the result is off by
+    its rounding, half a step, and by what float32 leaves in front of it -- 2e-6 (fit and polynomial), and the exponent's three
+    roundings, 1.5 z^2 2^-24.  The slope is a difference of two such terms, Phi + z pdf, and its error is theirs."""
+    t = TYPES[dtype]
+    z = torch.cat([torch.linspace(-12, 9, 4001), torch.linspace(-6, -3, 3000)]).to(t)
+    x = z[:, None].cuda().requires_grad_(True)
+    w = torch.ones(1, 1, dtype=t, device="cuda")
+    y = ops.linear(x, w, None, "gelu")
+    (dx,) = torch.autograd.grad(y, [x], torch.ones_like(y))
+    z = z.double()[:, None]
+    cdf, pdf = 0.5 * torch.erfc(-z * 0.5 ** 0.5), torch.exp(-0.5 * z * z) / (2 * torch.pi) ** 0.5
+    inexact = 2e-6 + 1.5 * z * z * 2.0 ** -24
+    least = 2.0 ** -25 if dtype == "fp16" else 0.0  # half of the smallest number
+    half = ref.HALF_STEP[t]
+    for got, want, terms in ((y, z * cdf, (z * cdf).abs()), (dx, cdf + z * pdf, cdf + (z * pdf).abs())):
+        tol = half * want.abs() + inexact * terms * (1 + half) + least
+        over = (got.detach().cpu().double() - want).abs() - tol
+        i = int(over.argmax())
+        assert float(over.max()) <= 0, (float(z[i]), float(got[i]), float(want[i]))
+    assert dtype == "fp16" or bool(y[:100].detach().any())
