@@ -1309,3 +1309,45 @@ def test_parameter_gradients_of_more_columns_than_a_launch_holds():
     assert torch.equal(y.detach(), x)
     dw, db = torch.autograd.grad(y, [w, b], dy)
     assert torch.equal(db, dy[0, 0]) and torch.equal(dw[:, 1], (dy * x)[0, 0]) and not dw[:, 0].any()
+
+
+@pytest.mark.parametrize("dtype, m, k, n, act, bias, residual", [
+    ("bf16", 32, 4104, 8200, "relu", "fp32", False),  # few rows, 32 columns at a time: whole slabs, a k tail, a column tail
+    ("bf16", 19, 4104, 8200, "silu", "same", True),
+    ("fp16", 32, 2048, 8192, "none", None, False),
+    ("fp16", 25, 1000, 16421, "gelu", "fp32", True),  # ... k not split, rows copied
+    ("fp16", 140, 513, 250, "relu", "fp32", True),
+    ("fp32", 130, 100, 257, "relu", "fp32", True),
+])
+def test_linear_on_inputs_as_they_are(dtype, m, k, n, act, bias, residual):
+    """As test_linear_forward_and_gradients, of x as it is drawn: where z is within its rounding errors of relu's corner, the
+    gradient that comes in is zero instead.  (y is continuous there.)  Tolerances are those of that test."""
+    g = torch.Generator().manual_seed(m + k + n)
+    t = TYPES[dtype]
+    v = dict(x=_rnd(g, m, k, dtype=t), w=_rnd(g, n, k, scale=k ** -0.5, dtype=t),
+             b=None if bias is None else _rnd(g, n, dtype=t if bias == "same" else torch.float32),
+             residual=_rnd(g, m, n, dtype=t) if residual else None)
+    dy = _rnd(g, m, n, dtype=t)
+    if act == "relu":
+        near = ref.linear(v["x"], v["w"], v["b"])["z"].abs() < 1e-3
+        assert float(near.double().mean()) < 0.01
+        dy[near.cuda()] = 0
+    for x in v.values():
+        if x is not None:
+            x.requires_grad_(True)
+    y = ops.linear(v["x"], v["w"], v["b"], act, residual=v["residual"])
+    with torch.no_grad():
+        assert torch.equal(ops.linear(v["x"], v["w"], v["b"], act, residual=v["residual"]), y)
+    names = [key for key, x in v.items() if x is not None]
+    grads = dict(zip(names, torch.autograd.grad(y, [v[key] for key in names], dy)))
+    want, bound = ref.linear(**v, act=act, dy=dy), ref.linear(**v, act=act, dy=dy, absolute=True)
+    ref.close(y, want["y"], bound["y"], k + 10, "y")
+    dz_err = ref.HALF_STEP[t] * want["dz"].abs()
+    xa, wa = v["x"].detach().cpu().double().abs(), v["w"].detach().cpu().double().abs()
+    extra = {"x": dz_err @ wa, "w": dz_err.t() @ xa, "b": 0}
+    for name in names:
+        if name == "residual":
+            assert torch.equal(grads[name], dy)
+        else:
+            e = torch.as_tensor(extra[name])
+            ref.close(grads[name], want["d" + name], bound["d" + name] * (m + n + k + 20) + e * 2.0 ** 24, 1, "d" + name)
