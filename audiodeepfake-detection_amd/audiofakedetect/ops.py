@@ -1862,7 +1862,9 @@ def state_scan(x, dt, a, b, c, d=None, gate=None, dt_bias=None, softplus: bool =
     a [D, N], 1 <= N <= 64, d [D], dt_bias [D] and `state` [B, D, N] float32.  gate, d, dt_bias and state may be absent.
     `lengths` and `return_state` as `causal_conv`'s; the state is float32.  Differentiable in every tensor but lengths; the
     recurrence and all sums in float32, results rounded once to the type of their tensor.  Gradients do not depend on the
-    order of execution.  Training keeps the state in front of every 8 tokens (float32)."""
+    order of execution.  Training keeps the state in front of every 8 tokens (float32); the backward pass computes every
+    gradient, wanted or not, in a workspace of 8 N ceil(D / 64) bytes per token and more (N rounded up to 4, 8, 16, 32 or
+    64; D / 32 and D / 16 above 16 and 32 states)."""
     _scan_check("state_scan", x, dt, a, b, c, d, gate, dt_bias, state, 3)
     lengths = _seq_lengths("state_scan", lengths, x)
     _no_tangents("state_scan", x, dt, a, b, c, d, gate, dt_bias, state)
@@ -1961,7 +1963,7 @@ def linear(x, w, b=None, activation: str = "none", residual=None):
     float16), b [N] float32 or of that type; `activation` "none", "relu", "silu" or "gelu" (with the error function).  float32
     products are exact, all sums are float32, the result is rounded once.  Differentiable in every tensor; the backward
     keeps x @ w.T + b in float32 for the activation's slope, rounds the gradient to the type of x in front of its two
-    products (not for b's), and takes at most 8 million rows."""
+    products (not for b's), and takes at most 8 million rows.  K and N up to 2^20 - 64."""
     what = "linear"
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what}: x is a {type(x).__name__}, not a tensor")

@@ -639,7 +639,10 @@ template <typename T> __global__ void __launch_bounds__(256) pad_kernel(const Pa
 }
 
 // dz = dy act'(z) as rows (ldz, zeros behind N) and turned (ldt, zeros behind M), and its column sums over the tile's rows;
-// NULL: not wanted.
+// NULL: not wanted.  The rows are rounded to T: the matrix instructions take 16-bit operands, and two of them for one dz (its
+// rounding's remainder as the second) would double both products, 255 of 533 us at 16384 x 2048 x 2048 bf16.  It is the rounding that an
+// activation's gradient has wherever it is a tensor of its own; dx and dw of that case are off by 2.35e-3 (root mean
+// square) with it, by 1.66e-3, their own rounding, without.  The column sums are of the unrounded dz.
 struct DzJob {
     const void* dy;
     const float* z;

@@ -20,8 +20,9 @@ inline bool dtype_ok(int dtype) { return dtype == AFD_T_F32 || dtype == AFD_T_BF
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// 1 / (1 + exp(-x)): the hardware's base-2 exponential and reciprocal, 1 ulp each.  exp overflows to inf for x < -88 and
-// the reciprocal of that is 0, which is the limit.
+// 1 / (1 + exp(-x)): the hardware's base-2 exponential and reciprocal, 1 ulp each, and the rounding of the exponent's product,
+// 2^-24 |x| of the result for x << 0 (5e-6 at x = -80).  exp overflows to inf for x < -88 and the reciprocal of that is 0, which
+// is the limit.
 __device__ __forceinline__ float sigmoid_f32(float x) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * x));
 }

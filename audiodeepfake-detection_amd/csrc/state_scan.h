@@ -242,8 +242,9 @@ template <typename T, int Q, int TOK> struct TokLoad {
 // stores of the one before it would wait for those too when it takes its loaded values, so the wait comes in front of them.
 __device__ __forceinline__ void loads_arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
-// No LDS access moves across: left to itself the compiler puts each token's rows right in front of their use and waits for
-// them there, once or twice a token.
+// No instruction moves across, LDS accesses among them, which is what it is for: left to itself the compiler puts each token's
+// rows right in front of their use and waits for them there, once or twice a token.  It also keeps the next token's
+// exponentials, which do not depend on the state, behind this token's chain.
 __device__ __forceinline__ void hold_lds() { __builtin_amdgcn_sched_barrier(0); }
 
 struct ScanPlace {
