@@ -164,6 +164,13 @@ template <int NS> __device__ __forceinline__ void store_states(float* p, int n0,
         if (live && n0 + k < N) p[n0 + k] = r[k];
 }
 
+// a log2 e, finite from below: a of -inf forgets the state at every token, and tokens that only hold it (padding in the last block,
+// lanes behind the last channel: delta = 0) would make 0 x inf of it.
+__device__ __forceinline__ float log2_decay(float a) {
+    const float v = a * kLog2e;
+    return v < -3.402823466e38f ? -3.402823466e38f : v;
+}
+
 // The carry over a time segment: v exp(a sum delta) + e, a2 = a log2 e.  A whole segment's decay leaves the range of fp32 where
 // the value that it multiplies does not (growing decays over a stretch of zeros, a large state that fades): half of it is
 // applied at a time, and no half is infinite, so that zero stays zero as it does token by token.

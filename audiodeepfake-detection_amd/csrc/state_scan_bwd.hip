@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kScanT, LOCAL ? 4 : kBwdWaves) scan_bwd_kernel
     load_states<NS>(p.a + (size_t)w.cl * p.N, w.n0, p.N, true, a2);
 #pragma unroll
     for (int k = 0; k < NS; ++k) {
-        a2[k] *= kLog2e;
+        a2[k] = log2_decay(a2[k]);
         X[k] = da[k] = 0.f;
     }
     const int last = w.n > 0 ? (w.n - 1) / p.seg : 0;  // the segment with the last token

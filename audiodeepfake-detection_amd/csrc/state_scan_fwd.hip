@@ -25,7 +25,7 @@ __global__ void __launch_bounds__(kScanT) scan_fwd_kernel(const ScanArgs p) {
     load_states<NS>(p.a + (size_t)w.cl * p.N, w.n0, p.N, true, a2);
 #pragma unroll
     for (int k = 0; k < NS; ++k) {
-        a2[k] *= kLog2e;
+        a2[k] = log2_decay(a2[k]);
         h[k] = 0.f;
     }
     if (!LOCAL) {

@@ -1351,3 +1351,21 @@ def test_linear_on_inputs_as_they_are(dtype, m, k, n, act, bias, residual):
         else:
             e = torch.as_tensor(extra[name])
             ref.close(grads[name], want["d" + name], bound["d" + name] * (m + n + k + 20) + e * 2.0 ** 24, 1, "d" + name)
+
+
+@pytest.mark.parametrize("l, d", [(13, 5), (400, 70)])  # in one piece, and in time segments
+def test_scan_of_states_that_forget_at_once(l, d):
+    """a = -inf (minus the exponential of a large logarithm): every token clears the state, as with any finite a far below.
+    Padding and the lanes behind the last channel, which hold their state by a step of zero, stay what they are."""
+    t = _scan_inputs(84, "fp32", 2, l, d, 6)
+    lengths = torch.tensor([l - 3, l], device="cuda")
+    far = dict(t, a=t["a"].clone())
+    far["a"][0, 1], far["a"][d - 1] = -1e30, -1e30
+    outs = []
+    for a in (far["a"], torch.where(far["a"] < -1e29, torch.full_like(far["a"], -float("inf")), far["a"])):
+        v = {k: u.detach().requires_grad_(True) for k, u in dict(far, a=a).items()}
+        y, state = ops.state_scan(**v, softplus=True, lengths=lengths, return_state=True)
+        grads = torch.autograd.grad([y, state], list(v.values()), [torch.ones_like(y), torch.ones_like(state)])
+        outs.append([y.detach(), state.detach(), *grads])
+    for got, want in zip(*outs):
+        assert bool(torch.isfinite(want).all()) and torch.equal(got, want)
