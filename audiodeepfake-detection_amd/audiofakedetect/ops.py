@@ -2065,7 +2065,7 @@ def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     if not dense:
         return torch.zeros(())
     _no_tangents("global_norm", *tensors)
-    if _wants_grad(*tensors):
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
         raise RuntimeError("global_norm: the norm has no backward pass: call it under torch.no_grad(), or of detached tensors")
     _seq_gpu("global_norm", dense[0])
     with _OnDevice(dense[0]) as stream:
