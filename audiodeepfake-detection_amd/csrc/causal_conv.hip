@@ -249,6 +249,10 @@ __global__ void __launch_bounds__(kT) conv_bwd_kernel(const ConvArgs p) {
 #pragma unroll
                         for (int i = 0; i < V; ++i) out[i] += e[i];
                     }
+                    if (at >= n) {  // (no product of zeros: a tap need not be finite)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) out[i] = 0.f;
+                    }
                     if (at >= 0) {
                         store_row<T, V>(static_cast<T*>(p.dx) + ((size_t)b * p.L + at) * p.D + c, out);
                     } else if (p.dstate) {

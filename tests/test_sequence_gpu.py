@@ -1369,3 +1369,16 @@ def test_scan_of_states_that_forget_at_once(l, d):
         outs.append([y.detach(), state.detach(), *grads])
     for got, want in zip(*outs):
         assert bool(torch.isfinite(want).all()) and torch.equal(got, want)
+
+
+def test_conv_padding_has_zero_gradients_whatever_the_taps_are():
+    t = _conv_inputs(85, "bf16", 3, 50, 24, 4)
+    lengths = torch.tensor([50, 33, 0], device="cuda")
+    x, w = t["x"].requires_grad_(True), t["w"].clone()
+    w[3, 1], w[7, 0] = float("inf"), float("nan")
+    dy = torch.ones(3, 50, 24, device="cuda", dtype=torch.bfloat16)
+    (dx,) = torch.autograd.grad(ops.causal_conv(x, w, t["b"], lengths=lengths), [x], dy)
+    assert not dx[1, 33:].any() and not dx[2].any()
+    (want,) = torch.autograd.grad(ops.causal_conv(x, t["w"], t["b"], lengths=lengths), [x], dy)
+    keep = [i for i in range(24) if i not in (3, 7)]
+    assert torch.equal(dx[..., keep], want[..., keep])
