@@ -2102,10 +2102,10 @@ def _check_behind(back, src, dst, sizes) -> None:
 
 def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """Scales `grads` by min(1, max_norm / (norm + 1e-6)), norm being their `global_norm`, in place or into the tensors of
-    `out` (same shapes and types; contiguous, or strided as a gradient without gaps, or the gradient itself).  Returns the norm in front of the
-    scaling, a float32 scalar on the device; nothing waits for it on the host.  With a norm of inf the finite elements become
-    zero and the others NaN (as inf * 0 is); a norm of NaN makes all of them NaN.  Autograd records nothing of it, as of an
-    optimizer's step."""
+    `out` (same shapes and types; contiguous, or strided as a gradient without gaps, or the gradient itself).  Returns the
+    norm in front of the scaling, a float32 scalar on the device; nothing waits for it on the host.  With a norm of inf the
+    finite elements become zero and the others NaN (as inf * 0 is); a norm of NaN makes all of them NaN.  Autograd records
+    nothing of it, as of an optimizer's step."""
     what = "clip_gradients"
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
